@@ -1,0 +1,540 @@
+"""What the long-context operators are timed and compared on: attention of
+ragged chunks over the paged cache with a sliding window and sinks, the
+attention weight each cached key gathers, and the eviction of the lightest
+keys into fresh pages.
+
+Kinds of case (``case["kind"]``) and the ranges draw() takes them from. Head
+shapes are those of the models the repository's benchmark and configurations
+name (Qwen3-0.6B, Qwen3-8B, Qwen2.5-0.5B, Qwen2.5-7B).
+
+attn   a step's attention in ``layers`` layers (rlse_chunk_plan once, then
+       rlse_chunk_attn per layer): every sequence attends its new tokens -- one
+       of a decode step, a few of a speculative one, or a chunk of a prompt --
+       to its cached keys and to the new ones up to their own, all of them or
+       the last ``window`` and the first ``sinks``. 1 to 64 sequences, 1 to
+       4096 new tokens after 0 to 65536 cached ones, bf16, f16 and f32.
+score  the weight every key receives from the step's queries, summed over the
+       queries and heads that share its KV head (rlse_kv_scores), added to what
+       it had (``prev``) or counted anew. Same ranges, up to 2048 new tokens.
+evict  the cut of every layer's cache to ``budget`` keys a head: the first
+       ``sinks``, the last ``recent`` and the heaviest between them, moved to
+       fresh pages (rlse_kv_evict). 1 to 28 layers, 1 to 32 sequences, 64 to
+       16384 cached keys, bf16, f16 and f32.
+"""
+import math
+import os
+import sys
+
+import torch
+
+own = False
+
+DEV = "cuda:0"
+TORCH = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+BYTES = {"f32": 4, "bf16": 2, "f16": 2}
+
+# name: (query heads, KV heads, head_dim)
+HEADS = {
+    "qwen3_0_6b": (16, 8, 128),
+    "qwen2_5_0_5b": (14, 2, 64),
+    "qwen2_5_7b": (28, 4, 128),
+    "qwen3_8b": (32, 8, 128),
+}
+
+
+def _kv():
+    """The framework's binding (only where the calls are its own)."""
+    at = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
+                      "mini-serve-rs_amd")
+    if at not in sys.path:
+        sys.path.insert(0, at)
+    import rlse_kv
+    return rlse_kv
+
+
+def _attn(name, model, dtype, layers, seqs, tlo, thi, lo, hi, window=0, sinks=0):
+    return {"name": name, "kind": "attn", "model": model, "dtype": dtype, "layers": layers,
+            "seqs": seqs, "tlo": tlo, "thi": thi, "lo": lo, "hi": hi, "window": window,
+            "sinks": sinks}
+
+
+def _score(name, model, dtype, layers, seqs, tlo, thi, lo, hi, window=0, sinks=0, prev=True):
+    return dict(_attn(name, model, dtype, layers, seqs, tlo, thi, lo, hi, window, sinks),
+                kind="score", prev=prev)
+
+
+def _evict(name, model, dtype, layers, seqs, lo, hi, budget, sinks, recent):
+    return {"name": name, "kind": "evict", "model": model, "dtype": dtype, "layers": layers,
+            "seqs": seqs, "lo": lo, "hi": hi, "budget": budget, "sinks": sinks, "recent": recent}
+
+
+def listed():
+    return [
+        # One user's next token, one layer: the smallest call, all latency.
+        _attn("attn_one", "qwen3_0_6b", "bf16", 1, 1, 1, 1, 700, 700),
+        # A draft of five tokens checked for six users, in f32.
+        _attn("attn_draft_f32", "qwen3_0_6b", "f32", 1, 6, 5, 5, 900, 2100),
+        # A busy server's step over long chats kept to a window and sinks.
+        _attn("attn_step_window", "qwen3_0_6b", "bf16", 8, 32, 1, 1, 2000, 12000, 1024, 4),
+        # Many users with whole long documents in the cache.
+        _attn("attn_step_long", "qwen3_8b", "f16", 1, 48, 1, 1, 4096, 32768),
+        # Chunked prefill of some users among others: odd, ragged chunks.
+        _attn("attn_mixed", "qwen2_5_7b", "bf16", 1, 24, 1, 301, 100, 3000),
+        # Chunks of three long documents under a window.
+        _attn("attn_chunk_window", "qwen3_8b", "f16", 1, 3, 1500, 2500, 6000, 10000, 2048, 16),
+        # Two long prompts' chunks over everything before them: the largest products.
+        _attn("attn_prompts", "qwen3_8b", "bf16", 1, 2, 4096, 4096, 0, 6000),
+        # A step's weights added to what the keys have, the high-GQA model.
+        _score("score_step", "qwen2_5_0_5b", "bf16", 4, 64, 1, 1, 1000, 4000),
+        # The weights a prompt's chunk gives, counted anew.
+        _score("score_chunk", "qwen3_0_6b", "f16", 1, 4, 400, 777, 1000, 3000, prev=False),
+        # The same for a long chunk under a window.
+        _score("score_chunk_window", "qwen3_8b", "bf16", 1, 2, 2000, 2048, 4096, 8192, 4096, 4),
+        # One user's cache of one layer cut to a third.
+        _evict("evict_one_f32", "qwen2_5_0_5b", "f32", 1, 1, 1500, 1500, 500, 4, 100),
+        # The whole model's caches of sixteen users cut to 1024 keys a head.
+        _evict("evict_model", "qwen3_0_6b", "bf16", 28, 16, 1500, 4096, 1024, 4, 256),
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    kind = rng.choice(["attn", "attn", "attn", "score", "score", "evict", "evict"])
+    model = rng.choice(list(HEADS))
+    hq, hkv, d = HEADS[model]
+    dtype = rng.choice(["bf16", "bf16", "f16", "f32"])
+    es = BYTES[dtype]
+    if kind == "evict":
+        lo = _log_int(rng, 64, 8192)
+        hi = rng.randint(lo, 2 * lo)
+        layers, seqs = rng.randint(1, 28), _log_int(rng, 1, 32)
+        # at most 1.8 GB of K/V
+        per = 2 * hi * hkv * d * es
+        seqs = max(1, min(seqs, 1_800_000_000 // per))
+        layers = max(1, min(layers, 1_800_000_000 // (per * seqs)))
+        budget = _log_int(rng, 32, lo)
+        sinks = min(budget // 2, rng.choice([0, 1, 4, 16]))
+        case = _evict("", model, dtype, layers, seqs, lo, hi, budget, sinks,
+                      rng.randint(0, budget - sinks))
+    else:
+        shape = rng.choice(["step", "step", "draft", "chunk", "chunk"])
+        thi = {"step": 1, "draft": rng.randint(2, 17)}.get(shape) or _log_int(rng, 18, 2048)
+        tlo = thi if shape != "chunk" else rng.randint(1, thi)
+        lo = 0 if rng.random() < 0.15 else _log_int(rng, 16, 16384)
+        hi = rng.randint(lo, 2 * lo + 64)
+        window = rng.choice([0, _log_int(rng, 16, 4096)])
+        sinks = rng.choice([0, 4, 16, rng.randint(1, 200)]) if window else 0
+        seqs = _log_int(rng, 1, 64)
+        # at most 3 GB of K/V and 60 G (query head, key) products of d values
+        keys = min(hi + thi, window + sinks + thi) if window else hi + thi
+        seqs = max(1, min(seqs, 3_000_000_000 // (2 * (hi + thi) * hkv * d * es),
+                          1_000_000_000 // (keys * thi * hq)))
+        layers = rng.randint(1, 4) if thi == 1 and seqs * (hi + thi) < 200_000 else 1
+        make = _attn if kind == "attn" else _score
+        case = make("", model, dtype, layers, seqs, tlo, thi, lo, hi, window, sinks)
+        if kind == "score":
+            case["prev"] = rng.choice([True, False])
+    del case["name"]
+    return case
+
+
+# -- inputs ------------------------------------------------------------------
+def _spread(n, lo, hi):
+    """n values evenly over [lo, hi]."""
+    return [lo + (2 * i + 1) * (hi - lo + 1) // (2 * n) for i in range(n)]
+
+
+def _lengths(case):
+    """New tokens and cached keys of every sequence (before their shuffle)."""
+    n = case["seqs"]
+    cached = [min(c, case["hi"]) for c in _spread(n, case["lo"], case["hi"])]
+    if case["kind"] == "evict":
+        return None, cached
+    new = [min(t, case["thi"]) for t in _spread(n, case["tlo"], case["thi"])]
+    # long chunks after short caches as well as after long ones
+    return new[::2] + new[1::2][::-1], cached
+
+
+def _randn(g, dtype, *shape):
+    return torch.randn(shape, generator=g, device=DEV, dtype=TORCH[dtype])
+
+
+def _tables(g, pages, first, count):
+    """Block tables drawing each sequence's pages from a shuffle of the ids
+    first .. first+count-1."""
+    perm = (torch.randperm(count, generator=g, device=DEV) + first).to(torch.int32).cpu()
+    t = torch.zeros((len(pages), max(pages)), dtype=torch.int32)
+    used = 0
+    for i, k in enumerate(pages):
+        t[i, :k] = perm[used:used + k]
+        used += k
+    return t
+
+
+def prepare(case, seed):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(int(seed))
+    hq, hkv, d = HEADS[case["model"]]
+    dt, layers, n = case["dtype"], case["layers"], case["seqs"]
+    new, cached = _lengths(case)
+    order = torch.randperm(n, generator=g, device=DEV).cpu().tolist()
+    cached = [cached[i] for i in order]
+    s = {"case": case}
+    if case["kind"] == "evict":
+        lens, budget = cached, case["budget"]
+        pages = [(x + 15) // 16 for x in lens]
+        npages = (budget + 15) // 16
+        nb = sum(pages)
+        s["tables"] = _tables(g, pages, 0, nb).to(DEV)
+        # the fresh pages follow the old ones in the pool, in a shuffled order
+        s["new_tables"] = _tables(g, [npages] * n, nb, n * npages).to(DEV)
+        s["nb"], s["old"] = nb + n * npages, nb
+        for name in ("k", "v"):
+            s[name] = torch.zeros((layers, s["nb"], hkv, 16, d), dtype=TORCH[dt], device=DEV)
+            s[name][:, :nb] = _randn(g, dt, layers, nb, hkv, 16, d)
+        slots = s["tables"].shape[1] * 16
+        # Gathered weights: few keys hold most; some (never in a window) none.
+        w = torch.randn((layers, n, hkv, slots), generator=g, device=DEV).mul_(2).exp_()
+        w[torch.rand(w.shape, generator=g, device=DEV) < 0.1] = 0
+        s["scores"], s["new_scores"] = w, torch.zeros_like(w)
+        s["lens"] = torch.tensor(lens, dtype=torch.int32).to(DEV)
+        s["new_lens"] = torch.zeros(n, dtype=torch.int32, device=DEV)
+        s["keep"] = torch.zeros((layers, n, hkv, budget), dtype=torch.int32, device=DEV)
+        return s
+    new = [new[i] for i in order]
+    lens = [a + b for a, b in zip(new, cached)]
+    pages = [(x + 15) // 16 for x in lens]
+    s["nb"] = sum(pages) + 16
+    s["tables"] = _tables(g, pages, 0, s["nb"]).to(DEV)
+    s["total"], s["most"], s["longest"] = sum(new), max(new), max(lens)
+    s["new"], s["host_lens"] = new, lens
+    cu = [sum(new[:i]) for i in range(n + 1)]
+    s["cu"] = torch.tensor(cu, dtype=torch.int32).to(DEV)
+    s["lens"] = torch.tensor(lens, dtype=torch.int32).to(DEV)
+    s["q"] = _randn(g, dt, layers, s["total"], hq, d)
+    s["k"] = _randn(g, dt, layers, s["nb"], hkv, 16, d)
+    s["scale"] = 1.0 / math.sqrt(d)
+    if case["kind"] == "attn":
+        s["v"] = _randn(g, dt, layers, s["nb"], hkv, 16, d)
+        s["out"] = torch.empty_like(s["q"])
+        s["lse"] = torch.empty((layers, s["total"], hq), device=DEV)
+    else:
+        slots = s["tables"].shape[1] * 16
+        shape = (layers, n, hkv, slots)
+        s["prev"] = None
+        if case["prev"]:
+            s["prev"] = torch.rand(shape, generator=g, device=DEV) * 4
+        s["scores"] = torch.zeros(shape, device=DEV)
+        # what the attention over the same keys left behind
+        s["lse"] = torch.empty((layers, s["total"], hq), device=DEV)
+        for l in range(layers):
+            for b in range(n):
+                at = slice(cu[b], cu[b + 1])
+                pos = torch.arange(lens[b], device=DEV)
+                kb = s["k"][l][s["tables"][b, pos // 16].long(), :, pos % 16]
+                see = _visible(case, pos[None, :], pos[lens[b] - new[b]:, None])
+                for h in range(hkv):
+                    heads = slice(h * (hq // hkv), (h + 1) * (hq // hkv))
+                    x = s["q"][l, at, heads].float() @ kb[:, h].float().t()
+                    x = (x * s["scale"]).masked_fill(~see[:, None, :], -math.inf)
+                    s["lse"][l, at, heads] = torch.logsumexp(x, -1)
+    if own:
+        _own_state(s)
+    return s
+
+
+def _own_state(s):
+    """The step's plan buffer and workspace, kept by a program for all steps."""
+    kv = _kv()
+    hq, hkv, d = HEADS[s["case"]["model"]]
+    n = s["case"]["seqs"]
+    s["plan"] = torch.zeros(kv.chunk_plan_size(n, s["total"], hq, hkv), dtype=torch.uint8,
+                            device=DEV)
+    s["ws"] = torch.zeros(kv.chunk_workspace_size(n, s["total"], s["most"], hq, hkv, d),
+                          dtype=torch.uint8, device=DEV)
+
+
+def _visible(case, key, query):
+    """Whether the query at one position sees the key at another."""
+    see = key <= query
+    if case["window"]:
+        see = see & ((query - key < case["window"]) | (key < case["sinks"]))
+    return see
+
+
+# -- the plain form ----------------------------------------------------------
+def _keys(s):
+    """Positions [seqs][n] of every key that one of a sequence's queries sees
+    (with some that none does), and which of them are real."""
+    case = s["case"]
+    lens = s["lens"].long()[:, None]
+    span = case["window"] + s["most"] - 1
+    if not case["window"] or span + case["sinks"] >= s["longest"]:
+        pos = torch.arange(s["longest"], device=DEV).expand(len(lens), -1)
+        return pos, pos < lens
+    first = torch.arange(case["sinks"], device=DEV).expand(len(lens), -1)
+    last = lens - span + torch.arange(span, device=DEV)
+    pos = torch.cat([first, last], 1)
+    real = torch.cat([first < lens, last >= case["sinks"]], 1)
+    return pos.clamp(min=0), real
+
+
+def _queries(s):
+    """Rows of q of every sequence, padded to the longest chunk, their
+    positions, and which of them are real."""
+    cu, lens = s["cu"].long(), s["lens"].long()
+    new = (cu[1:] - cu[:-1])[:, None]
+    t = torch.arange(s["most"], device=DEV)[None, :]
+    return (cu[:-1, None] + t).clamp(max=s["total"] - 1), lens[:, None] - new + t, t < new
+
+
+def _logits(s, layer, pos, real):
+    """Scaled products [seqs][kv heads][group][new tokens][keys] in 32 bits,
+    -inf where the query does not see the key, with the padded rows' mask."""
+    hq, hkv, d = HEADS[s["case"]["model"]]
+    page = s["tables"].gather(1, pos // 16).long()
+    row, at, is_row = _queries(s)
+    k = s["k"][layer][page, :, pos % 16].float().permute(0, 2, 3, 1).contiguous()
+    q = s["q"][layer][row].float()
+    n, t = row.shape
+    q = q.view(n, t, hkv, hq // hkv, d).permute(0, 2, 3, 1, 4).reshape(n, hkv, -1, d)
+    x = torch.matmul(q, k).mul_(s["scale"]).view(n, hkv, hq // hkv, t, -1)
+    see = _visible(s["case"], pos[:, None, :], at[:, :, None]) & real[:, None, :]
+    x.masked_fill_(~see[:, None, None], -math.inf)
+    return x, page, row, is_row
+
+
+def _plain_attn(s, layer):
+    hq, hkv, d = HEADS[s["case"]["model"]]
+    pos, real = _keys(s)
+    x, page, row, is_row = _logits(s, layer, pos, real)
+    v = s["v"][layer][page, :, pos % 16].float().permute(0, 2, 1, 3).contiguous()
+    top = x.amax(-1, keepdim=True)
+    top = top.masked_fill(top == -math.inf, 0)
+    p = x.sub_(top).exp_()
+    total = p.sum(-1, keepdim=True)
+    n, t = row.shape
+    o = torch.matmul(p.view(n, hkv, -1, p.shape[-1]), v).view(n, hkv, hq // hkv, t, d)
+    o = torch.where(total > 0, o / total, torch.zeros_like(o))
+    lse = (top + total.log()).squeeze(-1)
+    o = o.permute(0, 3, 1, 2, 4).reshape(n, t, hq, d)[is_row]
+    lse = lse.permute(0, 3, 1, 2).reshape(n, t, hq)[is_row]
+    return o.to(s["q"].dtype), lse
+
+
+def _plain_score(s, layer):
+    hq, hkv, d = HEADS[s["case"]["model"]]
+    pos, real = _keys(s)
+    x, _, row, is_row = _logits(s, layer, pos, real)
+    n, t = row.shape
+    lse = s["lse"][layer][row].view(n, t, hkv, hq // hkv).permute(0, 2, 3, 1)
+    p = x.sub_(lse[..., None]).exp_().masked_fill_(~is_row[:, None, None, :, None], 0)
+    w = p.sum((2, 3)) * real[:, None, :]
+    slots = s["scores"].shape[-1]
+    got = torch.zeros((n, hkv, slots), device=DEV)
+    got.scatter_add_(2, pos[:, None, :].expand(n, hkv, -1), w)
+    at = torch.arange(slots, device=DEV)
+    lens = s["lens"].long()[:, None, None]
+    new = (s["cu"][1:] - s["cu"][:-1]).long()[:, None, None]
+    if s["prev"] is not None:
+        got += torch.where(at < lens - new, s["prev"][layer], torch.zeros_like(got))
+    return got.masked_fill_(at >= lens, 0)
+
+
+def _plain_evict(s):
+    case, lens, w = s["case"], s["lens"].long(), s["scores"]
+    layers, n, hkv, slots = w.shape
+    budget = case["budget"]
+    at = torch.arange(slots, device=DEV)
+    ends = lens[:, None]
+    rank = torch.where((at >= case["sinks"]) & (at < ends - case["recent"]), 1, 0)
+    rank = torch.where(ends <= budget, torch.zeros_like(rank), rank)
+    rank = torch.where(at >= ends, torch.full_like(rank, 2), rank)  # [n][slots]
+    # kept ones first (rank 0), then by weight, then nothing; ties by index
+    key = torch.where(rank == 1, w.permute(0, 2, 1, 3), torch.zeros(1, device=DEV))
+    key = torch.where(rank == 0, math.inf, torch.where(rank == 2, -math.inf, key))
+    best = key.sort(dim=-1, descending=True, stable=True).indices[..., :budget]
+    short = torch.arange(best.shape[-1], device=DEV) >= ends.clamp(max=budget)
+    keep = best.masked_fill(short, slots).sort(dim=-1).values.permute(0, 2, 1, 3)
+    is_kept = keep < slots
+    keep = torch.where(is_kept, keep, torch.full_like(keep, -1))
+    src = keep.clamp(min=0)
+    page = s["tables"].long()[None, :, None].expand(layers, n, hkv, -1).gather(3, src // 16)
+    layer = torch.arange(layers, device=DEV)[:, None, None, None]
+    head = torch.arange(hkv, device=DEV)[None, None, :, None]
+    j = torch.arange(keep.shape[-1], device=DEV)
+    to = (s["new_tables"].long()[:, j // 16] - s["old"])[None, :, None].expand_as(keep)
+    slot = (j % 16).expand_as(keep)
+    layer, head = layer.expand_as(keep)[is_kept], head.expand_as(keep)[is_kept]
+    outs = []
+    for pool in (s["k"], s["v"]):
+        new = torch.zeros((layers, s["nb"] - s["old"]) + pool.shape[2:], dtype=pool.dtype,
+                          device=DEV)
+        new[layer, to[is_kept], head, slot[is_kept]] = pool[layer, page[is_kept], head,
+                                                            (src % 16)[is_kept]]
+        outs.append(new)
+    kept = torch.zeros_like(w)
+    kept[..., :keep.shape[-1]] = w.gather(3, src).masked_fill(~is_kept, 0)
+    full = torch.full((layers, n, hkv, budget), -1, dtype=torch.int32, device=DEV)
+    full[..., :keep.shape[-1]] = keep.to(torch.int32)
+    return {"k": outs[0], "v": outs[1], "scores": kept, "keep": full,
+            "lens": lens.clamp(max=budget).to(torch.int32)}
+
+
+def run(state):
+    if own:
+        return _own_run(state)
+    case = state["case"]
+    if case["kind"] == "evict":
+        return _plain_evict(state)
+    each = range(case["layers"])
+    if case["kind"] == "score":
+        return [_plain_score(state, l) for l in each]
+    return [_plain_attn(state, l) for l in each]
+
+
+def _own_run(s):
+    kv, case = _kv(), s["case"]
+    hq, hkv, d = HEADS[case["model"]]
+    n, dt, mbps = case["seqs"], case["dtype"], s["tables"].shape[1]
+    st = torch.cuda.current_stream()
+    if case["kind"] == "evict":
+        kv.kv_evict(s["k"], s["v"], s["k"][0].numel(), case["layers"], s["tables"], s["lens"],
+                    s["scores"], s["scores"][0].numel(), s["new_tables"], s["new_lens"],
+                    s["new_scores"], s["keep"], n, hkv, d, mbps, s["new_tables"].shape[1],
+                    s["nb"], case["budget"], case["sinks"], case["recent"], dt, st)
+        return {"k": s["k"][:, s["old"]:], "v": s["v"][:, s["old"]:], "scores": s["new_scores"],
+                "keep": s["keep"], "lens": s["new_lens"]}
+    kv.chunk_plan(s["cu"], s["lens"], n, s["total"], s["most"], hq, hkv, mbps, case["window"],
+                  case["sinks"], s["plan"], s["plan"].numel(), st)
+    shape = (n, s["total"], s["most"], hq, hkv, d, mbps, s["nb"], case["window"], case["sinks"],
+             s["scale"], dt)
+    for l in range(case["layers"]):
+        if case["kind"] == "attn":
+            kv.chunk_attn(s["q"][l], s["k"][l], s["v"][l], s["tables"], s["cu"], s["lens"],
+                          s["plan"], s["out"][l], s["lse"][l], *shape, s["ws"], s["ws"].numel(),
+                          st)
+        else:
+            kv.kv_scores(s["q"][l], s["k"][l], s["tables"], s["cu"], s["lens"], s["plan"],
+                         s["lse"][l], None if s["prev"] is None else s["prev"][l],
+                         s["scores"][l], *shape, st)
+    if case["kind"] == "attn":
+        return [(s["out"][l], s["lse"][l]) for l in range(case["layers"])]
+    return [s["scores"][l] for l in range(case["layers"])]
+
+
+# -- the definition in 64 bits -----------------------------------------------
+def exact(case, seed):
+    s = prepare(case, seed)
+    hq, hkv, d = HEADS[case["model"]]
+    group = hq // hkv
+    if case["kind"] == "evict":
+        return _exact_evict(s)
+    answers = []
+    for l in range(case["layers"]):
+        out = torch.zeros((s["total"], hq, d), dtype=torch.float64, device=DEV)
+        lse = torch.zeros((s["total"], hq), dtype=torch.float64, device=DEV)
+        weight = torch.zeros(s["scores"].shape[1:] if case["kind"] == "score" else 1,
+                             dtype=torch.float64, device=DEV)
+        row = 0
+        for b, (t, length) in enumerate(zip(s["new"], s["host_lens"])):
+            table = s["tables"][b, :(length + 15) // 16].long()
+            dist = torch.arange(length - t, length, device=DEV)[:, None] - torch.arange(
+                length, device=DEV)[None, :]
+            hidden = dist < 0
+            if case["window"]:
+                hidden = hidden | ((dist >= case["window"]) & (
+                    torch.arange(length, device=DEV)[None, :] >= case["sinks"]))
+            for h in range(hkv):
+                keys = s["k"][l, table, h].reshape(-1, d)[:length].double()
+                for j in range(h * group, (h + 1) * group):
+                    x = s["q"][l, row:row + t, j].double() @ keys.T / math.sqrt(d)
+                    x[hidden] = -math.inf
+                    if case["kind"] == "score":
+                        weight[b, h, :length] += (
+                            x - s["lse"][l, row:row + t, j].double()[:, None]).exp().sum(0)
+                        continue
+                    values = s["v"][l, table, h].reshape(-1, d)[:length].double()
+                    lse[row:row + t, j] = x.logsumexp(-1)
+                    out[row:row + t, j] = x.softmax(-1) @ values
+            if case["kind"] == "score" and case["prev"]:
+                weight[b, :, :length - t] += s["prev"][l, b, :, :length - t].double()
+            row += t
+        answers.append(weight if case["kind"] == "score" else (out, lse))
+    return answers
+
+
+def _exact_evict(s):
+    case, w = s["case"], s["scores"].double().cpu().numpy()
+    layers, n, hkv, _ = w.shape
+    if layers * n * hkv > 6000:
+        return None
+    budget, sinks, recent = case["budget"], case["sinks"], case["recent"]
+    keep = torch.full((layers, n, hkv, budget), -1, dtype=torch.int32)
+    scores = torch.zeros(w.shape, dtype=torch.float64)
+    new_lens = torch.zeros(n, dtype=torch.int32)
+    for b, length in enumerate(s["lens"].tolist()):
+        new_lens[b] = min(length, budget)
+        for l in range(layers):
+            for h in range(hkv):
+                mine = w[l, b, h, :length]
+                kept = list(range(length))
+                if length > budget:
+                    middle = mine[sinks:length - recent]
+                    heavy = (-middle).argsort(kind="stable")[:budget - sinks - recent] + sinks
+                    kept = (list(range(sinks)) + sorted(heavy.tolist()) +
+                            list(range(length - recent, length)))
+                keep[l, b, h, :len(kept)] = torch.tensor(kept, dtype=torch.int32)
+                scores[l, b, h, :len(kept)] = torch.from_numpy(mine[kept])
+    pools = {}
+    tables, new_tables = s["tables"].long(), s["new_tables"].long()
+    for name in ("k", "v"):
+        new = torch.zeros((layers, s["nb"] - s["old"]) + s[name].shape[2:], dtype=torch.float64,
+                          device=DEV)
+        for l in range(layers):
+            for b in range(n):
+                count = int(new_lens[b])
+                for h in range(hkv):
+                    whole = s[name][l, tables[b], h].reshape(-1, new.shape[-1])
+                    rows = whole[keep[l, b, h, :count].long().to(DEV)].double()
+                    ids = new_tables[b, :(count + 15) // 16] - s["old"]
+                    full = torch.zeros((len(ids) * 16, new.shape[-1]), dtype=torch.float64,
+                                       device=DEV)
+                    full[:count] = rows
+                    new[l, ids, h] = full.view(len(ids), 16, -1)
+        pools[name] = new
+    return {"k": pools["k"], "v": pools["v"], "scores": scores, "keep": keep, "lens": new_lens}
+
+
+def work(case):
+    """K/V rows (and weights) that a pass has to read, new ones it has to
+    write; the products over the visible (query head, key) pairs."""
+    hq, hkv, d = HEADS[case["model"]]
+    es, layers = BYTES[case["dtype"]], case["layers"]
+    new, cached = _lengths(case)
+    if case["kind"] == "evict":
+        kept = sum(min(c, case["budget"]) for c in cached)
+        rows, slots = layers * hkv * kept, layers * hkv * sum(cached)
+        # K and V rows read and written, weights read, kept ones and indices written
+        return {"bytes": 4 * rows * d * es + 4 * slots + 8 * rows, "flops": slots}
+    w, sinks = case["window"], case["sinks"]
+    pairs = keys = slots = 0
+    for t, c in zip(new, cached):
+        if w:
+            # query at position p sees min(p + 1, w) keys and the sinks before them
+            pairs += sum(min(p + 1, w) + min(max(p + 1 - w, 0), sinks) for p in range(c, c + t))
+            keys += min(c + t, w + t - 1) + min(max(c + 1 - w, 0), sinks)
+        else:
+            pairs += t * c + t * (t + 1) // 2
+            keys += c + t
+        slots += c + t
+    total = sum(new)
+    if case["kind"] == "attn":
+        return {"bytes": layers * (2 * keys * hkv * d * es + 2 * total * hq * d * es +
+                                   4 * total * hq), "flops": layers * 4 * pairs * hq * d}
+    return {"bytes": layers * (keys * hkv * d * es + total * hq * (d * es + 4) +
+                               4 * slots * hkv * (2 if case["prev"] else 1)),
+            "flops": layers * 2 * pairs * hq * d}
