@@ -414,13 +414,11 @@ def _own_run(s):
              s["scale"], dt)
     for l in range(case["layers"]):
         if case["kind"] == "attn":
-            kv.chunk_attn(s["q"][l], s["k"][l], s["v"][l], s["tables"], s["cu"], s["lens"],
-                          s["plan"], s["out"][l], s["lse"][l], *shape, s["ws"], s["ws"].numel(),
-                          st)
+            kv.chunk_attn(s["q"][l], s["k"][l], s["v"][l], s["tables"], s["plan"], s["out"][l],
+                          s["lse"][l], *shape, s["ws"], s["ws"].numel(), st)
         else:
-            kv.kv_scores(s["q"][l], s["k"][l], s["tables"], s["cu"], s["lens"], s["plan"],
-                         s["lse"][l], None if s["prev"] is None else s["prev"][l],
-                         s["scores"][l], *shape, st)
+            kv.kv_scores(s["q"][l], s["k"][l], s["tables"], s["plan"], s["lse"][l],
+                         None if s["prev"] is None else s["prev"][l], s["scores"][l], *shape, st)
     if case["kind"] == "attn":
         return [(s["out"][l], s["lse"][l]) for l in range(case["layers"])]
     return [s["scores"][l] for l in range(case["layers"])]
