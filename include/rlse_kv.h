@@ -62,6 +62,8 @@ int rlse_version(void);
 /*     sequence's first prefix_pages table entries differ from sequence */
 /*     0's, or its new token lies inside them); the step's outputs are  */
 /*     not its attention.                                               */
+/*   RLSE_WS_ERR_PLAN: a ragged step's plan was built for another step   */
+/*     (word 0 of the plan; the call wrote nothing).                      */
 /* The reference turns a failed step into BackendError and quarantines */
 /* the backend (src/backends/candle.rs:689-696); a caller maps a       */
 /* nonzero rlse_workspace_check to the same.                           */
@@ -69,6 +71,7 @@ int rlse_version(void);
 #define RLSE_WS_ERR_MERGE_TIMEOUT 1u
 #define RLSE_WS_ERR_LENGTH 2u
 #define RLSE_WS_ERR_PREFIX 4u
+#define RLSE_WS_ERR_PLAN 8u
 /* Synchronises stream, then reads and clears the flags of a decode or
  * projection workspace (NULL: the library's own decode workspaces of the
  * current device -- the one used by calls without a workspace and the
@@ -395,6 +398,66 @@ int rlse_prefill_attn(const void* q, const void* k_pool, const void* v_pool,
                       int num_heads, int num_kv_heads, int head_dim, int max_blocks,
                       int num_blocks, float scale, int dtype, void* workspace,
                       size_t workspace_bytes, rlse_stream_t stream);
+
+/* ------------------------------------------------------------------ */
+/* Ragged steps: attention with a sliding window and sinks for any      */
+/* number of sequences with any number of new tokens each (a decode     */
+/* step, drafts, prompt chunks, or a mix), the weight every cached key  */
+/* receives, and the eviction of the lightest keys. No counterpart in   */
+/* the reference, which attends one sequence at a time without a window */
+/* (src/backends/qwen2.rs:177-203, 329-345) and drops nothing from a    */
+/* cache but whole requests.                                            */
+/*                                                                      */
+/* Sequence b's new tokens are rows cu_tokens[b] .. cu_tokens[b+1]-1 of  */
+/* q and out (device int32 [num_seqs+1], ascending from 0); its          */
+/* seq_lens[b] keys include theirs, already appended, so token t sits at */
+/* slot p = seq_lens[b] - n + t and sees key k when k <= p and (window == 0 */
+/* or p - k < window or k < sinks). A sequence may have no new token in  */
+/* a step; its entry of seq_lens is then not looked at. Table entries of */
+/* pages that no new token sees are not read (a window's caller may have */
+/* given them back). Rows of q and out outside every sequence are left   */
+/* as they were.                                                         */
+/*                                                                      */
+/* num_seqs <= 4096; total_tokens: rows of q at least cu_tokens[num_seqs]; */
+/* max_tokens: the most new tokens of a sequence, or a bound on it (1 for */
+/* a decode step). A sequence with more, or with seq_lens below its new  */
+/* tokens or above max_blocks_per_seq*16, or with offsets that descend or */
+/* pass total_tokens, raises RLSE_WS_ERR_LENGTH in word 0 of the plan and */
+/* is left out (its rows are not written). rlse_workspace_check(plan, ...) */
+/* reads and clears the flags.                                           */
+/* ------------------------------------------------------------------ */
+
+/* The step's plan, built once on the device and read by every layer's
+ * calls with the same arguments: plan is rlse_chunk_plan_size bytes, 16-byte
+ * aligned. A call given a plan of other arguments raises RLSE_WS_ERR_PLAN in
+ * it and writes nothing. Steps that overlap need a plan each. */
+int rlse_chunk_plan_size(int num_seqs, int total_tokens, int num_heads, int num_kv_heads,
+                         size_t* bytes);
+int rlse_chunk_plan(const int32_t* cu_tokens, const int32_t* seq_lens, int num_seqs,
+                    int total_tokens, int max_tokens, int num_heads, int num_kv_heads,
+                    int max_blocks_per_seq, int window, int sinks, void* plan, size_t plan_bytes,
+                    rlse_stream_t stream);
+/* softmax(scale q K^T) V over the visible keys: q and out [total_tokens]
+ * [num_heads][head_dim], lse (may be NULL) float [total_tokens][num_heads],
+ * the logarithm of the sum of e^(scale q.k) over them. A row that sees no key
+ * (its pages' ids are all outside [0, num_blocks)) gives zeros and -inf.
+ * Scores that are NaN, and infinite or NaN values of a visible key, reach
+ * the rows that see it and no others. f32, bf16 or f16, head_dim 64 or 128,
+ * any group size; q, out and pools 16-byte aligned. workspace:
+ * rlse_chunk_workspace_size bytes (grows with none of the lengths), 16-byte
+ * aligned, zero-filled once before its first use and then left to the
+ * library; one serves every call with the same head shape and at most the
+ * max_tokens it was sized for. Calls that share one must be ordered (same
+ * stream). Results do not depend on what shares the step with a sequence
+ * beyond rounding: its keys are divided among workgroups differently. */
+int rlse_chunk_workspace_size(int num_seqs, int total_tokens, int max_tokens, int num_heads,
+                              int num_kv_heads, int head_dim, size_t* bytes);
+int rlse_chunk_attn(const void* q, const void* k_pool, const void* v_pool,
+                    const int32_t* block_tables, void* plan, void* out, float* lse, int num_seqs,
+                    int total_tokens, int max_tokens, int num_heads, int num_kv_heads,
+                    int head_dim, int max_blocks_per_seq, int num_blocks, int window, int sinks,
+                    float scale, int dtype, void* workspace, size_t workspace_bytes,
+                    rlse_stream_t stream);
 
 /* ------------------------------------------------------------------ */
 /* Normalisation and rotary embedding.                                 */

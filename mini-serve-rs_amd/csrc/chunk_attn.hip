@@ -1,0 +1,1145 @@
+// Attention of a ragged step over the paged KV pool, with a sliding window
+// and sinks, on MFMA tiles (gfx950).
+//
+// The reference attends one sequence at a time, causally and without a window
+// (src/backends/qwen2.rs:177-203, 329-345, 476-503). Here a step holds any
+// number of sequences with any number of new tokens each; the query at
+// position p sees key k when k <= p and (no window, or p - k < window, or
+// k < sinks), and
+//   out = sum_k e^(s_k - max) v_k / sum_k e^(s_k - max),  s_k = scale q.k,
+// with lse = max + log sum beside it. The rows, pages and shares are the
+// plan's (chunk_plan.cuh).
+//
+// Two kernels, by the rows a sequence has per KV head (tokens * group size):
+//  - thin (at most 32 rows: decode steps, drafts): HBM bound. A wave streams
+//    its own pages, 16 keys at a time, and every key meets all rows at once
+//    (S^T = K.Q^T on 16x16 MFMAs with K straight from memory in the operand
+//    layout); the four waves of a workgroup meet at the tile's end.
+//  - wide: MFMA bound. Eight waves of 32 rows share 64 keys staged in LDS.
+// Softmax statistics, sums and accumulators are f32; probabilities are
+// rounded to the K/V type for the product with V (2^-9 relative in bf16, as
+// large as the output's own rounding), while the sum takes them unrounded.
+//
+// Keys a row does not see get no weight whatever their K and V hold: scores
+// are replaced, not added to, and where a page is not wholly visible an
+// infinite or NaN value of V reaches only the rows that see its key (split_word).
+#include <math.h>
+
+#include <mutex>
+
+#include "chunk_plan.cuh"
+#include "chunk_plan.h"
+#include "host_common.h"
+
+namespace rlse {
+namespace {
+
+// The running max of a query's softmax moves only when a score exceeds it by
+// more than this many powers of two (probabilities stay below 2^8).
+constexpr float kLazyLog2 = 8.f;
+constexpr float kLn2 = 0.69314718055994531f;
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4_t __attribute__((ext_vector_type(4)));
+typedef short i16x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) i16x4_t lds_i16x4_t;
+
+// 16-bit tiles: 16x16x32 and 32x32x16 products of 16-byte operands, and
+// 16x16x16 ones of 8-byte operands.
+template <typename T>
+struct Tile;
+template <>
+struct Tile<bf16> {
+  static __device__ __forceinline__ f32x4_t mma16(uint4 a, uint4 b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                   __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x4_t mma16h(uint2 a, uint2 b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(i16x4_t, a),
+                                                     __builtin_bit_cast(i16x4_t, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x16_t mma32(uint4 a, uint4 b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                   __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+  }
+  static constexpr uint32_t kInf = 0x7f80u, kOne = 0x3f80u;
+};
+template <>
+struct Tile<f16> {
+  static __device__ __forceinline__ f32x4_t mma16(uint4 a, uint4 b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a),
+                                                  __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x4_t mma16h(uint2 a, uint2 b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4_t, a),
+                                                 __builtin_bit_cast(f16x4_t, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x16_t mma32(uint4 a, uint4 b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a),
+                                                  __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+  }
+  static constexpr uint32_t kInf = 0x7c00u, kOne = 0x3c00u;
+};
+
+struct ChunkParams {
+  const void* q;       // [tokens][Hq][D]
+  const void* k_pool;  // [num_blocks][Hkv][16][D]
+  const void* v_pool;
+  const int* tables;   // [num_seqs][mbps]
+  void* out;           // [tokens][Hq][D]
+  float* lse;          // [tokens][Hq] or NULL
+  ChunkPlanView v;
+  uint32_t stamp;
+  float* thin_part;    // [2 * groups][kThinRows * (D + 2)]
+  uint32_t* thin_done; // [groups]: pieces of the tile cut at a share's end
+  float4* wide_part;   // [2 * groups][(D / 8 + 1) * kWideThreads]
+  int Hq, Hkv, G, mbps, num_blocks, window, sinks;
+  float c;             // scale * log2(e)
+};
+
+// Two 16-bit values of one operand word, split: those that are not
+// finite taken out of `w` and marked with a one in pos (+inf, NaN) and
+// neg (-inf, NaN).
+template <typename T>
+__device__ __forceinline__ uint32_t split_word(uint32_t w, uint32_t* pos, uint32_t* neg) {
+  constexpr uint32_t inf = Tile<T>::kInf, one = Tile<T>::kOne;
+  uint32_t keep = 0;
+  *pos = *neg = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t x = w >> (16 * i) & 0xffffu, mag = x & 0x7fffu;
+    keep |= (mag >= inf ? 0u : x) << (16 * i);
+    *pos |= (mag > inf || x == inf ? one : 0u) << (16 * i);
+    *neg |= (mag > inf || (mag == inf && x != inf) ? one : 0u) << (16 * i);
+  }
+  return keep;
+}
+__device__ __forceinline__ float split_word(float w, float* pos, float* neg) {
+  const float mag = fabsf(w);
+  const bool nan = w != w, big = mag == INFINITY;
+  *pos = nan || w == INFINITY ? 1.f : 0.f;
+  *neg = nan || (big && w < 0.f) ? 1.f : 0.f;
+  return nan || big ? 0.f : w;
+}
+// One where a probability is not zero: its row sees that key.
+template <typename T>
+__device__ __forceinline__ uint32_t seen_word(uint32_t w) {
+  return ((w & 0x7fffu) ? Tile<T>::kOne : 0u) | ((w & 0x7fff0000u) ? Tile<T>::kOne << 16 : 0u);
+}
+// What infinities and NaNs of V add to a row that sees them p or n times.
+__device__ __forceinline__ float not_finite(float p, float n) {
+  return (p > 0.f ? INFINITY : 0.f) + (n > 0.f ? -INFINITY : 0.f);
+}
+
+// Partial states handed between workgroups of one launch: pairs of floats
+// stored and loaded at agent scope, coherent across the XCDs' caches.
+__device__ __forceinline__ void st_pair(float* p, float a, float b) {
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(p),
+                     (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a), __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void ld_pair(const float* p, float* out) {
+  const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED,
+                                       __HIP_MEMORY_SCOPE_AGENT);
+  out[0] = __uint_as_float((uint32_t)v);
+  out[1] = __uint_as_float((uint32_t)(v >> 32));
+}
+
+// The weight of a partial state of max m under the joint max M (both -inf:
+// nothing was seen; its sums are 0, or NaN from a NaN score, and stay so).
+__device__ __forceinline__ float state_weight(float m, float M) {
+  return __builtin_amdgcn_exp2f(m - (M == -INFINITY ? 0.f : M));
+}
+__device__ __forceinline__ float inverse_sum(float L) { return L == 0.f ? 0.f : 1.f / L; }
+__device__ __forceinline__ float state_lse(float M, float L) {
+  return (M + __builtin_amdgcn_logf(L)) * kLn2;
+}
+// N consecutive values of a row, N a multiple of 4.
+template <typename T, int N>
+__device__ __forceinline__ void write_row(T* dst, const float* v, float inv) {
+#pragma unroll
+  for (int i = 0; i < N; i += 4) {
+    if constexpr (sizeof(T) == 2)
+      *reinterpret_cast<uint2*>(dst + i) = make_uint2(Packet<T>::pack2(v[i] * inv, v[i + 1] * inv),
+                                                      Packet<T>::pack2(v[i + 2] * inv, v[i + 3] * inv));
+    else
+      *reinterpret_cast<float4*>(dst + i) =
+          make_float4(v[i] * inv, v[i + 1] * inv, v[i + 2] * inv, v[i + 3] * inv);
+  }
+}
+
+// One row's limits: it sees key k when k <= kmax and (k >= wlo or k < sinks).
+struct RowSpan {
+  int kmax, wlo;
+  __device__ __forceinline__ bool sees(int k, int sinks) const {
+    return k <= kmax && (k >= wlo || k < sinks);
+  }
+};
+__device__ __forceinline__ RowSpan row_span(int off, int t, int window) {
+  RowSpan s;
+  s.kmax = off + t;
+  s.wlo = window > 0 ? s.kmax - window + 1 : 0;
+  return s;
+}
+
+// ---------------------------------------------------------------------------
+// Thin sequences
+// ---------------------------------------------------------------------------
+constexpr int kThinWaves = 4;
+constexpr int kThinThreads = 64 * kThinWaves;
+
+// A page of K and V in registers. 16-bit: K in the A-operand layout of
+// 16x16x32 products (lane l: key l % 16, elements 32 r + 8 (l / 16) .. +8 in
+// load r), V as it lies (packet l + 64 r). f32: the same with 16-byte packets
+// of four elements, K's being 16 r + 4 (l / 16) .. +4.
+template <typename T, int D>
+struct PageRegs {
+  static constexpr int N = D * (int)sizeof(T) / 64;
+  uint4 k[N], v[N];
+  int pos;  // position of its first key, -1: no page
+};
+
+// V rows of a wave's page in LDS, padded: 16-bit rows by 16 elements (the
+// four rows of a transposing read on banks of their own), f32 rows by 4.
+template <typename T, int D>
+struct ThinLds {
+  static constexpr int kPad = sizeof(T) == 2 ? 16 : 4;
+  T v[kThinWaves][16][D + kPad];
+};
+
+template <typename T, int D, int RT>
+__global__ __launch_bounds__(kThinThreads, sizeof(T) == 4 && RT == 2 ? 1 : 2) void chunk_thin_kernel(ChunkParams p) {
+  constexpr int N = PageRegs<T, D>::N;
+  constexpr int ES = (int)sizeof(T), PPR = D * ES / 16;  // packets per row
+  constexpr int DT = D / 16;
+  constexpr int NBUF = sizeof(T) == 2 ? 3 : 2;
+  constexpr int kExRow = D + 4;
+  __shared__ __align__(16) ThinLds<T, D> s;
+  __shared__ __align__(16) float s_ex[kThinWaves][16][kExRow];
+  __shared__ float s_ml[kThinWaves][16][2];
+  __shared__ int s_last;
+
+  if (p.v.head->stamp != p.stamp) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) ws_raise(&p.v.head->flags, RLSE_WS_ERR_PLAN);
+    return;
+  }
+  const int groups = p.v.head->thin_groups, tiles = p.v.head->thin_tiles;
+  if ((int)blockIdx.x >= groups) return;
+  const int w = share_index(blockIdx.x, groups);
+  const ChunkShare share = p.v.thin_share[w];
+
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int col = lane & 15, quad = lane >> 4;
+  const int Hq = p.Hq, Hkv = p.Hkv, G = p.G;
+  const int sink_pages = (p.sinks + 15) >> 4;
+  const T* __restrict__ qb = static_cast<const T*>(p.q);
+  const T* __restrict__ kp = static_cast<const T*>(p.k_pool);
+  const T* __restrict__ vp = static_cast<const T*>(p.v_pool);
+
+  int ti = __builtin_amdgcn_readfirstlane(share.tile);
+  int h = __builtin_amdgcn_readfirstlane(share.head);
+  int u0 = __builtin_amdgcn_readfirstlane(share.u0);
+  int left = __builtin_amdgcn_readfirstlane(share.count);
+  bool head_piece = u0 > 0;
+  while (left > 0) {
+    const ChunkTile t = p.v.thin[ti];
+    const int n = __builtin_amdgcn_readfirstlane(t.n), off = __builtin_amdgcn_readfirstlane(t.off);
+    const int tok0 = __builtin_amdgcn_readfirstlane(t.tok0);
+    const int wp0 = __builtin_amdgcn_readfirstlane(t.wp0);
+    const int pages = __builtin_amdgcn_readfirstlane(t.pages);
+    const int* __restrict__ table =
+        p.tables + (size_t)__builtin_amdgcn_readfirstlane(t.seq) * p.mbps;
+    const int seg = min(left, pages - u0);
+    const int rows = n * G;
+    const int kend = off + n;
+
+    // This wave's pages: virtual pages u0 + wave, + kThinWaves, ...
+    const int np = (seg - wave + kThinWaves - 1) / kThinWaves;
+    int ids = -1, pgs = 0, ids_at = 0;
+    auto fetch_ids = [&](int from) __attribute__((always_inline)) {
+      const int i = from + lane;
+      ids = -1;
+      pgs = 0;
+      if (i < np) {
+        pgs = real_page(u0 + wave + i * kThinWaves, wp0, sink_pages);
+        const int id = table[pgs];
+        ids = (unsigned)id < (unsigned)p.num_blocks ? id : -1;
+      }
+      ids_at = from;
+    };
+    fetch_ids(0);
+
+    uint4 q[RT][N];
+    RowSpan span[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int row = rt * 16 + col;
+      const bool real = row < rows;
+      const int tok = real ? row / G : 0, g = real ? row - tok * G : 0;
+      span[rt] = row_span(off, tok, p.window);
+      const T* src = qb + ((size_t)(tok0 + tok) * Hq + h * G + g) * D + quad * (16 / ES);
+#pragma unroll
+      for (int r = 0; r < N; ++r)
+        q[rt][r] = real ? *reinterpret_cast<const uint4*>(src + r * (64 / ES))
+                        : make_uint4(0, 0, 0, 0);
+    }
+
+    f32x4_t o[RT][DT];
+    float m[RT], l[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      m[rt] = -INFINITY;
+      l[rt] = 0.f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[rt][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // Raw buffer loads through a descriptor of the (page, head) tile: no page
+    // (past the wave's last, an id out of range) is a descriptor of no
+    // records, and rows past the last key any row sees lie past its end;
+    // both read as zeros without a memory access.
+    auto load = [&](PageRegs<T, D>& b, int i) __attribute__((always_inline)) {
+      if (i >= ids_at + 64) fetch_ids(i);
+      const int id = __builtin_amdgcn_readlane(ids, i - ids_at);
+      const int pos = __builtin_amdgcn_readlane(pgs, i - ids_at) * 16;
+      const size_t at = ((size_t)(id < 0 ? 0 : id) * Hkv + h) * 16 * D;
+      const int rec = id < 0 ? 0 : min(kend - pos, 16) * D * ES;
+      const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(kp + at), 0, rec,
+                                                        kBufferWord3);
+      const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(vp + at), 0, rec,
+                                                        kBufferWord3);
+#pragma unroll
+      for (int r = 0; r < N; ++r) {
+        b.k[r] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(
+                                               rk, col * D * ES + quad * 16 + r * 64, 0, 0));
+        b.v[r] = __builtin_bit_cast(
+            uint4, __builtin_amdgcn_raw_buffer_load_b128(rv, (lane + 64 * r) * 16, 0, 0));
+      }
+      b.pos = id < 0 ? -1 : pos;
+    };
+
+    auto compute = [&](const PageRegs<T, D>& b) __attribute__((always_inline)) {
+      if (b.pos < 0) return;  // (uniform)
+      // V to this wave's LDS rows; the products below read it transposed.
+#pragma unroll
+      for (int r = 0; r < N; ++r) {
+        const int pk = lane + 64 * r;
+        *reinterpret_cast<uint4*>(&s.v[wave][pk / PPR][(pk % PPR) * (16 / ES)]) = b.v[r];
+      }
+      f32x4_t x[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) x[rt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int r = 0; r < N; ++r)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          if constexpr (ES == 2) {
+            x[rt] = Tile<T>::mma16(b.k[r], q[rt][r], x[rt]);
+          } else {
+            const float* kf = reinterpret_cast<const float*>(&b.k[r]);
+            const float* qf = reinterpret_cast<const float*>(&q[rt][r]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              x[rt] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j], qf[j], x[rt], 0, 0, 0);
+          }
+        }
+      // Every row sees every key of the page: up to the first new token, and
+      // from the last one's window on or among the sinks.
+      const bool whole = b.pos + 15 <= off &&
+                         (p.window <= 0 || b.pos > kend - 1 - p.window || b.pos + 16 <= p.sinks);
+      uint2 pk[RT];
+      float pf[RT][4];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        if (!whole) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (!span[rt].sees(b.pos + quad * 4 + i, p.sinks)) x[rt][i] = -INFINITY;
+        }
+        // Lazy online softmax in log2 units, the state equal in the four
+        // lanes of a row.
+        const float mx = fmaxf(fmaxf(x[rt][0], x[rt][1]), fmaxf(x[rt][2], x[rt][3])) * p.c;
+        if (__any(mx > m[rt] + kLazyLog2)) {
+          float top = fmaxf(mx, __shfl_xor(mx, 16, 64));
+          top = fmaxf(top, __shfl_xor(top, 32, 64));
+          const float mn = fmaxf(m[rt], top);
+          const float a = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[rt] - mn);
+          l[rt] *= a;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) o[rt][d] *= a;
+          m[rt] = mn;
+        }
+        const float nm = m[rt] == -INFINITY ? 0.f : -m[rt];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          pf[rt][i] = __builtin_amdgcn_exp2f(fmaf(x[rt][i], p.c, nm));
+          l[rt] += pf[rt][i];
+        }
+        if constexpr (ES == 2)
+          pk[rt] = make_uint2(Packet<T>::pack2(pf[rt][0], pf[rt][1]),
+                              Packet<T>::pack2(pf[rt][2], pf[rt][3]));
+      }
+      // O^T += V^T . P^T
+      if constexpr (ES == 2) {
+        const uint16_t* row =
+            reinterpret_cast<const uint16_t*>(&s.v[wave][quad * 4 + (col >> 2)][(col & 3) * 4]);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          const uint2 a = __builtin_bit_cast(
+              uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(row + 16 * d)));
+          if (whole) {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) o[rt][d] = Tile<T>::mma16h(a, pk[rt], o[rt][d]);
+          } else {
+            // Values that are not finite reach only the rows that see their key.
+            uint2 pos, neg;
+            const uint2 fin = make_uint2(split_word<T>(a.x, &pos.x, &neg.x),
+                                         split_word<T>(a.y, &pos.y, &neg.y));
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+              const uint2 see = make_uint2(seen_word<T>(pk[rt].x), seen_word<T>(pk[rt].y));
+              const f32x4_t zero{0.f, 0.f, 0.f, 0.f};
+              const f32x4_t cp = Tile<T>::mma16h(pos, see, zero);
+              const f32x4_t cn = Tile<T>::mma16h(neg, see, zero);
+              o[rt][d] = Tile<T>::mma16h(fin, pk[rt], o[rt][d]);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) o[rt][d][i] += not_finite(cp[i], cn[i]);
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            const float a = s.v[wave][quad * 4 + i][16 * d + col];
+            if (whole) {
+#pragma unroll
+              for (int rt = 0; rt < RT; ++rt)
+                o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, pf[rt][i], o[rt][d], 0, 0, 0);
+            } else {
+              float pos, neg;
+              const float fin = split_word(a, &pos, &neg);
+#pragma unroll
+              for (int rt = 0; rt < RT; ++rt) {
+                const float see = pf[rt][i] != 0.f ? 1.f : 0.f;
+                const f32x4_t zero{0.f, 0.f, 0.f, 0.f};
+                const f32x4_t cp = __builtin_amdgcn_mfma_f32_16x16x4f32(pos, see, zero, 0, 0, 0);
+                const f32x4_t cn = __builtin_amdgcn_mfma_f32_16x16x4f32(neg, see, zero, 0, 0, 0);
+                o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(fin, pf[rt][i], o[rt][d], 0, 0, 0);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[rt][d][k] += not_finite(cp[k], cn[k]);
+              }
+            }
+          }
+      }
+    };
+
+    PageRegs<T, D> buf[NBUF];
+#pragma unroll
+    for (int i = 0; i < NBUF - 1; ++i) load(buf[i], i);
+    for (int i = 0; i < np; i += NBUF) {
+#pragma unroll
+      for (int j = 0; j < NBUF; ++j) {
+        load(buf[(j + NBUF - 1) % NBUF], i + j + NBUF - 1);
+        compute(buf[j]);
+      }
+    }
+
+    // The waves' states meet in LDS, 16 rows at a time. Thread tid finishes
+    // row tid / 16, its dimensions (tid % 16) * D / 16 ...
+    const bool cut = seg < pages;
+    float* part = nullptr;
+    if (cut)
+      part = p.thin_part + (size_t)(2 * w + (head_piece ? 0 : 1)) * kThinRows * (D + 2);
+    const int er = tid >> 4, ed = (tid & 15) * DT;
+    auto finish = [&](int row, float M, float L, const float* acc)
+                      __attribute__((always_inline)) {
+      if (row >= rows) return;
+      const int tok = row / G;
+      const size_t at = (size_t)(tok0 + tok) * Hq + h * G + row - tok * G;
+      write_row<T, DT>(static_cast<T*>(p.out) + at * D + ed, acc, inverse_sum(L));
+      if (p.lse && (tid & 15) == 0) p.lse[at] = state_lse(M, L);
+    };
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      if (rt * 16 >= rows) break;
+      __syncthreads();
+      float ls = l[rt] + __shfl_xor(l[rt], 16, 64);
+      ls += __shfl_xor(ls, 32, 64);
+      if (lane < 16) {
+        s_ml[wave][col][0] = m[rt];
+        s_ml[wave][col][1] = ls;
+      }
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+        *reinterpret_cast<f32x4_t*>(&s_ex[wave][col][16 * d + quad * 4]) = o[rt][d];
+      __syncthreads();
+      float M = -INFINITY, L = 0.f, acc[DT];
+#pragma unroll
+      for (int i = 0; i < DT; ++i) acc[i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < kThinWaves; ++k) M = fmaxf(M, s_ml[k][er][0]);
+#pragma unroll
+      for (int k = 0; k < kThinWaves; ++k) {
+        const float a = state_weight(s_ml[k][er][0], M);
+        L += s_ml[k][er][1] * a;
+#pragma unroll
+        for (int i = 0; i < DT; ++i) acc[i] += s_ex[k][er][ed + i] * a;
+      }
+      const int row = rt * 16 + er;
+      if (!cut) {
+        finish(row, M, L, acc);
+      } else {
+        float* dst = part + row * (D + 2);
+#pragma unroll
+        for (int i = 0; i < DT; i += 2) st_pair(dst + ed + i, acc[i], acc[i + 1]);
+        if ((tid & 15) == 0) st_pair(dst + D, M, L);
+      }
+    }
+
+    if (cut) {
+      // The tile's last piece to arrive joins them all, in their order (the
+      // result does not depend on who does). Piece stores are agent scope and
+      // waited for before the count rises, so no cache holds an older copy.
+      const int first = head_piece ? share.first : w;
+      const int npieces = p.v.thin_share[first].last - first + 1;
+      wait_vm_stores();
+      __syncthreads();
+      if (tid == 0)
+        s_last = (int)__hip_atomic_fetch_add(p.thin_done + first, 1u, __ATOMIC_RELAXED,
+                                             __HIP_MEMORY_SCOPE_AGENT) == npieces - 1;
+      __syncthreads();
+      if (s_last) {
+        if (tid == 0) st_word(p.thin_done + first, 0u);
+        for (int r0 = 0; r0 < rows; r0 += 16) {
+          const int row = r0 + er;
+          if (row >= rows) break;
+          float M = -INFINITY, L = 0.f, acc[DT];
+#pragma unroll
+          for (int i = 0; i < DT; ++i) acc[i] = 0.f;
+          for (int k = 0; k < npieces; ++k) {
+            const float* src = p.thin_part + (size_t)(2 * (first + k) + (k == 0 ? 1 : 0)) *
+                                                 kThinRows * (D + 2) + row * (D + 2);
+            float ml[2], a[DT];
+            ld_pair(src + D, ml);
+#pragma unroll
+            for (int i = 0; i < DT; i += 2) ld_pair(src + ed + i, a + i);
+            const float mn = fmaxf(M, ml[0]);
+            const float sa = state_weight(M, mn), sb = state_weight(ml[0], mn);
+            L = L * sa + ml[1] * sb;
+#pragma unroll
+            for (int i = 0; i < DT; ++i) acc[i] = acc[i] * sa + a[i] * sb;
+            M = mn;
+          }
+          finish(row, M, L, acc);
+        }
+      }
+    }
+    left -= seg;
+    u0 = 0;
+    head_piece = false;
+    if (++ti == tiles) {
+      ti = 0;
+      ++h;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Wide sequences
+// ---------------------------------------------------------------------------
+// A workgroup of 8 waves takes a tile of 256 rows, each wave 32 of them, and
+// streams its share of the tile's pages four at a time: K and V rows staged
+// in LDS once, the next four in flight during the math, one barrier each.
+// Per wave (v_mfma_f32_32x32x16; lane l holds A[l%32][8*(l/32)+j],
+// B[8*(l/32)+j][l%32] and accumulator element i at
+// [8*(i/4) + 4*(l/32) + i%4][l%32]):
+//   S^T (keys x rows) = K . Q^T, so each lane owns one row: the max and sum
+//   are 16 values in the lane plus one exchange with lane l^32, and
+//   O^T (d x rows) += V^T . P^T takes the probabilities from the accumulator
+//   as they lie; V^T comes from row-major LDS through transposing reads.
+// f32 runs on v_mfma_f32_32x32x2_f32: lane half h contracts dimension
+// h*D/2 + j at step j of S^T, and for O^T step j pairs the two keys the lane
+// halves hold in accumulator element j.
+constexpr int kWideWaves = 8;
+constexpr int kWideThreads = 64 * kWideWaves;
+constexpr int kWideKeys = 16 * kWidePages;
+
+template <typename T, int D>
+struct WideLds {
+  // Row strides that put the rows one read takes together on banks of their
+  // own (64 four-byte banks): 16-bit K rows 4 banks apart, V rows of a
+  // transposing read 16; f32 K rows 4, the V rows of the lane halves 32.
+  static constexpr int kPadK = sizeof(T) == 2 ? 8 : 4;
+  static constexpr int kPadV = sizeof(T) == 2 ? 32 : 8;
+  T k[2][kWideKeys][D + kPadK];
+  T v[2][kWideKeys][D + kPadV];
+};
+
+template <typename T, int D>
+__global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams p) {
+  constexpr int ES = (int)sizeof(T);
+  constexpr int DB = D / 32;                      // 32-dimension blocks of O^T
+  constexpr int KB = D * ES / 32;                 // 16-byte packets of a lane's query
+  constexpr int PPR = D * ES / 16;                // packets per row
+  constexpr int KPT = kWideKeys * PPR / kWideThreads;  // packets per thread and stage
+  __shared__ __align__(16) WideLds<T, D> s;
+  __shared__ int s_odd[2];  // the stage holds a value of V that is not finite
+
+  if (p.v.head->stamp != p.stamp) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) ws_raise(&p.v.head->flags, RLSE_WS_ERR_PLAN);
+    return;
+  }
+  const int groups = p.v.head->wide_groups, tiles = p.v.head->wide_tiles;
+  if ((int)blockIdx.x >= groups) return;
+  const int w = share_index(blockIdx.x, groups);
+  const ChunkShare share = p.v.wide_share[w];
+
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int half = lane >> 5, col = lane & 31;
+  const int Hq = p.Hq, Hkv = p.Hkv, G = p.G;
+  const int sink_pages = (p.sinks + 15) >> 4;
+  const T* __restrict__ qb = static_cast<const T*>(p.q);
+  const T* __restrict__ kp = static_cast<const T*>(p.k_pool);
+  const T* __restrict__ vp = static_cast<const T*>(p.v_pool);
+
+  // Packet j of this thread in a stage: key kk, 16-byte chunk dc of its row.
+  // Its page, kk >> 4, is the same for the whole wave.
+  int voff[KPT], pg_of[KPT];
+#pragma unroll
+  for (int j = 0; j < KPT; ++j) {
+    const int pk = tid + j * kWideThreads;
+    const int kk = pk / PPR, dc = pk - kk * PPR;
+    voff[j] = (kk & 15) * D * ES + dc * 16;
+    pg_of[j] = __builtin_amdgcn_readfirstlane(kk >> 4);
+  }
+  // Transposing V reads: within a 16-lane group lane 4j + a points at key row
+  // j, columns 4a ..; half h takes keys 4h .. and 8 + 4h ..
+  const int tr_g = lane >> 4, tr_j = (lane & 15) >> 2, tr_a = lane & 3;
+  const int tr_row = (tr_g >> 1) * 4 + tr_j, tr_col = (tr_g & 1) * 16 + tr_a * 4;
+
+  int ti = __builtin_amdgcn_readfirstlane(share.tile);
+  int h = __builtin_amdgcn_readfirstlane(share.head);
+  int u0 = __builtin_amdgcn_readfirstlane(share.u0);
+  int left = __builtin_amdgcn_readfirstlane(share.count);
+  bool head_piece = u0 > 0;
+  while (left > 0) {
+    const ChunkTile t = p.v.wide[ti];
+    const int n = __builtin_amdgcn_readfirstlane(t.n), off = __builtin_amdgcn_readfirstlane(t.off);
+    const int tok0 = __builtin_amdgcn_readfirstlane(t.tok0);
+    const int row0 = __builtin_amdgcn_readfirstlane(t.row0);
+    const int wp0 = __builtin_amdgcn_readfirstlane(t.wp0);
+    const int pages = __builtin_amdgcn_readfirstlane(t.pages);
+    const int* __restrict__ table =
+        p.tables + (size_t)__builtin_amdgcn_readfirstlane(t.seq) * p.mbps;
+    const int units = (pages + kWidePages - 1) / kWidePages;
+    const int seg = min(left, units - u0);
+    const int rows = n * G;
+    const int last_row = min(rows, row0 + kWideRows) - 1;
+    const int kend = off + last_row / G + 1;  // keys the tile's rows see end here
+
+    const int wrow = row0 + wave * 32;
+    const bool live = wrow < rows;  // the wave has rows (else it only stages)
+    const int myrow = wrow + col;
+    const int row_c = min(myrow, rows - 1);
+    const int tok = row_c / G, qh = h * G + row_c - tok * G;
+    const RowSpan span = row_span(off, tok, p.window);
+    // Every row of the wave sees keys up to the first one's own, and from the
+    // last one's window on.
+    const int kmin = off + min(wrow, rows - 1) / G;
+    const int wlo_max = p.window > 0 ? off + min(wrow + 31, rows - 1) / G - p.window + 1 : 0;
+    // The same for the whole tile (its stages with keys some row masks).
+    const int kmin_t = off + row0 / G;
+    const int wlo_max_t = p.window > 0 ? kend - p.window : 0;
+
+    // Virtual pages 4u .. 4u+3 of unit u: positions of their first keys and
+    // ids (-1: none).
+    struct Stage {
+      int pos[kWidePages], id[kWidePages];
+    };
+    auto stage_of = [&](int u) __attribute__((always_inline)) {
+      Stage st;
+#pragma unroll
+      for (int i = 0; i < kWidePages; ++i) {
+        const int vi = u * kWidePages + i;
+        const int pg = real_page(min(vi, pages - 1), wp0, sink_pages);
+        const int id = table[pg];
+        st.pos[i] = pg * 16;
+        st.id[i] = vi < pages && (unsigned)id < (unsigned)p.num_blocks ? id : -1;
+      }
+      return st;
+    };
+    auto tile_whole = [&](const Stage& st, int kmin_, int wlo_) __attribute__((always_inline)) {
+      bool all = true;
+#pragma unroll
+      for (int i = 0; i < kWidePages; ++i)
+        all = all && st.id[i] >= 0 && st.pos[i] + 15 <= kmin_ &&
+              (st.pos[i] >= wlo_ || st.pos[i] + 16 <= p.sinks);
+      return all;
+    };
+
+    uint4 q[KB];
+    {
+      const T* src = qb + ((size_t)(tok0 + tok) * Hq + qh) * D;
+#pragma unroll
+      for (int i = 0; i < KB; ++i) {
+        // 16-bit: elements 16 i + 8 half ..; f32: half * D/2 + 4 i ..
+        const int at = ES == 2 ? i * 16 + half * 8 : half * (D / 2) + i * 4;
+        q[i] = *reinterpret_cast<const uint4*>(src + at);
+      }
+    }
+    f32x16_t o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+    float m = -INFINITY, lsum = 0.f;
+
+    u32x4_t kst[KPT], vst[KPT];
+    auto load = [&](const Stage& st) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < KPT; ++j) {
+        int id = st.id[0], pos = st.pos[0];
+#pragma unroll
+        for (int i = 1; i < kWidePages; ++i)
+          if (pg_of[j] == i) {
+            id = st.id[i];
+            pos = st.pos[i];
+          }
+        const size_t at = ((size_t)(id < 0 ? 0 : id) * Hkv + h) * 16 * D;
+        const int rec = id < 0 ? 0 : min(max(kend - pos, 0), 16) * D * ES;
+        const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(kp + at), 0, rec,
+                                                          kBufferWord3);
+        const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(vp + at), 0, rec,
+                                                          kBufferWord3);
+        kst[j] = __builtin_amdgcn_raw_buffer_load_b128(rk, voff[j], 0, 0);
+        vst[j] = __builtin_amdgcn_raw_buffer_load_b128(rv, voff[j], 0, 0);
+      }
+    };
+    auto store = [&](int bf, bool whole) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < KPT; ++j) {
+        const int pk = tid + j * kWideThreads;
+        const int kk = pk / PPR, dc = pk - kk * PPR;
+        *reinterpret_cast<u32x4_t*>(&s.k[bf][kk][dc * (16 / ES)]) = kst[j];
+        *reinterpret_cast<u32x4_t*>(&s.v[bf][kk][dc * (16 / ES)]) = vst[j];
+      }
+      if (!whole) {
+        bool odd = false;
+#pragma unroll
+        for (int j = 0; j < KPT; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t x = vst[j][i];
+            if constexpr (ES == 2) {
+              constexpr uint32_t inf = Tile<T>::kInf;
+              odd = odd || (x & inf) == inf || (x & inf << 16) == inf << 16;
+            } else {
+              odd = odd || (x & 0x7f800000u) == 0x7f800000u;
+            }
+          }
+        if (odd) s_odd[bf] = 1;
+      }
+    };
+
+    __syncthreads();  // the stages of the segment before are read
+    if (tid < 2) s_odd[tid] = 0;
+    __syncthreads();
+    const int u_end = u0 + seg;
+    Stage cur = stage_of(u0);
+    load(cur);
+    store(0, tile_whole(cur, kmin_t, wlo_max_t));
+    Stage next = stage_of(min(u0 + 1, u_end - 1));
+    __syncthreads();
+    int bf = 0;
+    for (int u = u0;; ++u) {
+      const bool more = u + 1 < u_end;
+      load(next);  // in flight during this stage's math
+      const Stage after = stage_of(min(u + 2, u_end - 1));
+      if (live) {
+        const bool whole = tile_whole(cur, kmin, wlo_max);
+        f32x16_t x[2];
+#pragma unroll
+        for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[sb][i] = 0.f;
+        if constexpr (ES == 2) {
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int sb = 0; sb < 2; ++sb)
+              x[sb] = Tile<T>::mma32(
+                  *reinterpret_cast<const uint4*>(&s.k[bf][sb * 32 + col][kb * 16 + half * 8]),
+                  q[kb], x[sb]);
+        } else {
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int sb = 0; sb < 2; ++sb) {
+              const float4 a = *reinterpret_cast<const float4*>(
+                  &s.k[bf][sb * 32 + col][half * (D / 2) + kb * 4]);
+              const float4 b = __builtin_bit_cast(float4, q[kb]);
+              x[sb] = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x, b.x, x[sb], 0, 0, 0);
+              x[sb] = __builtin_amdgcn_mfma_f32_32x32x2f32(a.y, b.y, x[sb], 0, 0, 0);
+              x[sb] = __builtin_amdgcn_mfma_f32_32x32x2f32(a.z, b.z, x[sb], 0, 0, 0);
+              x[sb] = __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, b.w, x[sb], 0, 0, 0);
+            }
+        }
+        if (!whole) {
+#pragma unroll
+          for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int kk = sb * 32 + (i >> 2) * 8 + half * 4 + (i & 3);
+              const int pg = sb * 2 + (i >> 3);
+              if (!(cur.id[pg] >= 0 && span.sees(cur.pos[pg] + (kk & 15), p.sinks)))
+                x[sb][i] = -INFINITY;
+            }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[sb][i]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float cand = mx * p.c;
+        if (__any(cand > m + kLazyLog2)) {
+          const float mn = fmaxf(m, cand);
+          const float a = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+          lsum *= a;
+#pragma unroll
+          for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] *= a;
+          m = mn;
+        }
+        const float nm = m == -INFINITY ? 0.f : -m;
+        float rs = 0.f;
+#pragma unroll
+        for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            x[sb][i] = __builtin_amdgcn_exp2f(fmaf(x[sb][i], p.c, nm));
+            rs += x[sb][i];
+          }
+        rs += __shfl_xor(rs, 32, 64);
+        lsum += rs;
+        const bool apart = !whole && s_odd[bf] != 0;
+        if constexpr (ES == 2) {
+          uint4 pk[4];  // P^T operands of the four 16-key blocks
+#pragma unroll
+          for (int kq = 0; kq < 4; ++kq) {
+            const f32x16_t& y = x[kq >> 1];
+            const int e = (kq & 1) * 8;
+            pk[kq] = make_uint4(
+                Packet<T>::pack2(y[e], y[e + 1]), Packet<T>::pack2(y[e + 2], y[e + 3]),
+                Packet<T>::pack2(y[e + 4], y[e + 5]), Packet<T>::pack2(y[e + 6], y[e + 7]));
+          }
+          auto vt = [&](int kq, int d) __attribute__((always_inline)) {
+            const uint16_t* v0 =
+                reinterpret_cast<const uint16_t*>(&s.v[bf][kq * 16 + tr_row][d * 32 + tr_col]);
+            const uint2 lo = __builtin_bit_cast(
+                uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)v0));
+            const uint2 hi = __builtin_bit_cast(
+                uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                           (lds_i16x4_t*)(v0 + 8 * (D + WideLds<T, D>::kPadV))));
+            return make_uint4(lo.x, lo.y, hi.x, hi.y);
+          };
+          if (!apart) {
+#pragma unroll
+            for (int kq = 0; kq < 4; ++kq)
+#pragma unroll
+              for (int d = 0; d < DB; ++d) o[d] = Tile<T>::mma32(vt(kq, d), pk[kq], o[d]);
+          } else {
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+              f32x16_t cp, cn;
+#pragma unroll
+              for (int i = 0; i < 16; ++i) cp[i] = cn[i] = 0.f;
+#pragma unroll
+              for (int kq = 0; kq < 4; ++kq) {
+                const uint4 a = vt(kq, d);
+                uint4 pos, neg;
+                const uint4 fin = make_uint4(
+                    split_word<T>(a.x, &pos.x, &neg.x), split_word<T>(a.y, &pos.y, &neg.y),
+                    split_word<T>(a.z, &pos.z, &neg.z), split_word<T>(a.w, &pos.w, &neg.w));
+                const uint4 see = make_uint4(seen_word<T>(pk[kq].x), seen_word<T>(pk[kq].y),
+                                             seen_word<T>(pk[kq].z), seen_word<T>(pk[kq].w));
+                o[d] = Tile<T>::mma32(fin, pk[kq], o[d]);
+                cp = Tile<T>::mma32(pos, see, cp);
+                cn = Tile<T>::mma32(neg, see, cn);
+              }
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[d][i] += not_finite(cp[i], cn[i]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int d = 0; d < DB; ++d) {
+            f32x16_t cp, cn;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) cp[i] = cn[i] = 0.f;
+#pragma unroll
+            for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                const float a =
+                    s.v[bf][sb * 32 + (j >> 2) * 8 + half * 4 + (j & 3)][d * 32 + col];
+                if (!apart) {
+                  o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, x[sb][j], o[d], 0, 0, 0);
+                } else {
+                  float pos, neg;
+                  const float fin = split_word(a, &pos, &neg);
+                  const float see = x[sb][j] != 0.f ? 1.f : 0.f;
+                  o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(fin, x[sb][j], o[d], 0, 0, 0);
+                  cp = __builtin_amdgcn_mfma_f32_32x32x2f32(pos, see, cp, 0, 0, 0);
+                  cn = __builtin_amdgcn_mfma_f32_32x32x2f32(neg, see, cn, 0, 0, 0);
+                }
+              }
+            if (apart)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[d][i] += not_finite(cp[i], cn[i]);
+          }
+        }
+      }
+      if (!more) break;
+      cur = next;
+      next = after;
+      store(bf ^ 1, tile_whole(cur, kmin_t, wlo_max_t));
+      __syncthreads();
+      bf ^= 1;
+    }
+
+    // Lane holds O^T rows d = 32 db + 8 (i/4) + 4 half + i%4 of its row.
+    if (seg == units) {
+      if (myrow < rows) {
+        const size_t at = (size_t)(tok0 + tok) * Hq + qh;
+        T* dst = static_cast<T*>(p.out) + at * D;
+        const float inv = inverse_sum(lsum);
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int i4 = 0; i4 < 4; ++i4) {
+            const float v[4] = {o[d][i4 * 4], o[d][i4 * 4 + 1], o[d][i4 * 4 + 2],
+                                o[d][i4 * 4 + 3]};
+            write_row<T, 4>(dst + d * 32 + i4 * 8 + half * 4, v, inv);
+          }
+        if (p.lse && half == 0) p.lse[at] = state_lse(m, lsum);
+      }
+    } else if (live) {
+      // The partial state in register order: float4 slot k of thread tid, so
+      // every store covers 1 KB of consecutive bytes.
+      float4* part = p.wide_part +
+                     (size_t)(2 * w + (head_piece ? 0 : 1)) * (4 * DB + 1) * kWideThreads + tid;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i4 = 0; i4 < 4; ++i4)
+          part[(d * 4 + i4) * kWideThreads] = make_float4(o[d][i4 * 4], o[d][i4 * 4 + 1],
+                                                          o[d][i4 * 4 + 2], o[d][i4 * 4 + 3]);
+      part[4 * DB * kWideThreads] = make_float4(m, lsum, 0.f, 0.f);
+    }
+    left -= seg;
+    u0 = 0;
+    head_piece = false;
+    if (++ti == tiles) {
+      ti = 0;
+      ++h;
+    }
+  }
+}
+
+// Joins the pieces of the wide tiles that the shares cut: workgroup (w, d)
+// dimension block d of the tile that workgroup w's share ends in, if others
+// hold the rest of it. The pieces combine online in their order.
+template <typename T, int D>
+__global__ __launch_bounds__(kWideThreads) void chunk_merge_kernel(ChunkParams p) {
+  constexpr int DB = D / 32;
+  if (p.v.head->stamp != p.stamp) return;
+  const int w = blockIdx.x / DB, d = blockIdx.x % DB;
+  const int groups = p.v.head->wide_groups;
+  if (w >= groups) return;
+  const ChunkShare share = p.v.wide_share[w];
+  if (share.last == w) return;
+  // The tile the share ends in, and its head.
+  const int tiles = p.v.head->wide_tiles, units = p.v.head->wide_units;
+  const long long end =
+      (long long)share.head * units + p.v.wide[share.tile].unit0 + share.u0 + share.count - 1;
+  const int h = (int)(end / units), u = (int)(end - (long long)h * units);
+  int lo = 0, hi = tiles;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (p.v.wide[mid].unit0 <= u) lo = mid; else hi = mid;
+  }
+  const ChunkTile t = p.v.wide[lo];
+  // (A share inside one tile of three pieces or more: its first piece's
+  // workgroup joins it.)
+  const long long begin = (long long)share.head * units + p.v.wide[share.tile].unit0 + share.u0;
+  if ((long long)h * units + t.unit0 < begin) return;
+
+  const int tid = threadIdx.x;
+  const int wave = tid >> 6, lane = tid & 63, half = lane >> 5, col = lane & 31;
+  const int row = t.row0 + wave * 32 + col, rows = t.n * p.G;
+  if (row >= rows) return;
+  float M = -INFINITY, L = 0.f, acc[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+  for (int k = w; k <= share.last; ++k) {
+    const float4* part = p.wide_part +
+                         (size_t)(2 * k + (k == w ? 1 : 0)) * (4 * DB + 1) * kWideThreads + tid;
+    const float4 ml = part[4 * DB * kWideThreads];
+    float4 a[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = part[(d * 4 + i) * kWideThreads];
+    const float mn = fmaxf(M, ml.x);
+    const float sa = state_weight(M, mn), sb = state_weight(ml.x, mn);
+    L = L * sa + ml.y * sb;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      acc[i * 4] = acc[i * 4] * sa + a[i].x * sb;
+      acc[i * 4 + 1] = acc[i * 4 + 1] * sa + a[i].y * sb;
+      acc[i * 4 + 2] = acc[i * 4 + 2] * sa + a[i].z * sb;
+      acc[i * 4 + 3] = acc[i * 4 + 3] * sa + a[i].w * sb;
+    }
+    M = mn;
+  }
+  const int tok = row / p.G;
+  const size_t at = (size_t)(t.tok0 + tok) * p.Hq + h * p.G + row - tok * p.G;
+  T* dst = static_cast<T*>(p.out) + at * D + d * 32;
+  const float inv = inverse_sum(L);
+#pragma unroll
+  for (int i4 = 0; i4 < 4; ++i4) write_row<T, 4>(dst + i4 * 8 + half * 4, acc + i4 * 4, inv);
+  if (p.lse && d == 0 && half == 0) p.lse[at] = state_lse(M, L);
+}
+
+// Workspace: header (word 0 unused by these kernels' errors, which the plan
+// holds), the thin tiles' piece counts, then the pieces.
+struct ChunkWorkspace {
+  size_t done, thin, wide, bytes;
+};
+ChunkWorkspace chunk_workspace(int max_rows, int D, int cus) {
+  ChunkWorkspace ws;
+  ws.done = 256;
+  ws.thin = ws.done + ((size_t)2 * cus * sizeof(uint32_t) + 255) / 256 * 256;
+  ws.wide = ws.thin + (size_t)4 * cus * kThinRows * (D + 2) * sizeof(float);
+  ws.bytes = ws.wide;
+  if (max_rows > kThinRows)
+    ws.bytes += (size_t)2 * cus * (D / 8 + 1) * kWideThreads * sizeof(float4);
+  return ws;
+}
+
+template <typename T, int D>
+int launch_chunk(const ChunkParams& p, int max_rows, int thin_rows, int cus, hipStream_t stream) {
+  int st = RLSE_OK;
+  if (thin_rows > 0) {
+    const dim3 grid(2 * cus), block(kThinThreads);
+    if (max_rows <= 16)
+      hipLaunchKernelGGL((chunk_thin_kernel<T, D, 1>), grid, block, 0, stream, p);
+    else
+      hipLaunchKernelGGL((chunk_thin_kernel<T, D, 2>), grid, block, 0, stream, p);
+    st = launch_status("chunk_thin_kernel");
+  }
+  if (st || max_rows <= thin_rows) return st;
+  hipLaunchKernelGGL((chunk_wide_kernel<T, D>), dim3(cus), dim3(kWideThreads), 0, stream, p);
+  st = launch_status("chunk_wide_kernel");
+  if (st) return st;
+  hipLaunchKernelGGL((chunk_merge_kernel<T, D>), dim3(cus * (D / 32)), dim3(kWideThreads), 0,
+                     stream, p);
+  return launch_status("chunk_merge_kernel");
+}
+
+}  // namespace
+}  // namespace rlse
+
+using namespace rlse;
+
+extern "C" int rlse_chunk_workspace_size(int num_seqs, int total_tokens, int max_tokens,
+                                         int num_heads, int num_kv_heads, int head_dim,
+                                         size_t* bytes) {
+  if (!bytes) return fail(RLSE_ERR_INVALID_VALUE, "chunk_workspace_size: null output");
+  int st = validate_chunk_shape("chunk_workspace_size", num_seqs, total_tokens, max_tokens,
+                                num_heads, num_kv_heads, 1, 0, 0);
+  if (st) return st;
+  if (head_dim != 64 && head_dim != 128)
+    return fail(RLSE_ERR_INVALID_VALUE, "chunk_workspace_size: head_dim %d not in {64, 128}",
+                head_dim);
+  int cus = 0;
+  st = device_cu_count(&cus);
+  if (st) return st;
+  *bytes = chunk_workspace(max_tokens * (num_heads / num_kv_heads), head_dim, cus).bytes;
+  return RLSE_OK;
+}
+
+extern "C" int rlse_chunk_attn(const void* q, const void* k_pool, const void* v_pool,
+                               const int32_t* block_tables, void* plan, void* out, float* lse,
+                               int num_seqs, int total_tokens, int max_tokens, int num_heads,
+                               int num_kv_heads, int head_dim, int max_blocks_per_seq,
+                               int num_blocks, int window, int sinks, float scale, int dtype,
+                               void* workspace, size_t workspace_bytes, rlse_stream_t stream) {
+  int st = validate_chunk_shape("chunk_attn", num_seqs, total_tokens, max_tokens, num_heads,
+                                num_kv_heads, max_blocks_per_seq, window, sinks);
+  if (st) return st;
+  if (head_dim != 64 && head_dim != 128)
+    return fail(RLSE_ERR_INVALID_VALUE, "chunk_attn: head_dim %d not in {64, 128}", head_dim);
+  if (dtype != RLSE_DTYPE_BF16 && dtype != RLSE_DTYPE_F16 && dtype != RLSE_DTYPE_F32)
+    return fail(RLSE_ERR_INVALID_VALUE, "chunk_attn: bad dtype %d", dtype);
+  if (num_blocks <= 0)
+    return fail(RLSE_ERR_INVALID_VALUE, "chunk_attn: num_blocks %d", num_blocks);
+  if (!(scale > 0.f) || !isfinite(scale))
+    return fail(RLSE_ERR_INVALID_VALUE, "chunk_attn: scale must be finite and positive");
+  if (!q || !k_pool || !v_pool || !block_tables || !plan || !out || !workspace)
+    return fail(RLSE_ERR_INVALID_VALUE, "chunk_attn: null pointer argument");
+  const uintptr_t align = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_pool) |
+                          reinterpret_cast<uintptr_t>(v_pool) | reinterpret_cast<uintptr_t>(plan) |
+                          reinterpret_cast<uintptr_t>(out) |
+                          reinterpret_cast<uintptr_t>(workspace);
+  if (align & 15)
+    return fail(RLSE_ERR_INVALID_VALUE, "chunk_attn: a buffer is not 16-byte aligned");
+  int cus = 0;
+  st = device_cu_count(&cus);
+  if (st) return st;
+  ChunkParams p{};
+  p.G = num_heads / num_kv_heads;
+  const int max_rows = max_tokens * p.G;
+  const ChunkWorkspace ws = chunk_workspace(max_rows, head_dim, cus);
+  if (workspace_bytes < ws.bytes)
+    return fail(RLSE_ERR_BUFFER_TOO_SMALL, "chunk_attn: workspace %zu bytes < %zu needed",
+                workspace_bytes, ws.bytes);
+  char* base = static_cast<char*>(workspace);
+  p.q = q;
+  p.k_pool = k_pool;
+  p.v_pool = v_pool;
+  p.tables = block_tables;
+  p.out = out;
+  p.lse = lse;
+  p.v = chunk_plan_view(plan, num_seqs, total_tokens, p.G, cus);
+  p.stamp = chunk_stamp({num_seqs, total_tokens, max_tokens, num_heads, num_kv_heads,
+                         max_blocks_per_seq, window, sinks, cus});
+  p.thin_done = reinterpret_cast<uint32_t*>(base + ws.done);
+  p.thin_part = reinterpret_cast<float*>(base + ws.thin);
+  p.wide_part = reinterpret_cast<float4*>(base + ws.wide);
+  p.Hq = num_heads;
+  p.Hkv = num_kv_heads;
+  p.mbps = max_blocks_per_seq;
+  p.num_blocks = num_blocks;
+  p.window = window;
+  p.sinks = sinks;
+  p.c = scale * 1.4426950408889634f;
+  const hipStream_t s = as_stream(stream);
+  auto run = [&](auto t, auto d) {
+    using T = decltype(t);
+    constexpr int D = decltype(d)::value;
+    return launch_chunk<T, D>(p, max_rows, thin_row_limit(num_seqs, max_rows), cus, s);
+  };
+  const std::integral_constant<int, 64> d64;
+  const std::integral_constant<int, 128> d128;
+  if (dtype == RLSE_DTYPE_BF16) return head_dim == 128 ? run(bf16{}, d128) : run(bf16{}, d64);
+  if (dtype == RLSE_DTYPE_F16) return head_dim == 128 ? run(f16{}, d128) : run(f16{}, d64);
+  return head_dim == 128 ? run(float{}, d128) : run(float{}, d64);
+}

@@ -1,0 +1,141 @@
+// The plan of a ragged step: which tiles of query rows its sequences make,
+// which keys each tile reads, and which workgroup takes which of them. Built
+// once per step on the device (chunk_plan_kernel) and read by every layer's
+// attention and key-weight launches.
+//
+// Sequence b has n = cu_tokens[b+1] - cu_tokens[b] new tokens at positions
+// off .. off+n-1, off = seq_lens[b] - n. For a KV head its n*G rows (row =
+// t*G + g) are tiled: a thin sequence (n*G <= kThinRows) is one tile, of rows
+// that fit one or two MFMA columns blocks and whose keys every wave reads once;
+// a wide one takes tiles of kWideRows rows that share each key through LDS.
+//
+// A tile reads the pages that hold a key one of its rows sees. Under a window
+// these are the sinks' pages and the pages from the first row's window start
+// to the last row's own key: virtual page i is table entry i for i < the sink
+// pages, else i - sink pages + wp0 (wp0 = 0: no gap, i itself).
+//
+// Work units (thin: a page; wide: four pages) of all (KV head, tile) pairs,
+// heads outermost, are laid end to end and dealt to the workgroups in equal
+// contiguous shares, so ragged lengths balance; a tile cut by a share's end
+// leaves partial softmax states that a merge joins.
+#pragma once
+
+#include "common.cuh"
+
+namespace rlse {
+
+constexpr int kThinRows = 32;       // rows (tokens * group size) of a thin sequence at most
+constexpr int kWideRows = 256;      // rows per wide tile
+constexpr int kWidePages = 4;       // pages per wide unit
+constexpr int kScorePages = 16;     // pages per unit of the wide key-weight launch
+constexpr int kMaxChunkSeqs = 4096; // prefix tables of the plan launch live in LDS
+constexpr int kThinMinUnits = 8;    // smallest share of a workgroup: pages,
+constexpr int kWideMinUnits = 4;    //   and wide units
+
+// Rows of a thin sequence at most in a step of num_seqs sequences of up to
+// max_rows rows. A single sequence that may be wide is taken as wide whatever
+// it turns out to have: the step then has no thin launch.
+__host__ __device__ inline int thin_row_limit(int num_seqs, int max_rows) {
+  return num_seqs == 1 && max_rows > kThinRows ? 0 : kThinRows;
+}
+
+struct ChunkTile {
+  int unit0;     // units of this list's tiles before it (of one KV head)
+  int seq;
+  int tok0;      // cu_tokens[seq]
+  int n;         // new tokens
+  int off;       // keys before them
+  int row0;      // first row of the tile
+  int wp0;       // first page after the sinks' (0: the pages are 0, 1, ...)
+  int pages;     // virtual pages
+};
+
+// A workgroup's share of a list: units u0 .. of (head, tile), count in all,
+// going on through the following tiles. first: the workgroup that holds the
+// start of that first tile; last: the one that holds the end of the tile the
+// share ends in (w itself where it ends with a whole tile).
+struct ChunkShare {
+  int tile, head, u0, count, first, last, pad0, pad1;
+};
+
+struct ChunkHead {
+  uint32_t flags;  // RLSE_WS_ERR_* of this step
+  uint32_t stamp;  // chunk_stamp of the call that built the plan
+  int thin_tiles, thin_units, thin_groups;
+  int wide_tiles, wide_units, wide_groups;
+  int score_seqs, score_units;  // wide sequences, and their key blocks
+};
+constexpr int kChunkHeadBytes = 256;
+
+// What the plan's users agree on, in one word (FNV-1a over the arguments).
+struct ChunkShape {
+  int num_seqs, total_tokens, max_tokens, Hq, Hkv, mbps, window, sinks, cus;
+};
+inline uint32_t chunk_stamp(const ChunkShape& s) {
+  const int v[9] = {s.num_seqs, s.total_tokens, s.max_tokens, s.Hq, s.Hkv,
+                    s.mbps, s.window, s.sinks, s.cus};
+  uint32_t h = 2166136261u;
+  for (int x : v)
+    for (int i = 0; i < 4; ++i) h = (h ^ ((uint32_t)x >> (8 * i) & 255u)) * 16777619u;
+  return h;
+}
+
+// Places of the plan's parts.
+struct ChunkPlanView {
+  ChunkHead* head;
+  ChunkTile* thin;    // [num_seqs]
+  ChunkTile* score;   // [num_seqs]: wide sequences, all their rows
+  ChunkTile* wide;    // [wide_cap]
+  ChunkShare* thin_share;  // [2 * cus]
+  ChunkShare* wide_share;  // [cus]
+};
+__host__ __device__ inline long long wide_tile_cap(long long total_tokens, int G, int num_seqs) {
+  return total_tokens * G / kWideRows + num_seqs;
+}
+__host__ __device__ inline size_t chunk_plan_bytes(int num_seqs, int total_tokens, int G, int cus) {
+  return kChunkHeadBytes +
+         sizeof(ChunkTile) * (size_t)(2LL * num_seqs + wide_tile_cap(total_tokens, G, num_seqs)) +
+         sizeof(ChunkShare) * (size_t)(3 * cus);
+}
+__host__ __device__ inline ChunkPlanView chunk_plan_view(void* plan, int num_seqs,
+                                                         int total_tokens, int G, int cus) {
+  ChunkPlanView v;
+  char* p = static_cast<char*>(plan);
+  v.head = reinterpret_cast<ChunkHead*>(p);
+  v.thin = reinterpret_cast<ChunkTile*>(p + kChunkHeadBytes);
+  v.score = v.thin + num_seqs;
+  v.wide = v.score + num_seqs;
+  v.thin_share = reinterpret_cast<ChunkShare*>(v.wide + wide_tile_cap(total_tokens, G, num_seqs));
+  v.wide_share = v.thin_share + 2 * cus;
+  return v;
+}
+
+// Pages of a sequence's tile: tokens t0 .. t1 of off + n keys.
+__device__ __forceinline__ void tile_pages(int off, int t0, int t1, int window, int sinks, int* wp0,
+                                           int* pages) {
+  const int end = (off + t1 + 16) >> 4;  // pages up to the last row's own key
+  *wp0 = 0;
+  *pages = end;
+  if (window > 0) {
+    const int lo = off + t0 - window + 1;
+    const int sp = (sinks + 15) >> 4;
+    if (lo > 0 && (lo >> 4) > sp) {
+      *wp0 = lo >> 4;
+      *pages = sp + end - *wp0;
+    }
+  }
+}
+// Table entry of virtual page i.
+__device__ __forceinline__ int real_page(int i, int wp0, int sink_pages) {
+  return wp0 == 0 || i < sink_pages ? i : i - sink_pages + wp0;
+}
+
+// Workgroup b of the `groups` at work: workgroup b runs on XCD b % 8, so each
+// XCD gets a contiguous run of shares (neighbouring shares read one head's
+// keys) and few shares still spread over all XCDs.
+__device__ __forceinline__ int share_index(int b, int groups) {
+  const int x = b & 7, q = groups >> 3, r = groups & 7;
+  return x * q + min(x, r) + (b >> 3);
+}
+
+}  // namespace rlse

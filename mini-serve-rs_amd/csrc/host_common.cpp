@@ -83,6 +83,9 @@ int read_and_clear_ws_flags(void* workspace, hipStream_t stream, unsigned* flags
     return fail(RLSE_ERR_INVALID_VALUE,
                 "a cascade step's batch does not share its prefix pages, or a new token lies "
                 "inside them (flags 0x%x)", word);
+  if (word & RLSE_WS_ERR_PLAN)
+    return fail(RLSE_ERR_INVALID_VALUE,
+                "a ragged step's plan was built for other arguments (flags 0x%x)", word);
   return fail(RLSE_ERR_DEVICE_TIMEOUT, "unknown device error flags 0x%x", word);
 }
 

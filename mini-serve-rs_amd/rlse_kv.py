@@ -49,6 +49,7 @@ DECODE_STREAM = 1
 WS_ERR_MERGE_TIMEOUT = 1
 WS_ERR_LENGTH = 2
 WS_ERR_PREFIX = 4
+WS_ERR_PLAN = 8
 BLOCK_SIZE = 16
 
 # Every extern "C" symbol of include/rlse_kv.h (checked by the CPU tests).
@@ -82,6 +83,7 @@ EXPORTED = (
     "rlse_decode_step_noalloc", "rlse_decode_prefix_size", "rlse_decode_plan_cascade",
     "rlse_decode_step_cascade", "rlse_decode_plan_groups", "rlse_decode_step_groups",
     "rlse_kv_checksum", "rlse_kv_checksum_planned",
+    "rlse_chunk_plan_size", "rlse_chunk_plan", "rlse_chunk_workspace_size", "rlse_chunk_attn",
 )
 
 
@@ -208,6 +210,10 @@ _SIGS = {
     "rlse_prefill_workspace_size": (_i, [_i, _i, _i, _i, _i, ctypes.POINTER(_sz)]),
     "rlse_prefill_attn": (_i, [_vp, _vp, _vp, _vp, _i, _i, _vp, _i, _i, _i, _i, _i, _f, _i, _vp,
                                _sz, _vp]),
+    "rlse_chunk_plan_size": (_i, [_i, _i, _i, _i, ctypes.POINTER(_sz)]),
+    "rlse_chunk_plan": (_i, [_vp, _vp] + [_i] * 8 + [_vp, _sz, _vp]),
+    "rlse_chunk_workspace_size": (_i, [_i, _i, _i, _i, _i, _i, ctypes.POINTER(_sz)]),
+    "rlse_chunk_attn": (_i, [_vp] * 7 + [_i] * 10 + [_f, _i, _vp, _sz, _vp]),
     "rlse_rmsnorm": (_i, [_vp, _vp, _vp, _i, _i, _f, _i, _vp]),
     "rlse_rope_tables": (_i, [_d, _i, _i, _i, _vp, _vp]),
     "rlse_rope": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
@@ -915,6 +921,50 @@ def prefill_attn(q, k_pool, v_pool, block_table, ctx_len: int, num_tokens: int, 
                                     ctx_len, num_tokens, _ptr(out), num_heads, num_kv_heads,
                                     head_dim, max_blocks, num_blocks, scale, _dt(dtype),
                                     _ptr(workspace), workspace_bytes, _stream(stream)))
+
+
+def chunk_plan_size(num_seqs: int, total_tokens: int, num_heads: int, num_kv_heads: int) -> int:
+    """Bytes of a ragged step's plan (rlse_chunk_plan)."""
+    n = _sz(0)
+    _check(load().rlse_chunk_plan_size(num_seqs, total_tokens, num_heads, num_kv_heads,
+                                       ctypes.byref(n)))
+    return n.value
+
+
+def chunk_plan(cu_tokens, seq_lens, num_seqs: int, total_tokens: int, max_tokens: int,
+               num_heads: int, num_kv_heads: int, max_blocks_per_seq: int, window: int, sinks: int,
+               plan, plan_bytes: int, stream=None) -> None:
+    """Builds the plan that a ragged step's chunk_attn and kv_scores calls read:
+    sequence b's new tokens are rows cu_tokens[b] .. cu_tokens[b+1]-1, the last
+    of its seq_lens[b] keys. window 0: every earlier key is visible; else the
+    last `window` ones and the first `sinks`. workspace_check(plan) raises
+    for lengths that do not fit."""
+    _check(load().rlse_chunk_plan(_ptr(cu_tokens), _ptr(seq_lens), num_seqs, total_tokens,
+                                  max_tokens, num_heads, num_kv_heads, max_blocks_per_seq, window,
+                                  sinks, _ptr(plan), plan_bytes, _stream(stream)))
+
+
+def chunk_workspace_size(num_seqs: int, total_tokens: int, max_tokens: int, num_heads: int,
+                         num_kv_heads: int, head_dim: int) -> int:
+    """Bytes of chunk_attn's workspace; zero-fill it once before first use."""
+    n = _sz(0)
+    _check(load().rlse_chunk_workspace_size(num_seqs, total_tokens, max_tokens, num_heads,
+                                            num_kv_heads, head_dim, ctypes.byref(n)))
+    return n.value
+
+
+def chunk_attn(q, k_pool, v_pool, block_tables, plan, out, lse, num_seqs: int, total_tokens: int,
+               max_tokens: int, num_heads: int, num_kv_heads: int, head_dim: int,
+               max_blocks_per_seq: int, num_blocks: int, window: int, sinks: int, scale: float,
+               dtype, workspace, workspace_bytes: int, stream=None) -> None:
+    """Attention of a ragged step's new tokens over their sequences' pages,
+    every key up to their own or a sliding window and sinks; lse (f32
+    [total_tokens][num_heads], may be None) receives the log-sum-exp."""
+    _check(load().rlse_chunk_attn(_ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(block_tables),
+                                  _ptr(plan), _ptr(out), _ptr(lse), num_seqs, total_tokens,
+                                  max_tokens, num_heads, num_kv_heads, head_dim,
+                                  max_blocks_per_seq, num_blocks, window, sinks, scale, _dt(dtype),
+                                  _ptr(workspace), workspace_bytes, _stream(stream)))
 
 
 def rmsnorm(x, weight, out, rows: int, n: int, eps: float, dtype, stream=None) -> None:

@@ -1,0 +1,50 @@
+"""The ragged step's calls reject bad arguments before they touch a device."""
+import pytest
+
+GOOD = dict(n=2, total=10, most=8, hq=16, hkv=8, d=128, mbps=4, nb=64, window=0, sinks=0,
+            scale=0.1, dtype=1)
+
+
+def _plan(kv, **a):
+    return kv.load().rlse_chunk_plan(16, 16, a["n"], a["total"], a["most"], a["hq"], a["hkv"],
+                                     a["mbps"], a["window"], a["sinks"], 16, 1 << 40, None)
+
+
+def _attn(kv, ptr=16, **a):
+    return kv.load().rlse_chunk_attn(ptr, 16, 16, 16, 16, 16, None, a["n"], a["total"], a["most"],
+                                     a["hq"], a["hkv"], a["d"], a["mbps"], a["nb"], a["window"],
+                                     a["sinks"], a["scale"], a["dtype"], 16, 1 << 40, None)
+
+
+SHAPES = [dict(n=0), dict(n=4097), dict(total=0), dict(most=0), dict(most=11), dict(hq=12),
+          dict(hq=0), dict(hkv=0), dict(mbps=0), dict(mbps=1 << 25), dict(window=-1),
+          dict(sinks=-1), dict(total=1 << 24, hq=64)]
+
+
+@pytest.mark.parametrize("change", SHAPES, ids=str)
+def test_shapes(kv, change):
+    assert _plan(kv, **{**GOOD, **change}) == kv.ERR_INVALID_VALUE
+    assert "chunk_plan" in kv.last_error()
+    assert _attn(kv, **{**GOOD, **change}) == kv.ERR_INVALID_VALUE
+    assert "chunk_attn" in kv.last_error()
+
+
+@pytest.mark.parametrize("change", [dict(d=96), dict(dtype=7), dict(nb=0), dict(scale=0.0),
+                                    dict(scale=float("nan")), dict(scale=float("inf"))], ids=str)
+def test_attention_arguments(kv, change):
+    assert _attn(kv, **{**GOOD, **change}) == kv.ERR_INVALID_VALUE
+    assert "chunk_attn" in kv.last_error()
+
+
+def test_pointers(kv):
+    lib = kv.load()
+    assert _attn(kv, ptr=None, **GOOD) == kv.ERR_INVALID_VALUE
+    assert "null" in kv.last_error()
+    assert _attn(kv, ptr=24, **GOOD) == kv.ERR_INVALID_VALUE
+    assert "aligned" in kv.last_error()
+    assert lib.rlse_chunk_plan(None, 16, 1, 1, 1, 8, 8, 1, 0, 0, 16, 1 << 30,
+                               None) == kv.ERR_INVALID_VALUE
+    assert lib.rlse_chunk_plan(16, 16, 1, 1, 1, 8, 8, 1, 0, 0, 8, 1 << 30,
+                               None) == kv.ERR_INVALID_VALUE
+    assert lib.rlse_chunk_plan_size(1, 1, 8, 8, None) == kv.ERR_INVALID_VALUE
+    assert lib.rlse_chunk_workspace_size(1, 1, 1, 8, 8, 128, None) == kv.ERR_INVALID_VALUE
