@@ -459,6 +459,55 @@ int rlse_chunk_attn(const void* q, const void* k_pool, const void* v_pool,
                     float scale, int dtype, void* workspace, size_t workspace_bytes,
                     rlse_stream_t stream);
 
+/* The weight each cached key receives from the step's queries: for every key
+ * k < seq_lens[b] of a sequence with new tokens, scores [num_seqs]
+ * [num_kv_heads][max_blocks_per_seq*16] (float) becomes
+ *     (prev[b][h][k], if prev is given and k is older than the new tokens)
+ *   + sum over new tokens and the query heads of KV head h that see k of
+ *     e^(scale q.k - lse),
+ * lse being what rlse_chunk_attn gave for the same q, keys and plan. prev may
+ * be NULL (counted anew) or scores itself (added up in place from step to
+ * step); another overlap is not allowed. Slots from seq_lens[b] on, and
+ * sequences without new tokens, are left as they were. Keys of pages whose
+ * ids are out of range receive nothing; a row whose lse is -inf gives
+ * nothing. Each sum is formed in one order: the same call gives the same
+ * bits. Shapes, plan and dtypes as rlse_chunk_attn. */
+int rlse_kv_scores(const void* q, const void* k_pool, const int32_t* block_tables, void* plan,
+                   const float* lse, const float* prev, float* scores, int num_seqs,
+                   int total_tokens, int max_tokens, int num_heads, int num_kv_heads,
+                   int head_dim, int max_blocks_per_seq, int num_blocks, int window, int sinks,
+                   float scale, int dtype, rlse_stream_t stream);
+
+/* Eviction by accumulated weight, every layer at once. For layer l, sequence
+ * b and KV head h with more than `budget` keys, the first `sinks`, the last
+ * `recent` and the heaviest of those between by scores [num_layers] x
+ * [num_seqs][num_kv_heads][max_blocks_per_seq*16] (layers score_layer_stride
+ * elements apart; ties: the lower slot; NaN is the lightest) are kept, budget
+ * in all; with no more than budget keys all are. The kept ones, in their
+ * order, become slots 0, 1, .. of the sequence's new_tables row: K and V rows
+ * are copied there in every layer (layer l's pools at k_pool/v_pool +
+ * l*layer_stride_elems), their weights to new_scores (same layout as scores,
+ * not overlapping it), their old slots to keep [num_layers][num_seqs]
+ * [num_kv_heads][budget] (int32; -1 behind the last), and new_lens[b] =
+ * min(seq_lens[b], budget). RoPE stays as it was applied: a caller gives new
+ * tokens their true positions (rlse_rope) and appends them at the new slots
+ * (rlse_kv_append).
+ * Nothing the call reads is written, so pages shared by several sequences or
+ * held by the prefix cache may be evicted from: the pages of new_tables (the
+ * first ceil(new_lens[b]/16) of each row) must be distinct and none of them a
+ * page that a sequence of the call reads -- but for a sequence of at most
+ * budget keys, which may keep its own pages (its rows are copied onto
+ * themselves). A length below 0 or above max_blocks_per_seq*16 counts as 0.
+ * Rows of pages whose ids are out of range are not copied. f32, bf16 or f16,
+ * head_dim 64 or 128; 1 <= budget <= new_blocks_per_seq*16 and
+ * max_blocks_per_seq*16; sinks + recent <= budget. */
+int rlse_kv_evict(void* k_pool, void* v_pool, long long layer_stride_elems, int num_layers,
+                  const int32_t* block_tables, const int32_t* seq_lens, const float* scores,
+                  long long score_layer_stride, const int32_t* new_tables, int32_t* new_lens,
+                  float* new_scores, int32_t* keep, int num_seqs, int num_kv_heads, int head_dim,
+                  int max_blocks_per_seq, int new_blocks_per_seq, int num_blocks, int budget,
+                  int sinks, int recent, int dtype, rlse_stream_t stream);
+
 /* ------------------------------------------------------------------ */
 /* Normalisation and rotary embedding.                                 */
 /* ------------------------------------------------------------------ */

@@ -45,6 +45,7 @@ typedef _Float16 f16x4_t __attribute__((ext_vector_type(4)));
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) i16x4_t lds_i16x4_t;
 
 // 16-bit tiles: 16x16x32 and 32x32x16 products of 16-byte operands, and
@@ -215,7 +216,7 @@ __global__ __launch_bounds__(kThinThreads, sizeof(T) == 4 && RT == 2 ? 1 : 2) vo
   constexpr int N = PageRegs<T, D>::N;
   constexpr int ES = (int)sizeof(T), PPR = D * ES / 16;  // packets per row
   constexpr int DT = D / 16;
-  constexpr int NBUF = sizeof(T) == 2 ? 3 : 2;
+  constexpr int NBUF = sizeof(T) == 2 && RT == 1 ? 3 : 2;
   constexpr int kExRow = D + 4;
   __shared__ __align__(16) ThinLds<T, D> s;
   __shared__ __align__(16) float s_ex[kThinWaves][16][kExRow];
@@ -659,28 +660,24 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
     const int wlo_max_t = p.window > 0 ? kend - p.window : 0;
 
     // Virtual pages 4u .. 4u+3 of unit u: positions of their first keys and
-    // ids (-1: none).
-    struct Stage {
-      int pos[kWidePages], id[kWidePages];
-    };
-    auto stage_of = [&](int u) __attribute__((always_inline)) {
-      Stage st;
+    // ids (-1: none). (Native vectors: a struct of arrays is kept in scratch.)
+    auto stage_of = [&](int u, i32x4_t& pos, i32x4_t& id) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < kWidePages; ++i) {
         const int vi = u * kWidePages + i;
         const int pg = real_page(min(vi, pages - 1), wp0, sink_pages);
-        const int id = table[pg];
-        st.pos[i] = pg * 16;
-        st.id[i] = vi < pages && (unsigned)id < (unsigned)p.num_blocks ? id : -1;
+        const int x = table[pg];
+        pos[i] = pg * 16;
+        id[i] = vi < pages && (unsigned)x < (unsigned)p.num_blocks ? x : -1;
       }
-      return st;
     };
-    auto tile_whole = [&](const Stage& st, int kmin_, int wlo_) __attribute__((always_inline)) {
+    auto tile_whole = [&](const i32x4_t& pos, const i32x4_t& id, int kmin_, int wlo_)
+                          __attribute__((always_inline)) {
       bool all = true;
 #pragma unroll
       for (int i = 0; i < kWidePages; ++i)
-        all = all && st.id[i] >= 0 && st.pos[i] + 15 <= kmin_ &&
-              (st.pos[i] >= wlo_ || st.pos[i] + 16 <= p.sinks);
+        all = all && id[i] >= 0 && pos[i] + 15 <= kmin_ &&
+              (pos[i] >= wlo_ || pos[i] + 16 <= p.sinks);
       return all;
     };
 
@@ -702,15 +699,15 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
     float m = -INFINITY, lsum = 0.f;
 
     u32x4_t kst[KPT], vst[KPT];
-    auto load = [&](const Stage& st) __attribute__((always_inline)) {
+    auto load = [&](const i32x4_t& spos, const i32x4_t& sid) __attribute__((always_inline)) {
 #pragma unroll
       for (int j = 0; j < KPT; ++j) {
-        int id = st.id[0], pos = st.pos[0];
+        int id = sid[0], pos = spos[0];
 #pragma unroll
         for (int i = 1; i < kWidePages; ++i)
           if (pg_of[j] == i) {
-            id = st.id[i];
-            pos = st.pos[i];
+            id = sid[i];
+            pos = spos[i];
           }
         const size_t at = ((size_t)(id < 0 ? 0 : id) * Hkv + h) * 16 * D;
         const int rec = id < 0 ? 0 : min(max(kend - pos, 0), 16) * D * ES;
@@ -752,18 +749,19 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
     if (tid < 2) s_odd[tid] = 0;
     __syncthreads();
     const int u_end = u0 + seg;
-    Stage cur = stage_of(u0);
-    load(cur);
-    store(0, tile_whole(cur, kmin_t, wlo_max_t));
-    Stage next = stage_of(min(u0 + 1, u_end - 1));
+    i32x4_t pos, id, pos_next, id_next, pos_after, id_after;
+    stage_of(u0, pos, id);
+    load(pos, id);
+    store(0, tile_whole(pos, id, kmin_t, wlo_max_t));
+    stage_of(min(u0 + 1, u_end - 1), pos_next, id_next);
     __syncthreads();
     int bf = 0;
     for (int u = u0;; ++u) {
       const bool more = u + 1 < u_end;
-      load(next);  // in flight during this stage's math
-      const Stage after = stage_of(min(u + 2, u_end - 1));
+      load(pos_next, id_next);  // in flight during this stage's math
+      stage_of(min(u + 2, u_end - 1), pos_after, id_after);
       if (live) {
-        const bool whole = tile_whole(cur, kmin, wlo_max);
+        const bool whole = tile_whole(pos, id, kmin, wlo_max);
         f32x16_t x[2];
 #pragma unroll
         for (int sb = 0; sb < 2; ++sb)
@@ -798,7 +796,7 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
             for (int i = 0; i < 16; ++i) {
               const int kk = sb * 32 + (i >> 2) * 8 + half * 4 + (i & 3);
               const int pg = sb * 2 + (i >> 3);
-              if (!(cur.id[pg] >= 0 && span.sees(cur.pos[pg] + (kk & 15), p.sinks)))
+              if (!(id[pg] >= 0 && span.sees(pos[pg] + (kk & 15), p.sinks)))
                 x[sb][i] = -INFINITY;
             }
         }
@@ -909,9 +907,11 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
         }
       }
       if (!more) break;
-      cur = next;
-      next = after;
-      store(bf ^ 1, tile_whole(cur, kmin_t, wlo_max_t));
+      pos = pos_next;
+      id = id_next;
+      pos_next = pos_after;
+      id_next = id_after;
+      store(bf ^ 1, tile_whole(pos, id, kmin_t, wlo_max_t));
       __syncthreads();
       bf ^= 1;
     }

@@ -1,0 +1,551 @@
+// The weight every cached key receives from a ragged step's queries (gfx950):
+//   w[b][h][k] = (what k had before, for keys older than the chunk)
+//              + sum over new tokens t and heads of KV head h that see k of
+//                e^(scale q.k - lse[t][head])
+// with the log-sum-exp that the step's attention left, so every query gives a
+// weight of one in all. No counterpart in the reference. The rows, pages and
+// shares are the plan's (chunk_plan.cuh).
+//
+// Both kernels hold keys still and pass the queries over them, so that a key's
+// sum stays in one place and no partial sums are added by atomics: the same
+// call gives the same bits. S = Q . K^T puts one key in each accumulator
+// column, its rows in the lanes' accumulator elements, so the sum over rows is
+// a sum in the lane and one or two exchanges at the end. Products accumulate,
+// and weights sum, in f32.
+//  - thin sequences (at most 32 rows): HBM bound on K. A wave takes a page at
+//    a time, 16 keys of all rows on 16x16 MFMAs.
+//  - wide ones: bound by the exponentials (16 a lane and 32x32 tile, at a
+//    quarter of the VALU's rate) beside the MFMAs. A workgroup holds 256 keys
+//    in registers and streams the rows through LDS, 64 (f32: 32) at a time.
+#include <math.h>
+
+#include "chunk_plan.cuh"
+#include "chunk_plan.h"
+#include "host_common.h"
+
+namespace rlse {
+namespace {
+
+constexpr float kLog2E = 1.4426950408889634f;
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+struct ScoreParams {
+  const void* q;       // [tokens][Hq][D]
+  const void* k_pool;  // [num_blocks][Hkv][16][D]
+  const int* tables;   // [num_seqs][mbps]
+  const float* lse;    // [tokens][Hq]
+  const float* prev;   // [num_seqs][Hkv][mbps*16], NULL, or scores itself
+  float* scores;
+  ChunkPlanView v;
+  uint32_t stamp;
+  int Hq, Hkv, G, mbps, num_blocks, window, sinks;
+  float c;  // scale * log2(e)
+};
+
+template <typename T>
+__device__ __forceinline__ f32x4_t mma16(uint4 a, uint4 b, f32x4_t c) {
+  if constexpr (std::is_same<T, bf16>::value) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                   __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+  } else if constexpr (std::is_same<T, f16>::value) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a),
+                                                  __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+  } else {
+    const float4 x = __builtin_bit_cast(float4, a), y = __builtin_bit_cast(float4, b);
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(x.x, y.x, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(x.y, y.y, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(x.z, y.z, c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(x.w, y.w, c, 0, 0, 0);
+  }
+}
+template <typename T>
+__device__ __forceinline__ f32x16_t mma32(uint4 a, uint4 b, f32x16_t c) {
+  if constexpr (std::is_same<T, bf16>::value) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                   __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+  } else if constexpr (std::is_same<T, f16>::value) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a),
+                                                  __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+  } else {
+    const float4 x = __builtin_bit_cast(float4, a), y = __builtin_bit_cast(float4, b);
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(x.x, y.x, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(x.y, y.y, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(x.z, y.z, c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x2f32(x.w, y.w, c, 0, 0, 0);
+  }
+}
+
+// A row's log-sum-exp in log2 units; +inf (no weight) for a row that saw no
+// key.
+__device__ __forceinline__ float row_lse(float lse) {
+  return lse == -INFINITY ? INFINITY : lse * kLog2E;
+}
+// Whether a row whose own key is at kmax sees key k.
+__device__ __forceinline__ bool row_sees(int k, int kmax, int window, int sinks) {
+  return k <= kmax && (window <= 0 || k > kmax - window || k < sinks);
+}
+
+// Keys between the sinks' pages and the window's, which no row sees, keep
+// what they had: unit u of `units` carries its share of them over.
+__device__ __forceinline__ void carry_gap(const ScoreParams& p, size_t row, int wp0,
+                                          int sink_pages, int u, int units, int thread,
+                                          int threads) {
+  if (wp0 == 0 || p.prev == p.scores) return;
+  const long long lo = 16LL * sink_pages, gap = 16LL * wp0 - lo;
+  const int a = (int)(lo + gap * u / units), b = (int)(lo + gap * (u + 1) / units);
+  for (int k = a + thread; k < b; k += threads)
+    p.scores[row + k] = p.prev ? p.prev[row + k] : 0.f;
+}
+__device__ __forceinline__ void write_score(const ScoreParams& p, size_t row, int k, int off,
+                                            int kend, float w) {
+  if (k < kend) p.scores[row + k] = w + (p.prev && k < off ? p.prev[row + k] : 0.f);
+}
+
+constexpr int kThinWaves = 4;
+constexpr int kThinThreads = 64 * kThinWaves;
+
+template <typename T, int D, int RT>
+__global__ __launch_bounds__(kThinThreads) void score_thin_kernel(ScoreParams p) {
+  constexpr int ES = (int)sizeof(T), N = D * ES / 64;
+  constexpr int NBUF = 4;
+  if (p.v.head->stamp != p.stamp) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) ws_raise(&p.v.head->flags, RLSE_WS_ERR_PLAN);
+    return;
+  }
+  const int groups = p.v.head->thin_groups, tiles = p.v.head->thin_tiles;
+  if ((int)blockIdx.x >= groups) return;
+  const ChunkShare share = p.v.thin_share[share_index(blockIdx.x, groups)];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int col = lane & 15, quad = lane >> 4;
+  const int Hq = p.Hq, Hkv = p.Hkv, G = p.G;
+  const int sink_pages = (p.sinks + 15) >> 4;
+  const T* __restrict__ qb = static_cast<const T*>(p.q);
+  const T* __restrict__ kp = static_cast<const T*>(p.k_pool);
+
+  int ti = __builtin_amdgcn_readfirstlane(share.tile);
+  int h = __builtin_amdgcn_readfirstlane(share.head);
+  int u0 = __builtin_amdgcn_readfirstlane(share.u0);
+  int left = __builtin_amdgcn_readfirstlane(share.count);
+  while (left > 0) {
+    const ChunkTile t = p.v.thin[ti];
+    const int n = __builtin_amdgcn_readfirstlane(t.n), off = __builtin_amdgcn_readfirstlane(t.off);
+    const int tok0 = __builtin_amdgcn_readfirstlane(t.tok0);
+    const int wp0 = __builtin_amdgcn_readfirstlane(t.wp0);
+    const int pages = __builtin_amdgcn_readfirstlane(t.pages);
+    const int seq = __builtin_amdgcn_readfirstlane(t.seq);
+    const int* __restrict__ table = p.tables + (size_t)seq * p.mbps;
+    const size_t out = ((size_t)seq * Hkv + h) * p.mbps * 16;
+    const int seg = min(left, pages - u0);
+    const int rows = n * G, kend = off + n;
+    const int np = (seg - wave + kThinWaves - 1) / kThinWaves;  // this wave's pages
+
+    int ids = -1, pgs = 0, ids_at = 0;
+    auto fetch_ids = [&](int from) __attribute__((always_inline)) {
+      const int i = from + lane;
+      ids = -1;
+      pgs = 0;
+      if (i < np) {
+        pgs = real_page(u0 + wave + i * kThinWaves, wp0, sink_pages);
+        const int id = table[pgs];
+        ids = (unsigned)id < (unsigned)p.num_blocks ? id : -1;
+      }
+      ids_at = from;
+    };
+    fetch_ids(0);
+
+    // Queries in the A-operand layout (lane l: row l % 16), and the rows of
+    // this lane's accumulator elements: row 4 (l / 16) + i.
+    uint4 q[RT][N];
+    float lse[RT][4];
+    int kmax[RT][4];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      {
+        const int row = rt * 16 + col;
+        const bool real = row < rows;
+        const int tok = real ? row / G : 0, g = real ? row - tok * G : 0;
+        const T* src = qb + ((size_t)(tok0 + tok) * Hq + h * G + g) * D + quad * (16 / ES);
+#pragma unroll
+        for (int r = 0; r < N; ++r)
+          q[rt][r] = real ? *reinterpret_cast<const uint4*>(src + r * (64 / ES))
+                          : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = rt * 16 + quad * 4 + i;
+        const bool real = row < rows;
+        const int tok = real ? row / G : 0, g = real ? row - tok * G : 0;
+        lse[rt][i] = real ? row_lse(p.lse[(size_t)(tok0 + tok) * Hq + h * G + g]) : INFINITY;
+        kmax[rt][i] = off + tok;
+      }
+    }
+
+    struct Page {
+      uint4 k[N];
+      int id, pos;
+    };
+    auto load = [&](Page& b, int i) __attribute__((always_inline)) {
+      if (i >= ids_at + 64) fetch_ids(i);
+      b.id = __builtin_amdgcn_readlane(ids, i - ids_at);
+      b.pos = __builtin_amdgcn_readlane(pgs, i - ids_at) * 16;
+      const size_t at = ((size_t)(b.id < 0 ? 0 : b.id) * Hkv + h) * 16 * D;
+      const int rec = b.id < 0 ? 0 : min(kend - b.pos, 16) * D * ES;
+      const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(kp + at), 0, rec,
+                                                        kBufferWord3);
+#pragma unroll
+      for (int r = 0; r < N; ++r)
+        b.k[r] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(
+                                               rk, col * D * ES + quad * 16 + r * 64, 0, 0));
+    };
+    auto compute = [&](const Page& b, int i) __attribute__((always_inline)) {
+      if (i >= np) return;  // (uniform)
+      float w = 0.f;
+      if (b.id >= 0) {
+        f32x4_t x[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) x[rt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int r = 0; r < N; ++r)
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) x[rt] = mma16<T>(q[rt][r], b.k[r], x[rt]);
+        const bool whole = b.pos + 15 <= off && (p.window <= 0 || b.pos > kend - 1 - p.window ||
+                                                 b.pos + 16 <= p.sinks);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float e = __builtin_amdgcn_exp2f(fmaf(x[rt][j], p.c, -lse[rt][j]));
+            w += whole || (rt * 16 + quad * 4 + j < rows &&
+                           row_sees(b.pos + col, kmax[rt][j], p.window, p.sinks))
+                     ? e
+                     : 0.f;
+          }
+        w += __shfl_xor(w, 16, 64);
+        w += __shfl_xor(w, 32, 64);
+      }
+      if (lane < 16) write_score(p, out, b.pos + col, off, kend, w);
+    };
+
+    Page buf[NBUF];
+#pragma unroll
+    for (int i = 0; i < NBUF - 1; ++i) load(buf[i], i);
+    for (int i = 0; i < np; i += NBUF) {
+#pragma unroll
+      for (int j = 0; j < NBUF; ++j) {
+        load(buf[(j + NBUF - 1) % NBUF], i + j + NBUF - 1);
+        compute(buf[j], i + j);
+      }
+    }
+    for (int u = u0 + wave; u < u0 + seg; u += kThinWaves)
+      carry_gap(p, out, wp0, sink_pages, u, pages, lane, 64);
+    left -= seg;
+    u0 = 0;
+    if (++ti == tiles) {
+      ti = 0;
+      ++h;
+    }
+  }
+}
+
+constexpr int kWideWaves = 8;
+constexpr int kWideThreads = 64 * kWideWaves;
+constexpr int kScoreKeys = 16 * kScorePages;  // keys a workgroup holds
+
+template <typename T, int D>
+__global__ __launch_bounds__(kWideThreads, 2) void score_wide_kernel(ScoreParams p) {
+  constexpr int ES = (int)sizeof(T);
+  constexpr int KB = D * ES / 32;          // 16-byte packets of a lane's key
+  constexpr int KS = ES == 2 ? 2 : 1;      // 32-key blocks per wave
+  constexpr int KG = kScoreKeys / (32 * KS), RG = kWideWaves / KG;  // key and row groups
+  constexpr int ROWS = 32 * RG;            // rows per stage
+  constexpr int PPR = D * ES / 16;
+  constexpr int QPT = ROWS * PPR / kWideThreads;  // packets per thread and stage
+  constexpr int PAD = ES == 2 ? 8 : 4;     // rows 4 banks apart
+  static_assert(ROWS * PPR % kWideThreads == 0, "a stage splits evenly");
+  __shared__ __align__(16) T s_q[2][ROWS][D + PAD];
+  __shared__ __align__(16) float s_lse[2][ROWS];
+  __shared__ __align__(16) int s_kmax[2][ROWS];
+  __shared__ float s_sum[RG][kScoreKeys];
+
+  if (p.v.head->stamp != p.stamp) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) ws_raise(&p.v.head->flags, RLSE_WS_ERR_PLAN);
+    return;
+  }
+  const int units = p.v.head->score_units, seqs = p.v.head->score_seqs;
+  const long long total = (long long)units * p.Hkv;
+  const int groups = (int)min((long long)gridDim.x, total);
+  if ((int)blockIdx.x >= groups) return;
+  const int wg = share_index(blockIdx.x, groups);
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int half = lane >> 5, col = lane & 31;
+  const int kg = wave % KG, rg = wave / KG;
+  const int Hq = p.Hq, Hkv = p.Hkv, G = p.G;
+  const int sink_pages = (p.sinks + 15) >> 4;
+  const T* __restrict__ qb = static_cast<const T*>(p.q);
+  const T* __restrict__ kp = static_cast<const T*>(p.k_pool);
+
+  for (long long unit = total * wg / groups; unit < total * (wg + 1) / groups; ++unit) {
+    const int h = (int)(unit / units), ub = (int)(unit - (long long)h * units);
+    int lo = 0, hi = seqs;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (p.v.score[mid].unit0 <= ub) lo = mid; else hi = mid;
+    }
+    const ChunkTile t = p.v.score[lo];
+    const int n = __builtin_amdgcn_readfirstlane(t.n), off = __builtin_amdgcn_readfirstlane(t.off);
+    const int tok0 = __builtin_amdgcn_readfirstlane(t.tok0);
+    const int wp0 = __builtin_amdgcn_readfirstlane(t.wp0);
+    const int pages = __builtin_amdgcn_readfirstlane(t.pages);
+    const int seq = __builtin_amdgcn_readfirstlane(t.seq);
+    const int u = ub - __builtin_amdgcn_readfirstlane(t.unit0);
+    const int* __restrict__ table = p.tables + (size_t)seq * p.mbps;
+    const size_t out = ((size_t)seq * Hkv + h) * p.mbps * 16;
+    const int rows = n * G, kend = off + n;
+
+    // This lane's keys (one per 32-key block) and, for the wave, the pages
+    // of all its keys.
+    int key[KS];
+    bool here[KS];
+    uint4 k[KS][KB];
+    int pos[2 * KS];
+    bool valid = true;
+    int first_key = 0x7fffffff, last_key = -1;
+#pragma unroll
+    for (int i = 0; i < 2 * KS; ++i) {
+      const int vi = u * kScorePages + kg * 2 * KS + i;
+      const int pg = real_page(min(vi, pages - 1), wp0, sink_pages);
+      const int id = table[pg];
+      const bool ok = vi < pages && (unsigned)id < (unsigned)p.num_blocks;
+      pos[i] = vi < pages ? pg * 16 : -1;
+      valid = valid && ok;
+      if (ok) {
+        first_key = min(first_key, pg * 16);
+        last_key = max(last_key, pg * 16 + 15);
+      }
+      if ((col >> 4) == (i & 1)) {
+        key[i >> 1] = vi < pages ? pg * 16 + (col & 15) : kend;
+        here[i >> 1] = ok && key[i >> 1] < kend;
+        const T* src = kp + (((size_t)(ok ? id : 0) * Hkv + h) * 16 + (col & 15)) * D;
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+          // 16-bit: elements 16 b + 8 half ..; f32: half * D/2 + 4 b ..
+          const int at = ES == 2 ? b * 16 + half * 8 : half * (D / 2) + b * 4;
+          k[i >> 1][b] = here[i >> 1] ? *reinterpret_cast<const uint4*>(src + at)
+                                      : make_uint4(0, 0, 0, 0);
+        }
+      }
+    }
+    // Rows that see a key of the workgroup: from the first key's own token to
+    // the last one whose window reaches the last key (sinks: to the end).
+    const int vfirst = u * kScorePages, vlast = min(vfirst + kScorePages, pages) - 1;
+    const int pos0 = real_page(vfirst, wp0, sink_pages) * 16;
+    const int pos1 = real_page(vlast, wp0, sink_pages) * 16 + 15;
+    const int t_lo = max(0, pos0 - off);
+    int t_hi = n - 1;
+    if (p.window > 0 && pos0 >= p.sinks)
+      t_hi = (int)min((long long)t_hi, (long long)pos1 + p.window - 1 - off);
+    const int r_lo = t_lo * G / ROWS * ROWS, r_hi = (t_hi + 1) * G;
+
+    float sum[KS];
+#pragma unroll
+    for (int i = 0; i < KS; ++i) sum[i] = 0.f;
+
+    u32x4_t qst[QPT];
+    float lst = 0.f;
+    int kst = 0;
+    auto load = [&](int r0) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < QPT; ++j) {
+        const int pk = tid + j * kWideThreads;
+        const int row = r0 + pk / PPR, dc = pk % PPR;
+        const int tok = row / G;
+        qst[j] = u32x4_t{0, 0, 0, 0};
+        if (row < rows)
+          qst[j] = *reinterpret_cast<const u32x4_t*>(
+              qb + ((size_t)(tok0 + tok) * Hq + h * G + row - tok * G) * D + dc * (16 / ES));
+      }
+      if (tid < ROWS) {
+        const int row = r0 + tid, tok = row / G;
+        lst = row < rows ? row_lse(p.lse[(size_t)(tok0 + tok) * Hq + h * G + row - tok * G])
+                         : INFINITY;
+        kst = off + tok;
+      }
+    };
+    auto store = [&](int bf) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < QPT; ++j) {
+        const int pk = tid + j * kWideThreads;
+        *reinterpret_cast<u32x4_t*>(&s_q[bf][pk / PPR][pk % PPR * (16 / ES)]) = qst[j];
+      }
+      if (tid < ROWS) {
+        s_lse[bf][tid] = lst;
+        s_kmax[bf][tid] = kst;
+      }
+    };
+    __syncthreads();  // the stages of the unit before are read
+    if (r_lo < r_hi) {
+      load(r_lo);
+      store(0);
+      __syncthreads();
+      int bf = 0;
+      for (int r0 = r_lo;; r0 += ROWS) {
+        const bool more = r0 + ROWS < r_hi;
+        if (more) load(r0 + ROWS);
+        // This wave's rows, and what they see of its keys.
+        const int ra = r0 + rg * 32, rb = min(ra + 31, rows - 1);
+        const int kmax_lo = off + min(ra, rows - 1) / G, kmax_hi = off + rb / G;
+        const bool none =
+            ra >= rows || first_key > kmax_hi ||
+            (p.window > 0 && last_key <= kmax_lo - p.window && first_key >= p.sinks);
+        if (!none) {
+          f32x16_t x[KS];
+#pragma unroll
+          for (int i = 0; i < KS; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[i][e] = 0.f;
+#pragma unroll
+          for (int b = 0; b < KB; ++b) {
+            const int at = ES == 2 ? b * 16 + half * 8 : half * (D / 2) + b * 4;
+            const uint4 a = *reinterpret_cast<const uint4*>(&s_q[bf][rg * 32 + col][at]);
+#pragma unroll
+            for (int i = 0; i < KS; ++i) x[i] = mma32<T>(a, k[i][b], x[i]);
+          }
+          const bool whole = valid && last_key <= kmax_lo && last_key < kend && rb == ra + 31 &&
+                             (p.window <= 0 || first_key > kmax_hi - p.window ||
+                              last_key < p.sinks);
+#pragma unroll
+          for (int g4 = 0; g4 < 4; ++g4) {
+            const int r = rg * 32 + g4 * 8 + half * 4;
+            const float4 l4 = *reinterpret_cast<const float4*>(&s_lse[bf][r]);
+            const float l[4] = {l4.x, l4.y, l4.z, l4.w};
+            if (whole) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < KS; ++i)
+                  sum[i] += __builtin_amdgcn_exp2f(fmaf(x[i][g4 * 4 + j], p.c, -l[j]));
+            } else {
+              const int4 m4 = *reinterpret_cast<const int4*>(&s_kmax[bf][r]);
+              const int m[4] = {m4.x, m4.y, m4.z, m4.w};
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < KS; ++i) {
+                  const float e = __builtin_amdgcn_exp2f(fmaf(x[i][g4 * 4 + j], p.c, -l[j]));
+                  sum[i] += r0 + r + j < rows && here[i] &&
+                                    row_sees(key[i], m[j], p.window, p.sinks)
+                                ? e
+                                : 0.f;
+                }
+            }
+          }
+        }
+        if (!more) break;
+        store(bf ^ 1);
+        __syncthreads();
+        bf ^= 1;
+      }
+    }
+    // The row groups' and lane halves' sums, in that order.
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      const float w = sum[i] + __shfl_xor(sum[i], 32, 64);
+      if (half == 0) s_sum[rg][kg * 32 * KS + i * 32 + col] = w;
+    }
+    __syncthreads();
+    if (tid < kScoreKeys) {
+      const int vi = vfirst + (tid >> 4);
+      if (vi <= vlast) {
+        float w = s_sum[0][tid];
+#pragma unroll
+        for (int i = 1; i < RG; ++i) w += s_sum[i][tid];
+        write_score(p, out, real_page(vi, wp0, sink_pages) * 16 + (tid & 15), off, kend, w);
+      }
+    }
+    carry_gap(p, out, wp0, sink_pages, u, (pages + kScorePages - 1) / kScorePages, tid,
+              kWideThreads);
+  }
+}
+
+template <typename T, int D>
+int launch_scores(const ScoreParams& p, int max_rows, int thin_rows, int cus, hipStream_t stream) {
+  int st = RLSE_OK;
+  if (thin_rows > 0) {
+    const dim3 grid(2 * cus), block(kThinThreads);
+    if (max_rows <= 16)
+      hipLaunchKernelGGL((score_thin_kernel<T, D, 1>), grid, block, 0, stream, p);
+    else
+      hipLaunchKernelGGL((score_thin_kernel<T, D, 2>), grid, block, 0, stream, p);
+    st = launch_status("score_thin_kernel");
+  }
+  if (st || max_rows <= thin_rows) return st;
+  hipLaunchKernelGGL((score_wide_kernel<T, D>), dim3(2 * cus), dim3(kWideThreads), 0, stream, p);
+  return launch_status("score_wide_kernel");
+}
+
+}  // namespace
+}  // namespace rlse
+
+using namespace rlse;
+
+extern "C" int rlse_kv_scores(const void* q, const void* k_pool, const int32_t* block_tables,
+                              void* plan, const float* lse, const float* prev, float* scores,
+                              int num_seqs, int total_tokens, int max_tokens, int num_heads,
+                              int num_kv_heads, int head_dim, int max_blocks_per_seq,
+                              int num_blocks, int window, int sinks, float scale, int dtype,
+                              rlse_stream_t stream) {
+  int st = validate_chunk_shape("kv_scores", num_seqs, total_tokens, max_tokens, num_heads,
+                                num_kv_heads, max_blocks_per_seq, window, sinks);
+  if (st) return st;
+  if (head_dim != 64 && head_dim != 128)
+    return fail(RLSE_ERR_INVALID_VALUE, "kv_scores: head_dim %d not in {64, 128}", head_dim);
+  if (dtype != RLSE_DTYPE_BF16 && dtype != RLSE_DTYPE_F16 && dtype != RLSE_DTYPE_F32)
+    return fail(RLSE_ERR_INVALID_VALUE, "kv_scores: bad dtype %d", dtype);
+  if (num_blocks <= 0)
+    return fail(RLSE_ERR_INVALID_VALUE, "kv_scores: num_blocks %d", num_blocks);
+  if (!(scale > 0.f) || !isfinite(scale))
+    return fail(RLSE_ERR_INVALID_VALUE, "kv_scores: scale must be finite and positive");
+  if (!q || !k_pool || !block_tables || !plan || !lse || !scores)
+    return fail(RLSE_ERR_INVALID_VALUE, "kv_scores: null pointer argument");
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_pool) |
+       reinterpret_cast<uintptr_t>(plan)) & 15)
+    return fail(RLSE_ERR_INVALID_VALUE, "kv_scores: a buffer is not 16-byte aligned");
+  int cus = 0;
+  st = device_cu_count(&cus);
+  if (st) return st;
+  ScoreParams p{};
+  p.q = q;
+  p.k_pool = k_pool;
+  p.tables = block_tables;
+  p.lse = lse;
+  p.prev = prev;
+  p.scores = scores;
+  p.G = num_heads / num_kv_heads;
+  p.v = chunk_plan_view(plan, num_seqs, total_tokens, p.G, cus);
+  p.stamp = chunk_stamp({num_seqs, total_tokens, max_tokens, num_heads, num_kv_heads,
+                         max_blocks_per_seq, window, sinks, cus});
+  p.Hq = num_heads;
+  p.Hkv = num_kv_heads;
+  p.mbps = max_blocks_per_seq;
+  p.num_blocks = num_blocks;
+  p.window = window;
+  p.sinks = sinks;
+  p.c = scale * kLog2E;
+  const int max_rows = max_tokens * p.G;
+  const hipStream_t s = as_stream(stream);
+  auto run = [&](auto t, auto d) {
+    using T = decltype(t);
+    constexpr int D = decltype(d)::value;
+    return launch_scores<T, D>(p, max_rows, thin_row_limit(num_seqs, max_rows), cus, s);
+  };
+  const std::integral_constant<int, 64> d64;
+  const std::integral_constant<int, 128> d128;
+  if (dtype == RLSE_DTYPE_BF16) return head_dim == 128 ? run(bf16{}, d128) : run(bf16{}, d64);
+  if (dtype == RLSE_DTYPE_F16) return head_dim == 128 ? run(f16{}, d128) : run(f16{}, d64);
+  return head_dim == 128 ? run(float{}, d128) : run(float{}, d64);
+}

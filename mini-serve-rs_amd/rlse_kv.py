@@ -84,6 +84,7 @@ EXPORTED = (
     "rlse_decode_step_cascade", "rlse_decode_plan_groups", "rlse_decode_step_groups",
     "rlse_kv_checksum", "rlse_kv_checksum_planned",
     "rlse_chunk_plan_size", "rlse_chunk_plan", "rlse_chunk_workspace_size", "rlse_chunk_attn",
+    "rlse_kv_scores", "rlse_kv_evict",
 )
 
 
@@ -214,6 +215,8 @@ _SIGS = {
     "rlse_chunk_plan": (_i, [_vp, _vp] + [_i] * 8 + [_vp, _sz, _vp]),
     "rlse_chunk_workspace_size": (_i, [_i, _i, _i, _i, _i, _i, ctypes.POINTER(_sz)]),
     "rlse_chunk_attn": (_i, [_vp] * 7 + [_i] * 10 + [_f, _i, _vp, _sz, _vp]),
+    "rlse_kv_scores": (_i, [_vp] * 7 + [_i] * 10 + [_f, _i, _vp]),
+    "rlse_kv_evict": (_i, [_vp, _vp, _ll, _i, _vp, _vp, _vp, _ll] + [_vp] * 4 + [_i] * 10 + [_vp]),
     "rlse_rmsnorm": (_i, [_vp, _vp, _vp, _i, _i, _f, _i, _vp]),
     "rlse_rope_tables": (_i, [_d, _i, _i, _i, _vp, _vp]),
     "rlse_rope": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
@@ -965,6 +968,36 @@ def chunk_attn(q, k_pool, v_pool, block_tables, plan, out, lse, num_seqs: int, t
                                   max_tokens, num_heads, num_kv_heads, head_dim,
                                   max_blocks_per_seq, num_blocks, window, sinks, scale, _dt(dtype),
                                   _ptr(workspace), workspace_bytes, _stream(stream)))
+
+
+def kv_scores(q, k_pool, block_tables, plan, lse, prev, scores, num_seqs: int, total_tokens: int,
+              max_tokens: int, num_heads: int, num_kv_heads: int, head_dim: int,
+              max_blocks_per_seq: int, num_blocks: int, window: int, sinks: int, scale: float,
+              dtype, stream=None) -> None:
+    """The weight each cached key receives from a ragged step's queries (f32
+    [num_seqs][num_kv_heads][max_blocks_per_seq*16]), from the lse of the
+    step's chunk_attn, added to prev (None: counted anew; scores itself: in
+    place) for keys older than the new tokens."""
+    _check(load().rlse_kv_scores(_ptr(q), _ptr(k_pool), _ptr(block_tables), _ptr(plan), _ptr(lse),
+                                 _ptr(prev), _ptr(scores), num_seqs, total_tokens, max_tokens,
+                                 num_heads, num_kv_heads, head_dim, max_blocks_per_seq,
+                                 num_blocks, window, sinks, scale, _dt(dtype), _stream(stream)))
+
+
+def kv_evict(k_pool, v_pool, layer_stride_elems: int, num_layers: int, block_tables, seq_lens,
+             scores, score_layer_stride: int, new_tables, new_lens, new_scores, keep,
+             num_seqs: int, num_kv_heads: int, head_dim: int, max_blocks_per_seq: int,
+             new_blocks_per_seq: int, num_blocks: int, budget: int, sinks: int, recent: int, dtype,
+             stream=None) -> None:
+    """Cuts every layer's cache to budget keys a head -- the first sinks, the
+    last recent, the heaviest between by scores -- moved in order to the pages
+    of new_tables; new_lens, new_scores and the kept slots (keep) are written."""
+    _check(load().rlse_kv_evict(_ptr(k_pool), _ptr(v_pool), layer_stride_elems, num_layers,
+                                _ptr(block_tables), _ptr(seq_lens), _ptr(scores),
+                                score_layer_stride, _ptr(new_tables), _ptr(new_lens),
+                                _ptr(new_scores), _ptr(keep), num_seqs, num_kv_heads, head_dim,
+                                max_blocks_per_seq, new_blocks_per_seq, num_blocks, budget, sinks,
+                                recent, _dt(dtype), _stream(stream)))
 
 
 def rmsnorm(x, weight, out, rows: int, n: int, eps: float, dtype, stream=None) -> None:

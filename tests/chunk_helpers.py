@@ -152,3 +152,54 @@ def assert_within(got, want, tol, what):
         f"{float(over.max()):.3e}")
 
 
+
+
+def step_scores(step, lse, prev=None):
+    """(weights [n][hkv][slots], bound on their error) in 64 bits, from the
+    32-bit lse given. A weight is off by what its score is (as in
+    Step.attention) and 4 e |lse| for the subtraction in log2 units; the sum of
+    r weights by (r + 8) e of it."""
+    e = 2.0 ** -24
+    slots, g = step.mbps * 16, step.hq // step.hkv
+    w = torch.zeros(step.n, step.hkv, slots, dtype=torch.float64)
+    tol = torch.zeros_like(w)
+    for b in range(step.n):
+        if not step.new[b]:
+            continue
+        rows, n = slice(step.cu[b], step.cu[b + 1]), step.lens[b]
+        see = step.visible(b)
+        for h in range(step.hkv):
+            k = step.keys(step.k, b, h)
+            for j in range(h * g, (h + 1) * g):
+                q = step.q[rows, j].double()
+                s = (q @ k.T * step.scale).masked_fill(~see, -math.inf)
+                l = lse[rows, j].double()[:, None]
+                p = torch.where(see & (l > -math.inf), (s - l).exp(), torch.zeros_like(s))
+                off = q.abs() @ k.abs().T * step.scale * (step.d + 2) * e + 16 * e * (
+                    s.abs().nan_to_num(posinf=0) + l.abs().nan_to_num(posinf=0) + 1)
+                w[b, h, :n] += p.sum(0)
+                tol[b, h, :n] += (p * (2 * off + (step.new[b] * g + 8) * e)).sum(0)
+        if prev is not None:
+            w[b, :, :step.cached[b]] += prev[b, :, :step.cached[b]].double()
+            tol[b, :, :n] += 2 * e * w[b, :, :n].abs()
+    return w, tol + 1e-30
+
+
+def evict_reference(scores, lens, budget, sinks, recent):
+    """Kept slots [layers][n][hkv] as lists, from the definition."""
+    layers, n, hkv, _ = scores.shape
+    kept = [[[None] * hkv for _ in range(n)] for _ in range(layers)]
+    for l in range(layers):
+        for b in range(n):
+            for h in range(hkv):
+                size = lens[b]
+                if size <= budget:
+                    kept[l][b][h] = list(range(size))
+                    continue
+                w = scores[l, b, h, :size].tolist()
+                middle = range(sinks, size - recent)
+                order = sorted(middle, key=lambda i: (w[i] != w[i], -w[i] if w[i] == w[i] else 0.0,
+                                                      i))
+                best = sorted(order[:budget - sinks - recent])
+                kept[l][b][h] = list(range(sinks)) + best + list(range(size - recent, size))
+    return kept

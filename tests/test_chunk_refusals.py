@@ -48,3 +48,45 @@ def test_pointers(kv):
                                None) == kv.ERR_INVALID_VALUE
     assert lib.rlse_chunk_plan_size(1, 1, 8, 8, None) == kv.ERR_INVALID_VALUE
     assert lib.rlse_chunk_workspace_size(1, 1, 1, 8, 8, 128, None) == kv.ERR_INVALID_VALUE
+
+
+def _scores(kv, ptr=16, **a):
+    return kv.load().rlse_kv_scores(ptr, 16, 16, 16, 16, None, 16, a["n"], a["total"], a["most"],
+                                    a["hq"], a["hkv"], a["d"], a["mbps"], a["nb"], a["window"],
+                                    a["sinks"], a["scale"], a["dtype"], None)
+
+
+@pytest.mark.parametrize("change", SHAPES + [dict(d=96), dict(dtype=7), dict(nb=0),
+                                             dict(scale=0.0)], ids=str)
+def test_score_arguments(kv, change):
+    assert _scores(kv, **{**GOOD, **change}) == kv.ERR_INVALID_VALUE
+    assert "kv_scores" in kv.last_error()
+
+
+def test_score_pointers(kv):
+    assert _scores(kv, ptr=None, **GOOD) == kv.ERR_INVALID_VALUE
+    assert "null" in kv.last_error()
+    assert _scores(kv, ptr=24, **GOOD) == kv.ERR_INVALID_VALUE
+    assert "aligned" in kv.last_error()
+
+
+EVICT = dict(k=16, stride=64 * 8 * 16 * 128, layers=2, scores=16, sstride=2 * 8 * 128, new=32,
+             n=2, hkv=8, d=128, mbps=8, nbps=2, nb=64, budget=20, sinks=2, recent=3, dtype=1)
+
+
+def _evict(kv, **a):
+    return kv.load().rlse_kv_evict(a["k"], 16, a["stride"], a["layers"], 16, 16, a["scores"],
+                                   a["sstride"], 16, 16, a["new"], 16, a["n"], a["hkv"], a["d"],
+                                   a["mbps"], a["nbps"], a["nb"], a["budget"], a["sinks"],
+                                   a["recent"], a["dtype"], None)
+
+
+@pytest.mark.parametrize("change", [
+    dict(layers=0), dict(n=0), dict(hkv=0), dict(d=96), dict(mbps=0), dict(nbps=0), dict(nb=0),
+    dict(budget=0), dict(budget=33), dict(budget=129, nbps=20), dict(sinks=-1), dict(recent=-1),
+    dict(sinks=18), dict(dtype=5), dict(sstride=2047), dict(stride=64 * 8 * 16 * 128 - 1),
+    dict(stride=64 * 8 * 16 * 128 + 1), dict(k=None), dict(k=24), dict(new=16),
+    dict(layers=1 << 20, n=4096, sstride=1 << 40)], ids=str)
+def test_evict_arguments(kv, change):
+    assert _evict(kv, **{**EVICT, **change}) == kv.ERR_INVALID_VALUE
+    assert "kv_evict" in kv.last_error()
