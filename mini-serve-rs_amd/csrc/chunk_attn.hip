@@ -45,7 +45,6 @@ typedef _Float16 f16x4_t __attribute__((ext_vector_type(4)));
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
-typedef int i32x4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) i16x4_t lds_i16x4_t;
 
 // 16-bit tiles: 16x16x32 and 32x32x16 products of 16-byte operands, and
@@ -96,7 +95,7 @@ struct ChunkParams {
   uint32_t stamp;
   float* thin_part;    // [2 * groups][kThinRows * (D + 2)]
   uint32_t* thin_done; // [groups]: pieces of the tile cut at a share's end
-  float4* wide_part;   // [2 * groups][(D / 8 + 1) * kWideThreads]
+  float4* wide_part;   // [2 * groups][wide_part_slots(D)]
   int Hq, Hkv, G, mbps, num_blocks, window, sinks;
   float c;             // scale * log2(e)
 };
@@ -176,7 +175,7 @@ __device__ __forceinline__ void write_row(T* dst, const float* v, float inv) {
 struct RowSpan {
   int kmax, wlo;
   __device__ __forceinline__ bool sees(int k, int sinks) const {
-    return k <= kmax && (k >= wlo || k < sinks);
+    return (k <= kmax) & ((k >= wlo) | (k < sinks));  // (no branches)
   }
 };
 __device__ __forceinline__ RowSpan row_span(int off, int t, int window) {
@@ -551,8 +550,13 @@ __global__ __launch_bounds__(kThinThreads, sizeof(T) == 4 && RT == 2 ? 1 : 2) vo
   }
 }
 
+constexpr int kPartLanes = 2 * kWideRows;  // two lanes a row
+// float4 slots of a wide tile's partial state: the row's 4 D/32 of a lane, and
+// its (m, l).
+constexpr int wide_part_slots(int D) { return (D / 8 + 1) * kPartLanes; }
+
 // ---------------------------------------------------------------------------
-// Wide sequences
+// Wide sequences, 16-bit
 // ---------------------------------------------------------------------------
 // A workgroup of 8 waves takes a tile of 256 rows, each wave 32 of them, and
 // streams its share of the tile's pages four at a time: K and V rows staged
@@ -560,13 +564,10 @@ __global__ __launch_bounds__(kThinThreads, sizeof(T) == 4 && RT == 2 ? 1 : 2) vo
 // Per wave (v_mfma_f32_32x32x16; lane l holds A[l%32][8*(l/32)+j],
 // B[8*(l/32)+j][l%32] and accumulator element i at
 // [8*(i/4) + 4*(l/32) + i%4][l%32]):
-//   S^T (keys x rows) = K . Q^T, so each lane owns one row: the max and sum
-//   are 16 values in the lane plus one exchange with lane l^32, and
+//   S^T (keys x rows) = K . Q^T, so each lane owns one row: max and sum are
+//   over 16 values in the lane and lane l^32, and
 //   O^T (d x rows) += V^T . P^T takes the probabilities from the accumulator
 //   as they lie; V^T comes from row-major LDS through transposing reads.
-// f32 runs on v_mfma_f32_32x32x2_f32: lane half h contracts dimension
-// h*D/2 + j at step j of S^T, and for O^T step j pairs the two keys the lane
-// halves hold in accumulator element j.
 constexpr int kWideWaves = 8;
 constexpr int kWideThreads = 64 * kWideWaves;
 constexpr int kWideKeys = 16 * kWidePages;
@@ -574,23 +575,21 @@ constexpr int kWideKeys = 16 * kWidePages;
 template <typename T, int D>
 struct WideLds {
   // Row strides that put the rows one read takes together on banks of their
-  // own (64 four-byte banks): 16-bit K rows 4 banks apart, V rows of a
-  // transposing read 16; f32 K rows 4, the V rows of the lane halves 32.
-  static constexpr int kPadK = sizeof(T) == 2 ? 8 : 4;
-  static constexpr int kPadV = sizeof(T) == 2 ? 32 : 8;
+  // own (64 four-byte banks): K rows 4 banks apart, the rows of a transposing
+  // V read 16.
+  static constexpr int kPadK = 8, kPadV = 32;
   T k[2][kWideKeys][D + kPadK];
   T v[2][kWideKeys][D + kPadV];
 };
 
 template <typename T, int D>
 __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams p) {
-  constexpr int ES = (int)sizeof(T);
-  constexpr int DB = D / 32;                      // 32-dimension blocks of O^T
-  constexpr int KB = D * ES / 32;                 // 16-byte packets of a lane's query
-  constexpr int PPR = D * ES / 16;                // packets per row
+  constexpr int DB = D / 32;                           // 32-dimension blocks of O^T
+  constexpr int KB = D / 16;                           // 16-dimension steps of q.k
+  constexpr int PPR = D / 8;                           // packets per row
   constexpr int KPT = kWideKeys * PPR / kWideThreads;  // packets per thread and stage
   __shared__ __align__(16) WideLds<T, D> s;
-  __shared__ int s_odd[2];  // the stage holds a value of V that is not finite
+  __shared__ uint32_t s_odd[2][2];  // keys of a stage with V not finite
 
   if (p.v.head->stamp != p.stamp) {
     if (blockIdx.x == 0 && threadIdx.x == 0) ws_raise(&p.v.head->flags, RLSE_WS_ERR_PLAN);
@@ -610,16 +609,13 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
   const T* __restrict__ kp = static_cast<const T*>(p.k_pool);
   const T* __restrict__ vp = static_cast<const T*>(p.v_pool);
 
-  // Packet j of this thread in a stage: key kk, 16-byte chunk dc of its row.
-  // Its page, kk >> 4, is the same for the whole wave.
-  int voff[KPT], pg_of[KPT];
-#pragma unroll
-  for (int j = 0; j < KPT; ++j) {
-    const int pk = tid + j * kWideThreads;
-    const int kk = pk / PPR, dc = pk - kk * PPR;
-    voff[j] = (kk & 15) * D * ES + dc * 16;
-    pg_of[j] = __builtin_amdgcn_readfirstlane(kk >> 4);
-  }
+  // Packet j of this thread in a stage: key kk0 + j * kWideThreads / PPR,
+  // chunk dc of its row; its page is the same for the wave.
+  const int kk0 = tid / PPR, dc = tid % PPR;
+  constexpr int kStep = kWideThreads / PPR;  // 32 or 64 keys
+  const int voff = (kk0 & 15) * D * 2 + dc * 16;
+  const int pg0 = __builtin_amdgcn_readfirstlane(kk0 >> 4);
+
   // Transposing V reads: within a 16-lane group lane 4j + a points at key row
   // j, columns 4a ..; half h takes keys 4h .. and 8 + 4h ..
   const int tr_g = lane >> 4, tr_j = (lane & 15) >> 2, tr_a = lane & 3;
@@ -647,170 +643,134 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
 
     const int wrow = row0 + wave * 32;
     const bool live = wrow < rows;  // the wave has rows (else it only stages)
-    const int myrow = wrow + col;
-    const int row_c = min(myrow, rows - 1);
-    const int tok = row_c / G, qh = h * G + row_c - tok * G;
+    const int row = min(wrow + col, rows - 1), tok = row / G;
+    const size_t at = (size_t)(tok0 + tok) * Hq + h * G + row - tok * G;
     const RowSpan span = row_span(off, tok, p.window);
-    // Every row of the wave sees keys up to the first one's own, and from the
-    // last one's window on.
-    const int kmin = off + min(wrow, rows - 1) / G;
-    const int wlo_max = p.window > 0 ? off + min(wrow + 31, rows - 1) / G - p.window + 1 : 0;
-    // The same for the whole tile (its stages with keys some row masks).
-    const int kmin_t = off + row0 / G;
-    const int wlo_max_t = p.window > 0 ? kend - p.window : 0;
+    const int kmin = off + min(wrow, rows - 1) / G, kmin_t = off + row0 / G;
+    const int wlo = p.window > 0 ? off + min(wrow + 31, rows - 1) / G - p.window + 1 : 0;
+    const int wlo_t = p.window > 0 ? kend - p.window : 0;
 
-    // Virtual pages 4u .. 4u+3 of unit u: positions of their first keys and
-    // ids (-1: none). (Native vectors: a struct of arrays is kept in scratch.)
-    auto stage_of = [&](int u, i32x4_t& pos, i32x4_t& id) __attribute__((always_inline)) {
-#pragma unroll
-      for (int i = 0; i < kWidePages; ++i) {
-        const int vi = u * kWidePages + i;
-        const int pg = real_page(min(vi, pages - 1), wp0, sink_pages);
-        const int x = table[pg];
-        pos[i] = pg * 16;
-        id[i] = vi < pages && (unsigned)x < (unsigned)p.num_blocks ? x : -1;
-      }
+    // Page ids of 16 units at a time, one a lane; the valid ones as a mask.
+    int ids, ids_at;
+    uint64_t ids_ok;
+    auto fetch_ids = [&](int u) __attribute__((always_inline)) {
+      ids_at = u * kWidePages;
+      const int vi = ids_at + lane;
+      ids = table[real_page(min(vi, pages - 1), wp0, sink_pages)];
+      const bool ok = vi < pages && (unsigned)ids < (unsigned)p.num_blocks;
+      if (!ok) ids = -1;
+      ids_ok = __ballot(ok);
     };
-    auto tile_whole = [&](const i32x4_t& pos, const i32x4_t& id, int kmin_, int wlo_)
-                          __attribute__((always_inline)) {
+    auto page_pos = [&](int vi) __attribute__((always_inline)) {
+      return real_page(min(vi, pages - 1), wp0, sink_pages) * 16;
+    };
+    auto seen_whole = [&](int vi, unsigned ok, int kmin_, int wlo_) __attribute__((always_inline)) {
       bool all = true;
 #pragma unroll
-      for (int i = 0; i < kWidePages; ++i)
-        all = all && id[i] >= 0 && pos[i] + 15 <= kmin_ &&
-              (pos[i] >= wlo_ || pos[i] + 16 <= p.sinks);
+      for (int i = 0; i < kWidePages; ++i) {
+        const int pos = page_pos(vi + i);
+        all = all & (ok >> i & 1) & (pos + 15 <= kmin_) & ((pos >= wlo_) | (pos + 16 <= p.sinks));
+      }
       return all;
     };
 
     uint4 q[KB];
-    {
-      const T* src = qb + ((size_t)(tok0 + tok) * Hq + qh) * D;
 #pragma unroll
-      for (int i = 0; i < KB; ++i) {
-        // 16-bit: elements 16 i + 8 half ..; f32: half * D/2 + 4 i ..
-        const int at = ES == 2 ? i * 16 + half * 8 : half * (D / 2) + i * 4;
-        q[i] = *reinterpret_cast<const uint4*>(src + at);
-      }
-    }
+    for (int i = 0; i < KB; ++i)
+      q[i] = *reinterpret_cast<const uint4*>(qb + at * D + i * 16 + half * 8);
     f32x16_t o[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
-    float m = -INFINITY, lsum = 0.f;
+    float m = -INFINITY, l = 0.f;
 
     u32x4_t kst[KPT], vst[KPT];
-    auto load = [&](const i32x4_t& spos, const i32x4_t& sid) __attribute__((always_inline)) {
+    auto load = [&](int u) __attribute__((always_inline)) {
+      if (u * kWidePages >= ids_at + 64) fetch_ids(u);
 #pragma unroll
       for (int j = 0; j < KPT; ++j) {
-        int id = sid[0], pos = spos[0];
-#pragma unroll
-        for (int i = 1; i < kWidePages; ++i)
-          if (pg_of[j] == i) {
-            id = sid[i];
-            pos = spos[i];
-          }
-        const size_t at = ((size_t)(id < 0 ? 0 : id) * Hkv + h) * 16 * D;
-        const int rec = id < 0 ? 0 : min(max(kend - pos, 0), 16) * D * ES;
-        const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(kp + at), 0, rec,
+        const int vi = u * kWidePages + pg0 + j * (kStep / 16);
+        const int id = __builtin_amdgcn_readlane(ids, vi - ids_at);
+        const size_t base = ((size_t)(id < 0 ? 0 : id) * Hkv + h) * 16 * D;
+        const int rec = id < 0 ? 0 : min(max(kend - page_pos(vi), 0), 16) * D * 2;
+        const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(kp + base), 0, rec,
                                                           kBufferWord3);
-        const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(vp + at), 0, rec,
+        const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(vp + base), 0, rec,
                                                           kBufferWord3);
-        kst[j] = __builtin_amdgcn_raw_buffer_load_b128(rk, voff[j], 0, 0);
-        vst[j] = __builtin_amdgcn_raw_buffer_load_b128(rv, voff[j], 0, 0);
+        kst[j] = __builtin_amdgcn_raw_buffer_load_b128(rk, voff, 0, 0);
+        vst[j] = __builtin_amdgcn_raw_buffer_load_b128(rv, voff, 0, 0);
       }
+      return (unsigned)(ids_ok >> (u * kWidePages - ids_at)) & 15u;
     };
     auto store = [&](int bf, bool whole) __attribute__((always_inline)) {
 #pragma unroll
       for (int j = 0; j < KPT; ++j) {
-        const int pk = tid + j * kWideThreads;
-        const int kk = pk / PPR, dc = pk - kk * PPR;
-        *reinterpret_cast<u32x4_t*>(&s.k[bf][kk][dc * (16 / ES)]) = kst[j];
-        *reinterpret_cast<u32x4_t*>(&s.v[bf][kk][dc * (16 / ES)]) = vst[j];
-      }
-      if (!whole) {
-        bool odd = false;
-#pragma unroll
-        for (int j = 0; j < KPT; ++j)
+        const int kk = kk0 + j * kStep;
+        if (!whole) {
+          bool odd = false;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
+            constexpr uint32_t inf = Tile<T>::kInf;
             const uint32_t x = vst[j][i];
-            if constexpr (ES == 2) {
-              constexpr uint32_t inf = Tile<T>::kInf;
-              odd = odd || (x & inf) == inf || (x & inf << 16) == inf << 16;
-            } else {
-              odd = odd || (x & 0x7f800000u) == 0x7f800000u;
-            }
+            const bool lo = (x & inf) == inf, hi = (x & inf << 16) == inf << 16;
+            odd = odd | lo | hi;
+            vst[j][i] = x & (lo ? 0xffff0000u : ~0u) & (hi ? 0xffffu : ~0u);
           }
-        if (odd) s_odd[bf] = 1;
+          if (odd) atomicOr(&s_odd[bf][kk >> 5], 1u << (kk & 31));
+        }
+        *reinterpret_cast<u32x4_t*>(&s.k[bf][kk][dc * 8]) = kst[j];
+        *reinterpret_cast<u32x4_t*>(&s.v[bf][kk][dc * 8]) = vst[j];
       }
     };
 
     __syncthreads();  // the stages of the segment before are read
-    if (tid < 2) s_odd[tid] = 0;
+    if (tid < 4) s_odd[tid >> 1][tid & 1] = 0;
     __syncthreads();
     const int u_end = u0 + seg;
-    i32x4_t pos, id, pos_next, id_next, pos_after, id_after;
-    stage_of(u0, pos, id);
-    load(pos, id);
-    store(0, tile_whole(pos, id, kmin_t, wlo_max_t));
-    stage_of(min(u0 + 1, u_end - 1), pos_next, id_next);
+    fetch_ids(u0);
+    unsigned ok = load(u0), ok_next = 0;
+    bool whole_t = seen_whole(u0 * kWidePages, ok, kmin_t, wlo_t);
+    store(0, whole_t);
     __syncthreads();
     int bf = 0;
     for (int u = u0;; ++u) {
       const bool more = u + 1 < u_end;
-      load(pos_next, id_next);  // in flight during this stage's math
-      stage_of(min(u + 2, u_end - 1), pos_after, id_after);
+      if (more) ok_next = load(u + 1);  // in flight during this stage's math
       if (live) {
-        const bool whole = tile_whole(pos, id, kmin, wlo_max);
         f32x16_t x[2];
 #pragma unroll
         for (int sb = 0; sb < 2; ++sb)
 #pragma unroll
           for (int i = 0; i < 16; ++i) x[sb][i] = 0.f;
-        if constexpr (ES == 2) {
 #pragma unroll
-          for (int kb = 0; kb < KB; ++kb)
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int sb = 0; sb < 2; ++sb)
-              x[sb] = Tile<T>::mma32(
-                  *reinterpret_cast<const uint4*>(&s.k[bf][sb * 32 + col][kb * 16 + half * 8]),
-                  q[kb], x[sb]);
-        } else {
-#pragma unroll
-          for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-            for (int sb = 0; sb < 2; ++sb) {
-              const float4 a = *reinterpret_cast<const float4*>(
-                  &s.k[bf][sb * 32 + col][half * (D / 2) + kb * 4]);
-              const float4 b = __builtin_bit_cast(float4, q[kb]);
-              x[sb] = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x, b.x, x[sb], 0, 0, 0);
-              x[sb] = __builtin_amdgcn_mfma_f32_32x32x2f32(a.y, b.y, x[sb], 0, 0, 0);
-              x[sb] = __builtin_amdgcn_mfma_f32_32x32x2f32(a.z, b.z, x[sb], 0, 0, 0);
-              x[sb] = __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, b.w, x[sb], 0, 0, 0);
-            }
-        }
-        if (!whole) {
+          for (int sb = 0; sb < 2; ++sb) {
+            x[sb] = Tile<T>::mma32(
+                *reinterpret_cast<const uint4*>(&s.k[bf][sb * 32 + col][kb * 16 + half * 8]),
+                q[kb], x[sb]);
+          }
+        if (!seen_whole(u * kWidePages, ok, kmin, wlo)) {
 #pragma unroll
           for (int sb = 0; sb < 2; ++sb)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const int kk = sb * 32 + (i >> 2) * 8 + half * 4 + (i & 3);
-              const int pg = sb * 2 + (i >> 3);
-              if (!(id[pg] >= 0 && span.sees(pos[pg] + (kk & 15), p.sinks)))
-                x[sb][i] = -INFINITY;
+              const int kk = (i >> 2) * 8 + half * 4 + (i & 3), pg = sb * 2 + (i >> 3);
+              const bool see = (ok >> pg & 1) &
+                               span.sees(page_pos(u * kWidePages + pg) + (kk & 15), p.sinks);
+              x[sb][i] = see ? x[sb][i] : -INFINITY;
             }
         }
-        float mx = -INFINITY;
+        float mx = x[0][0];
 #pragma unroll
         for (int sb = 0; sb < 2; ++sb)
 #pragma unroll
           for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[sb][i]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float cand = mx * p.c;
-        if (__any(cand > m + kLazyLog2)) {
-          const float mn = fmaxf(m, cand);
+        if (__any(mx * p.c > m + kLazyLog2)) {
+          const float mn = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32, 64)) * p.c);
           const float a = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-          lsum *= a;
+          l *= a;
 #pragma unroll
           for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -818,28 +778,24 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
           m = mn;
         }
         const float nm = m == -INFINITY ? 0.f : -m;
-        float rs = 0.f;
+        float sum = 0.f;
 #pragma unroll
         for (int sb = 0; sb < 2; ++sb)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             x[sb][i] = __builtin_amdgcn_exp2f(fmaf(x[sb][i], p.c, nm));
-            rs += x[sb][i];
+            sum += x[sb][i];
           }
-        rs += __shfl_xor(rs, 32, 64);
-        lsum += rs;
-        const bool apart = !whole && s_odd[bf] != 0;
-        if constexpr (ES == 2) {
-          uint4 pk[4];  // P^T operands of the four 16-key blocks
+        l += sum;
 #pragma unroll
-          for (int kq = 0; kq < 4; ++kq) {
-            const f32x16_t& y = x[kq >> 1];
-            const int e = (kq & 1) * 8;
-            pk[kq] = make_uint4(
-                Packet<T>::pack2(y[e], y[e + 1]), Packet<T>::pack2(y[e + 2], y[e + 3]),
-                Packet<T>::pack2(y[e + 4], y[e + 5]), Packet<T>::pack2(y[e + 6], y[e + 7]));
-          }
-          auto vt = [&](int kq, int d) __attribute__((always_inline)) {
+        for (int kq = 0; kq < 4; ++kq) {
+          const f32x16_t& y = x[kq >> 1];
+          const int e = (kq & 1) * 8;
+          const uint4 pk = make_uint4(
+              Packet<T>::pack2(y[e], y[e + 1]), Packet<T>::pack2(y[e + 2], y[e + 3]),
+              Packet<T>::pack2(y[e + 4], y[e + 5]), Packet<T>::pack2(y[e + 6], y[e + 7]));
+#pragma unroll
+          for (int d = 0; d < DB; ++d) {
             const uint16_t* v0 =
                 reinterpret_cast<const uint16_t*>(&s.v[bf][kq * 16 + tr_row][d * 32 + tr_col]);
             const uint2 lo = __builtin_bit_cast(
@@ -847,79 +803,51 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
             const uint2 hi = __builtin_bit_cast(
                 uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                            (lds_i16x4_t*)(v0 + 8 * (D + WideLds<T, D>::kPadV))));
-            return make_uint4(lo.x, lo.y, hi.x, hi.y);
-          };
-          if (!apart) {
-#pragma unroll
-            for (int kq = 0; kq < 4; ++kq)
-#pragma unroll
-              for (int d = 0; d < DB; ++d) o[d] = Tile<T>::mma32(vt(kq, d), pk[kq], o[d]);
-          } else {
-#pragma unroll
-            for (int d = 0; d < DB; ++d) {
-              f32x16_t cp, cn;
-#pragma unroll
-              for (int i = 0; i < 16; ++i) cp[i] = cn[i] = 0.f;
-#pragma unroll
-              for (int kq = 0; kq < 4; ++kq) {
-                const uint4 a = vt(kq, d);
-                uint4 pos, neg;
-                const uint4 fin = make_uint4(
-                    split_word<T>(a.x, &pos.x, &neg.x), split_word<T>(a.y, &pos.y, &neg.y),
-                    split_word<T>(a.z, &pos.z, &neg.z), split_word<T>(a.w, &pos.w, &neg.w));
-                const uint4 see = make_uint4(seen_word<T>(pk[kq].x), seen_word<T>(pk[kq].y),
-                                             seen_word<T>(pk[kq].z), seen_word<T>(pk[kq].w));
-                o[d] = Tile<T>::mma32(fin, pk[kq], o[d]);
-                cp = Tile<T>::mma32(pos, see, cp);
-                cn = Tile<T>::mma32(neg, see, cn);
-              }
-#pragma unroll
-              for (int i = 0; i < 16; ++i) o[d][i] += not_finite(cp[i], cn[i]);
-            }
+            o[d] = Tile<T>::mma32(make_uint4(lo.x, lo.y, hi.x, hi.y), pk, o[d]);
           }
-        } else {
+        }
+        if (!whole_t) {
+          // What values of V that are not finite add to rows that see their keys.
+          for (int sb = 0; sb < 2; ++sb) {
+            uint32_t odd = __builtin_amdgcn_readfirstlane(s_odd[bf][sb]);
+            while (odd) {
+              const int kk = sb * 32 + __builtin_ctz(odd);
+              odd &= odd - 1;
+              if (!(ok >> (kk >> 4) & 1)) continue;
+              const int pg = real_page(u * kWidePages + (kk >> 4), wp0, sink_pages);
+              const T* src = vp + (((size_t)table[pg] * Hkv + h) * 16 + (kk & 15)) * D;
+              const bool see = span.sees(pg * 16 + (kk & 15), p.sinks);
 #pragma unroll
-          for (int d = 0; d < DB; ++d) {
-            f32x16_t cp, cn;
+              for (int d = 0; d < DB; ++d)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) cp[i] = cn[i] = 0.f;
+                for (int i4 = 0; i4 < 4; ++i4) {
+                  const uint2 y = *reinterpret_cast<const uint2*>(src + d * 32 + i4 * 8 + half * 4);
 #pragma unroll
-            for (int sb = 0; sb < 2; ++sb)
-#pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                const float a =
-                    s.v[bf][sb * 32 + (j >> 2) * 8 + half * 4 + (j & 3)][d * 32 + col];
-                if (!apart) {
-                  o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, x[sb][j], o[d], 0, 0, 0);
-                } else {
-                  float pos, neg;
-                  const float fin = split_word(a, &pos, &neg);
-                  const float see = x[sb][j] != 0.f ? 1.f : 0.f;
-                  o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(fin, x[sb][j], o[d], 0, 0, 0);
-                  cp = __builtin_amdgcn_mfma_f32_32x32x2f32(pos, see, cp, 0, 0, 0);
-                  cn = __builtin_amdgcn_mfma_f32_32x32x2f32(neg, see, cn, 0, 0, 0);
+                  for (int i = 0; i < 4; ++i) {
+                    T e;
+                    const uint16_t bits = (uint16_t)((i < 2 ? y.x : y.y) >> (16 * (i & 1)));
+                    __builtin_memcpy(&e, &bits, 2);
+                    const float v = Elem<T>::to_f32(e);
+                    o[d][i4 * 4 + i] += see & !(v - v == 0.f) ? v : 0.f;
+                  }
+                  __builtin_amdgcn_sched_barrier(0);  // (else all loads' registers at once)
                 }
-              }
-            if (apart)
-#pragma unroll
-              for (int i = 0; i < 16; ++i) o[d][i] += not_finite(cp[i], cn[i]);
+            }
           }
         }
       }
       if (!more) break;
-      pos = pos_next;
-      id = id_next;
-      pos_next = pos_after;
-      id_next = id_after;
-      store(bf ^ 1, tile_whole(pos, id, kmin_t, wlo_max_t));
+      ok = ok_next;
+      whole_t = seen_whole((u + 1) * kWidePages, ok, kmin_t, wlo_t);
+      store(bf ^ 1, whole_t);
       __syncthreads();
       bf ^= 1;
     }
 
     // Lane holds O^T rows d = 32 db + 8 (i/4) + 4 half + i%4 of its row.
+    const float lsum = l + __shfl_xor(l, 32, 64);
     if (seg == units) {
-      if (myrow < rows) {
-        const size_t at = (size_t)(tok0 + tok) * Hq + qh;
+      if (wrow + col < rows) {
         T* dst = static_cast<T*>(p.out) + at * D;
         const float inv = inverse_sum(lsum);
 #pragma unroll
@@ -933,17 +861,311 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
         if (p.lse && half == 0) p.lse[at] = state_lse(m, lsum);
       }
     } else if (live) {
-      // The partial state in register order: float4 slot k of thread tid, so
-      // every store covers 1 KB of consecutive bytes.
       float4* part = p.wide_part +
-                     (size_t)(2 * w + (head_piece ? 0 : 1)) * (4 * DB + 1) * kWideThreads + tid;
+                     (size_t)(2 * w + (head_piece ? 0 : 1)) * wide_part_slots(D) + tid;
 #pragma unroll
       for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int i4 = 0; i4 < 4; ++i4)
-          part[(d * 4 + i4) * kWideThreads] = make_float4(o[d][i4 * 4], o[d][i4 * 4 + 1],
-                                                          o[d][i4 * 4 + 2], o[d][i4 * 4 + 3]);
-      part[4 * DB * kWideThreads] = make_float4(m, lsum, 0.f, 0.f);
+          part[(d * 4 + i4) * kPartLanes] = make_float4(o[d][i4 * 4], o[d][i4 * 4 + 1],
+                                                        o[d][i4 * 4 + 2], o[d][i4 * 4 + 3]);
+      part[4 * DB * kPartLanes] = make_float4(m, lsum, 0.f, 0.f);
+    }
+    left -= seg;
+    u0 = 0;
+    head_piece = false;
+    if (++ti == tiles) {
+      ti = 0;
+      ++h;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Wide sequences, f32
+// ---------------------------------------------------------------------------
+// The same products on v_mfma_f32_32x32x2_f32, whose rate bounds them: lane half
+// h contracts dimension h*D/2 + j at step j of S^T = K . Q^T, and step j of
+// O^T += V^T . P^T pairs the two keys that the lane halves hold in accumulator
+// element j. Eight waves of 32 rows (a row's f32 state takes twice the
+// registers), 64 keys staged in one of two LDS buffers while the next are
+// loaded.
+constexpr int kWide32Waves = 8;
+constexpr int kWide32Threads = 64 * kWide32Waves;
+
+template <int D>
+struct Wide32Lds {
+  // K rows 4 banks apart, the V rows of the lane halves (4 apart) 32.
+  float k[2][kWideKeys][D + 4];
+  float v[2][kWideKeys][D + 8];
+};
+
+template <int D>
+__global__ __launch_bounds__(kWide32Threads, 1) void chunk_wide32_kernel(ChunkParams p) {
+  constexpr int DB = D / 32;                           // 32-dimension blocks of O^T
+  constexpr int KB = D / 8;                            // 16-byte packets of a lane's query
+  constexpr int PPR = D / 4;                           // packets per row
+  constexpr int KPT = kWideKeys * PPR / kWide32Threads;  // packets per thread and stage
+  __shared__ __align__(16) Wide32Lds<D> s;
+  __shared__ uint32_t s_odd[2][2];  // keys of a stage with V not finite
+
+  if (p.v.head->stamp != p.stamp) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) ws_raise(&p.v.head->flags, RLSE_WS_ERR_PLAN);
+    return;
+  }
+  const int groups = p.v.head->wide_groups, tiles = p.v.head->wide_tiles;
+  if ((int)blockIdx.x >= groups) return;
+  const int w = share_index(blockIdx.x, groups);
+  const ChunkShare share = p.v.wide_share[w];
+
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int half = lane >> 5, col = lane & 31;
+  const int Hq = p.Hq, Hkv = p.Hkv, G = p.G;
+  const int sink_pages = (p.sinks + 15) >> 4;
+  const float* __restrict__ qb = static_cast<const float*>(p.q);
+  const float* __restrict__ kp = static_cast<const float*>(p.k_pool);
+  const float* __restrict__ vp = static_cast<const float*>(p.v_pool);
+
+  // Packet j of this thread in a stage: key kk0 + j * kWide32Threads / PPR,
+  // chunk dc of its row; its page is the same for the wave.
+  const int kk0 = tid / PPR, dc = tid % PPR;
+  constexpr int kStep = kWide32Threads / PPR;  // 16 or 32 keys
+  const int voff = (kk0 & 15) * D * 4 + dc * 16;
+  const int pg0 = __builtin_amdgcn_readfirstlane(kk0 >> 4);
+
+  int ti = __builtin_amdgcn_readfirstlane(share.tile);
+  int h = __builtin_amdgcn_readfirstlane(share.head);
+  int u0 = __builtin_amdgcn_readfirstlane(share.u0);
+  int left = __builtin_amdgcn_readfirstlane(share.count);
+  bool head_piece = u0 > 0;
+  while (left > 0) {
+    const ChunkTile t = p.v.wide[ti];
+    const int n = __builtin_amdgcn_readfirstlane(t.n), off = __builtin_amdgcn_readfirstlane(t.off);
+    const int tok0 = __builtin_amdgcn_readfirstlane(t.tok0);
+    const int row0 = __builtin_amdgcn_readfirstlane(t.row0);
+    const int wp0 = __builtin_amdgcn_readfirstlane(t.wp0);
+    const int pages = __builtin_amdgcn_readfirstlane(t.pages);
+    const int* __restrict__ table =
+        p.tables + (size_t)__builtin_amdgcn_readfirstlane(t.seq) * p.mbps;
+    const int units = (pages + kWidePages - 1) / kWidePages;
+    const int seg = min(left, units - u0);
+    const int rows = n * G;
+    const int last_row = min(rows, row0 + kWideRows) - 1;
+    const int kend = off + last_row / G + 1;  // keys the tile's rows see end here
+
+    const int wrow = row0 + wave * 32;
+    const bool live = wrow < rows;  // the wave has rows (else it only stages)
+    const int row = min(wrow + col, rows - 1), tok = row / G;
+    const size_t at = (size_t)(tok0 + tok) * Hq + h * G + row - tok * G;
+    const RowSpan span = row_span(off, tok, p.window);
+    const int kmin = off + min(wrow, rows - 1) / G, kmin_t = off + row0 / G;
+    const int wlo = p.window > 0 ? off + min(wrow + 31, rows - 1) / G - p.window + 1 : 0;
+    const int wlo_t = p.window > 0 ? kend - p.window : 0;
+
+    // Page ids of 16 units at a time, one a lane; the valid ones as a mask.
+    int ids, ids_at;
+    uint64_t ids_ok;
+    auto fetch_ids = [&](int u) __attribute__((always_inline)) {
+      ids_at = u * kWidePages;
+      const int vi = ids_at + lane;
+      ids = table[real_page(min(vi, pages - 1), wp0, sink_pages)];
+      const bool ok = vi < pages && (unsigned)ids < (unsigned)p.num_blocks;
+      if (!ok) ids = -1;
+      ids_ok = __ballot(ok);
+    };
+    auto page_pos = [&](int vi) __attribute__((always_inline)) {
+      return real_page(min(vi, pages - 1), wp0, sink_pages) * 16;
+    };
+    auto seen_whole = [&](int vi, unsigned ok, int kmin_, int wlo_) __attribute__((always_inline)) {
+      bool all = true;
+#pragma unroll
+      for (int i = 0; i < kWidePages; ++i) {
+        const int pos = page_pos(vi + i);
+        all = all & (ok >> i & 1) & (pos + 15 <= kmin_) & ((pos >= wlo_) | (pos + 16 <= p.sinks));
+      }
+      return all;
+    };
+
+    float4 q[KB];  // dimensions half * D/2 + 4 i ..
+#pragma unroll
+    for (int i = 0; i < KB; ++i)
+      q[i] = *reinterpret_cast<const float4*>(qb + at * D + half * (D / 2) + i * 4);
+    f32x16_t o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+    float m = -INFINITY, l = 0.f;
+
+    u32x4_t kst[KPT], vst[KPT];
+    auto load = [&](int u) __attribute__((always_inline)) {
+      if (u * kWidePages >= ids_at + 64) fetch_ids(u);
+#pragma unroll
+      for (int j = 0; j < KPT; ++j) {
+        const int vi = u * kWidePages + pg0 + j * (kStep / 16);
+        const int id = __builtin_amdgcn_readlane(ids, vi - ids_at);
+        const size_t base = ((size_t)(id < 0 ? 0 : id) * Hkv + h) * 16 * D;
+        const int rec = id < 0 ? 0 : min(max(kend - page_pos(vi), 0), 16) * D * 4;
+        const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(kp + base), 0, rec,
+                                                          kBufferWord3);
+        const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(vp + base), 0, rec,
+                                                          kBufferWord3);
+        kst[j] = __builtin_amdgcn_raw_buffer_load_b128(rk, voff, 0, 0);
+        vst[j] = __builtin_amdgcn_raw_buffer_load_b128(rv, voff, 0, 0);
+      }
+      return (unsigned)(ids_ok >> (u * kWidePages - ids_at)) & 15u;
+    };
+    auto store = [&](int bf, bool whole) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < KPT; ++j) {
+        const int kk = kk0 + j * kStep;
+        if (!whole) {
+          bool odd = false;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool x = (vst[j][i] & 0x7f800000u) == 0x7f800000u;
+            odd = odd || x;
+            vst[j][i] = x ? 0u : vst[j][i];
+          }
+          if (odd) atomicOr(&s_odd[bf][kk >> 5], 1u << (kk & 31));
+        }
+        *reinterpret_cast<u32x4_t*>(&s.k[bf][kk][dc * 4]) = kst[j];
+        *reinterpret_cast<u32x4_t*>(&s.v[bf][kk][dc * 4]) = vst[j];
+      }
+    };
+
+    __syncthreads();  // the stages of the segment before are read
+    if (tid < 4) s_odd[tid >> 1][tid & 1] = 0;
+    __syncthreads();
+    const int u_end = u0 + seg;
+    fetch_ids(u0);
+    unsigned ok = load(u0), ok_next = 0;
+    bool whole_t = seen_whole(u0 * kWidePages, ok, kmin_t, wlo_t);
+    store(0, whole_t);
+    __syncthreads();
+    int bf = 0;
+    for (int u = u0;; ++u) {
+      const bool more = u + 1 < u_end;
+      if (more) ok_next = load(u + 1);  // in flight during this stage's math
+      if (live) {
+        f32x16_t x[2];
+#pragma unroll
+        for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[sb][i] = 0.f;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int sb = 0; sb < 2; ++sb) {
+            const float4 a = *reinterpret_cast<const float4*>(
+                &s.k[bf][sb * 32 + col][half * (D / 2) + kb * 4]);
+            x[sb] = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x, q[kb].x, x[sb], 0, 0, 0);
+            x[sb] = __builtin_amdgcn_mfma_f32_32x32x2f32(a.y, q[kb].y, x[sb], 0, 0, 0);
+            x[sb] = __builtin_amdgcn_mfma_f32_32x32x2f32(a.z, q[kb].z, x[sb], 0, 0, 0);
+            x[sb] = __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, q[kb].w, x[sb], 0, 0, 0);
+          }
+        if (!seen_whole(u * kWidePages, ok, kmin, wlo)) {
+#pragma unroll
+          for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int kk = (i >> 2) * 8 + half * 4 + (i & 3), pg = sb * 2 + (i >> 3);
+              const bool see = (ok >> pg & 1) &
+                               span.sees(page_pos(u * kWidePages + pg) + (kk & 15), p.sinks);
+              x[sb][i] = see ? x[sb][i] : -INFINITY;
+            }
+        }
+        float mx = x[0][0];
+#pragma unroll
+        for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[sb][i]);
+        if (__any(mx * p.c > m + kLazyLog2)) {
+          const float mn = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32, 64)) * p.c);
+          const float a = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+          l *= a;
+#pragma unroll
+          for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] *= a;
+          m = mn;
+        }
+        const float nm = m == -INFINITY ? 0.f : -m;
+        float sum = 0.f;
+#pragma unroll
+        for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            x[sb][i] = __builtin_amdgcn_exp2f(fmaf(x[sb][i], p.c, nm));
+            sum += x[sb][i];
+          }
+        l += sum;
+#pragma unroll
+        for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float* v = &s.v[bf][sb * 32 + (j >> 2) * 8 + half * 4 + (j & 3)][col];
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+              o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[d * 32], x[sb][j], o[d], 0, 0, 0);
+          }
+        if (!whole_t) {
+          // What values of V that are not finite add to rows that see their keys.
+          for (int sb = 0; sb < 2; ++sb) {
+            uint32_t odd = __builtin_amdgcn_readfirstlane(s_odd[bf][sb]);
+            while (odd) {
+              const int kk = sb * 32 + __builtin_ctz(odd);
+              odd &= odd - 1;
+              if (!(ok >> (kk >> 4) & 1)) continue;
+              const int pg = real_page(u * kWidePages + (kk >> 4), wp0, sink_pages);
+              const float* src = vp + (((size_t)table[pg] * Hkv + h) * 16 + (kk & 15)) * D;
+              const bool see = span.sees(pg * 16 + (kk & 15), p.sinks);
+#pragma unroll
+              for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  const float v = src[d * 32 + (i >> 2) * 8 + half * 4 + (i & 3)];
+                  o[d][i] += see && !(v - v == 0.f) ? v : 0.f;
+                }
+            }
+          }
+        }
+      }
+      if (!more) break;
+      ok = ok_next;
+      whole_t = seen_whole((u + 1) * kWidePages, ok, kmin_t, wlo_t);
+      store(bf ^ 1, whole_t);
+      __syncthreads();
+      bf ^= 1;
+    }
+
+    // Lane holds O^T rows d = 32 db + 8 (i/4) + 4 half + i%4 of its row.
+    const float lsum = l + __shfl_xor(l, 32, 64);
+    if (seg == units) {
+      if (wrow + col < rows) {
+        float* dst = static_cast<float*>(p.out) + at * D;
+        const float inv = inverse_sum(lsum);
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int i4 = 0; i4 < 4; ++i4) {
+            const float v[4] = {o[d][i4 * 4], o[d][i4 * 4 + 1], o[d][i4 * 4 + 2],
+                                o[d][i4 * 4 + 3]};
+            write_row<float, 4>(dst + d * 32 + i4 * 8 + half * 4, v, inv);
+          }
+        if (p.lse && half == 0) p.lse[at] = state_lse(m, lsum);
+      }
+    } else if (live) {
+      float4* part = p.wide_part +
+                     (size_t)(2 * w + (head_piece ? 0 : 1)) * wide_part_slots(D) + tid;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i4 = 0; i4 < 4; ++i4)
+          part[(d * 4 + i4) * kPartLanes] = make_float4(o[d][i4 * 4], o[d][i4 * 4 + 1],
+                                                        o[d][i4 * 4 + 2], o[d][i4 * 4 + 3]);
+      part[4 * DB * kPartLanes] = make_float4(m, lsum, 0.f, 0.f);
     }
     left -= seg;
     u0 = 0;
@@ -959,7 +1181,7 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
 // dimension block d of the tile that workgroup w's share ends in, if others
 // hold the rest of it. The pieces combine online in their order.
 template <typename T, int D>
-__global__ __launch_bounds__(kWideThreads) void chunk_merge_kernel(ChunkParams p) {
+__global__ __launch_bounds__(kPartLanes) void chunk_merge_kernel(ChunkParams p) {
   constexpr int DB = D / 32;
   if (p.v.head->stamp != p.stamp) return;
   const int w = blockIdx.x / DB, d = blockIdx.x % DB;
@@ -992,11 +1214,11 @@ __global__ __launch_bounds__(kWideThreads) void chunk_merge_kernel(ChunkParams p
   for (int i = 0; i < 16; ++i) acc[i] = 0.f;
   for (int k = w; k <= share.last; ++k) {
     const float4* part = p.wide_part +
-                         (size_t)(2 * k + (k == w ? 1 : 0)) * (4 * DB + 1) * kWideThreads + tid;
-    const float4 ml = part[4 * DB * kWideThreads];
+                         (size_t)(2 * k + (k == w ? 1 : 0)) * wide_part_slots(D) + tid;
+    const float4 ml = part[4 * DB * kPartLanes];
     float4 a[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) a[i] = part[(d * 4 + i) * kWideThreads];
+    for (int i = 0; i < 4; ++i) a[i] = part[(d * 4 + i) * kPartLanes];
     const float mn = fmaxf(M, ml.x);
     const float sa = state_weight(M, mn), sb = state_weight(ml.x, mn);
     L = L * sa + ml.y * sb;
@@ -1030,7 +1252,7 @@ ChunkWorkspace chunk_workspace(int max_rows, int D, int cus) {
   ws.wide = ws.thin + (size_t)4 * cus * kThinRows * (D + 2) * sizeof(float);
   ws.bytes = ws.wide;
   if (max_rows > kThinRows)
-    ws.bytes += (size_t)2 * cus * (D / 8 + 1) * kWideThreads * sizeof(float4);
+    ws.bytes += (size_t)2 * cus * wide_part_slots(D) * sizeof(float4);
   return ws;
 }
 
@@ -1046,10 +1268,13 @@ int launch_chunk(const ChunkParams& p, int max_rows, int thin_rows, int cus, hip
     st = launch_status("chunk_thin_kernel");
   }
   if (st || max_rows <= thin_rows) return st;
-  hipLaunchKernelGGL((chunk_wide_kernel<T, D>), dim3(cus), dim3(kWideThreads), 0, stream, p);
+  if constexpr (sizeof(T) == 4)
+    hipLaunchKernelGGL((chunk_wide32_kernel<D>), dim3(cus), dim3(kWide32Threads), 0, stream, p);
+  else
+    hipLaunchKernelGGL((chunk_wide_kernel<T, D>), dim3(cus), dim3(kWideThreads), 0, stream, p);
   st = launch_status("chunk_wide_kernel");
   if (st) return st;
-  hipLaunchKernelGGL((chunk_merge_kernel<T, D>), dim3(cus * (D / 32)), dim3(kWideThreads), 0,
+  hipLaunchKernelGGL((chunk_merge_kernel<T, D>), dim3(cus * (D / 32)), dim3(kPartLanes), 0,
                      stream, p);
   return launch_status("chunk_merge_kernel");
 }
