@@ -555,6 +555,27 @@ constexpr int kPartLanes = 2 * kWideRows;  // two lanes a row
 // its (m, l).
 constexpr int wide_part_slots(int D) { return (D / 8 + 1) * kPartLanes; }
 
+// The units (of kWidePages pages, 64 keys) of a wide tile whose keys some rows
+// all see: from lo to hi - 1, and the first `sunk` among the sinks. kmin: the
+// first row's own key; wlo: where the last row's window starts. Worked out
+// once per tile, so that a unit costs the loop three comparisons.
+struct UnitSpan {
+  int lo, hi, sunk;
+  __device__ __forceinline__ bool has(int u) const {
+    return ((u >= lo) & (u < hi)) | (u < sunk);
+  }
+};
+__device__ __forceinline__ UnitSpan unit_span(int kmin, int wlo, int wp0, int sink_pages,
+                                              int sinks) {
+  constexpr int P = kWidePages;
+  const int skip = wp0 > 0 ? sink_pages : 0;  // virtual pages before the window's
+  UnitSpan s;
+  s.lo = (skip + max(0, ((wlo + 15) >> 4) - wp0) + P - 1) / P;
+  s.hi = max(0, ((kmin + 1) >> 4) - wp0 + skip) / P;
+  s.sunk = min(sinks / (16 * P), wp0 > 0 ? sink_pages / P : s.hi);
+  return s;
+}
+
 // ---------------------------------------------------------------------------
 // Wide sequences, 16-bit
 // ---------------------------------------------------------------------------
@@ -646,9 +667,13 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
     const int row = min(wrow + col, rows - 1), tok = row / G;
     const size_t at = (size_t)(tok0 + tok) * Hq + h * G + row - tok * G;
     const RowSpan span = row_span(off, tok, p.window);
-    const int kmin = off + min(wrow, rows - 1) / G, kmin_t = off + row0 / G;
-    const int wlo = p.window > 0 ? off + min(wrow + 31, rows - 1) / G - p.window + 1 : 0;
-    const int wlo_t = p.window > 0 ? kend - p.window : 0;
+    // The units that every row of the wave sees whole, and of the tile.
+    const UnitSpan mine = unit_span(
+        off + min(wrow, rows - 1) / G,
+        p.window > 0 ? off + min(wrow + 31, rows - 1) / G - p.window + 1 : 0, wp0, sink_pages,
+        p.sinks);
+    const UnitSpan all = unit_span(off + row0 / G, p.window > 0 ? kend - p.window : 0, wp0,
+                                   sink_pages, p.sinks);
 
     // Page ids of 16 units at a time, one a lane; the valid ones as a mask.
     int ids, ids_at;
@@ -664,15 +689,6 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
     auto page_pos = [&](int vi) __attribute__((always_inline)) {
       return real_page(min(vi, pages - 1), wp0, sink_pages) * 16;
     };
-    auto seen_whole = [&](int vi, unsigned ok, int kmin_, int wlo_) __attribute__((always_inline)) {
-      bool all = true;
-#pragma unroll
-      for (int i = 0; i < kWidePages; ++i) {
-        const int pos = page_pos(vi + i);
-        all = all & (ok >> i & 1) & (pos + 15 <= kmin_) & ((pos >= wlo_) | (pos + 16 <= p.sinks));
-      }
-      return all;
-    };
 
     uint4 q[KB];
 #pragma unroll
@@ -685,6 +701,13 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
       for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
     float m = -INFINITY, l = 0.f;
 
+    // Raw buffer loads through descriptors of the (page, head) tiles: no valid
+    // page is a descriptor of no records, and the keys of the last page that
+    // no row sees lie past its end; both read as zeros.
+    const T* __restrict__ kh = kp + (size_t)h * 16 * D;
+    const T* __restrict__ vh = vp + (size_t)h * 16 * D;
+    const unsigned page_elems = Hkv * 16 * D;
+    const int last_rec = (((kend - 1) & 15) + 1) * D * 2;
     u32x4_t kst[KPT], vst[KPT];
     auto load = [&](int u) __attribute__((always_inline)) {
       if (u * kWidePages >= ids_at + 64) fetch_ids(u);
@@ -692,11 +715,11 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
       for (int j = 0; j < KPT; ++j) {
         const int vi = u * kWidePages + pg0 + j * (kStep / 16);
         const int id = __builtin_amdgcn_readlane(ids, vi - ids_at);
-        const size_t base = ((size_t)(id < 0 ? 0 : id) * Hkv + h) * 16 * D;
-        const int rec = id < 0 ? 0 : min(max(kend - page_pos(vi), 0), 16) * D * 2;
-        const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(kp + base), 0, rec,
+        const size_t base = (size_t)(unsigned)max(id, 0) * page_elems;
+        const int rec = id < 0 ? 0 : vi + 1 < pages ? 16 * D * 2 : last_rec;
+        const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(kh + base), 0, rec,
                                                           kBufferWord3);
-        const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(vp + base), 0, rec,
+        const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(vh + base), 0, rec,
                                                           kBufferWord3);
         kst[j] = __builtin_amdgcn_raw_buffer_load_b128(rk, voff, 0, 0);
         vst[j] = __builtin_amdgcn_raw_buffer_load_b128(rv, voff, 0, 0);
@@ -730,7 +753,7 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
     const int u_end = u0 + seg;
     fetch_ids(u0);
     unsigned ok = load(u0), ok_next = 0;
-    bool whole_t = seen_whole(u0 * kWidePages, ok, kmin_t, wlo_t);
+    bool whole_t = ok == 15u && all.has(u0);
     store(0, whole_t);
     __syncthreads();
     int bf = 0;
@@ -751,7 +774,7 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
                 *reinterpret_cast<const uint4*>(&s.k[bf][sb * 32 + col][kb * 16 + half * 8]),
                 q[kb], x[sb]);
           }
-        if (!seen_whole(u * kWidePages, ok, kmin, wlo)) {
+        if (!(ok == 15u && mine.has(u))) {
 #pragma unroll
           for (int sb = 0; sb < 2; ++sb)
 #pragma unroll
@@ -838,7 +861,7 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
       }
       if (!more) break;
       ok = ok_next;
-      whole_t = seen_whole((u + 1) * kWidePages, ok, kmin_t, wlo_t);
+      whole_t = ok == 15u && all.has(u + 1);
       store(bf ^ 1, whole_t);
       __syncthreads();
       bf ^= 1;
@@ -959,9 +982,13 @@ __global__ __launch_bounds__(kWide32Threads, 1) void chunk_wide32_kernel(ChunkPa
     const int row = min(wrow + col, rows - 1), tok = row / G;
     const size_t at = (size_t)(tok0 + tok) * Hq + h * G + row - tok * G;
     const RowSpan span = row_span(off, tok, p.window);
-    const int kmin = off + min(wrow, rows - 1) / G, kmin_t = off + row0 / G;
-    const int wlo = p.window > 0 ? off + min(wrow + 31, rows - 1) / G - p.window + 1 : 0;
-    const int wlo_t = p.window > 0 ? kend - p.window : 0;
+    // The units that every row of the wave sees whole, and of the tile.
+    const UnitSpan mine = unit_span(
+        off + min(wrow, rows - 1) / G,
+        p.window > 0 ? off + min(wrow + 31, rows - 1) / G - p.window + 1 : 0, wp0, sink_pages,
+        p.sinks);
+    const UnitSpan all = unit_span(off + row0 / G, p.window > 0 ? kend - p.window : 0, wp0,
+                                   sink_pages, p.sinks);
 
     // Page ids of 16 units at a time, one a lane; the valid ones as a mask.
     int ids, ids_at;
@@ -977,15 +1004,6 @@ __global__ __launch_bounds__(kWide32Threads, 1) void chunk_wide32_kernel(ChunkPa
     auto page_pos = [&](int vi) __attribute__((always_inline)) {
       return real_page(min(vi, pages - 1), wp0, sink_pages) * 16;
     };
-    auto seen_whole = [&](int vi, unsigned ok, int kmin_, int wlo_) __attribute__((always_inline)) {
-      bool all = true;
-#pragma unroll
-      for (int i = 0; i < kWidePages; ++i) {
-        const int pos = page_pos(vi + i);
-        all = all & (ok >> i & 1) & (pos + 15 <= kmin_) & ((pos >= wlo_) | (pos + 16 <= p.sinks));
-      }
-      return all;
-    };
 
     float4 q[KB];  // dimensions half * D/2 + 4 i ..
 #pragma unroll
@@ -998,6 +1016,13 @@ __global__ __launch_bounds__(kWide32Threads, 1) void chunk_wide32_kernel(ChunkPa
       for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
     float m = -INFINITY, l = 0.f;
 
+    // Raw buffer loads through descriptors of the (page, head) tiles: no valid
+    // page is a descriptor of no records, and the keys of the last page that
+    // no row sees lie past its end; both read as zeros.
+    const float* __restrict__ kh = kp + (size_t)h * 16 * D;
+    const float* __restrict__ vh = vp + (size_t)h * 16 * D;
+    const unsigned page_elems = Hkv * 16 * D;
+    const int last_rec = (((kend - 1) & 15) + 1) * D * 4;
     u32x4_t kst[KPT], vst[KPT];
     auto load = [&](int u) __attribute__((always_inline)) {
       if (u * kWidePages >= ids_at + 64) fetch_ids(u);
@@ -1005,11 +1030,11 @@ __global__ __launch_bounds__(kWide32Threads, 1) void chunk_wide32_kernel(ChunkPa
       for (int j = 0; j < KPT; ++j) {
         const int vi = u * kWidePages + pg0 + j * (kStep / 16);
         const int id = __builtin_amdgcn_readlane(ids, vi - ids_at);
-        const size_t base = ((size_t)(id < 0 ? 0 : id) * Hkv + h) * 16 * D;
-        const int rec = id < 0 ? 0 : min(max(kend - page_pos(vi), 0), 16) * D * 4;
-        const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(kp + base), 0, rec,
+        const size_t base = (size_t)(unsigned)max(id, 0) * page_elems;
+        const int rec = id < 0 ? 0 : vi + 1 < pages ? 16 * D * 4 : last_rec;
+        const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(kh + base), 0, rec,
                                                           kBufferWord3);
-        const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(vp + base), 0, rec,
+        const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(vh + base), 0, rec,
                                                           kBufferWord3);
         kst[j] = __builtin_amdgcn_raw_buffer_load_b128(rk, voff, 0, 0);
         vst[j] = __builtin_amdgcn_raw_buffer_load_b128(rv, voff, 0, 0);
@@ -1041,7 +1066,7 @@ __global__ __launch_bounds__(kWide32Threads, 1) void chunk_wide32_kernel(ChunkPa
     const int u_end = u0 + seg;
     fetch_ids(u0);
     unsigned ok = load(u0), ok_next = 0;
-    bool whole_t = seen_whole(u0 * kWidePages, ok, kmin_t, wlo_t);
+    bool whole_t = ok == 15u && all.has(u0);
     store(0, whole_t);
     __syncthreads();
     int bf = 0;
@@ -1065,7 +1090,7 @@ __global__ __launch_bounds__(kWide32Threads, 1) void chunk_wide32_kernel(ChunkPa
             x[sb] = __builtin_amdgcn_mfma_f32_32x32x2f32(a.z, q[kb].z, x[sb], 0, 0, 0);
             x[sb] = __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, q[kb].w, x[sb], 0, 0, 0);
           }
-        if (!seen_whole(u * kWidePages, ok, kmin, wlo)) {
+        if (!(ok == 15u && mine.has(u))) {
 #pragma unroll
           for (int sb = 0; sb < 2; ++sb)
 #pragma unroll
@@ -1134,7 +1159,7 @@ __global__ __launch_bounds__(kWide32Threads, 1) void chunk_wide32_kernel(ChunkPa
       }
       if (!more) break;
       ok = ok_next;
-      whole_t = seen_whole((u + 1) * kWidePages, ok, kmin_t, wlo_t);
+      whole_t = ok == 15u && all.has(u + 1);
       store(bf ^ 1, whole_t);
       __syncthreads();
       bf ^= 1;
