@@ -1214,22 +1214,8 @@ __global__ __launch_bounds__(kPartLanes) void chunk_merge_kernel(ChunkParams p) 
   if (w >= groups) return;
   const ChunkShare share = p.v.wide_share[w];
   if (share.last == w) return;
-  // The tile the share ends in, and its head.
-  const int tiles = p.v.head->wide_tiles, units = p.v.head->wide_units;
-  const long long end =
-      (long long)share.head * units + p.v.wide[share.tile].unit0 + share.u0 + share.count - 1;
-  const int h = (int)(end / units), u = (int)(end - (long long)h * units);
-  int lo = 0, hi = tiles;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (p.v.wide[mid].unit0 <= u) lo = mid; else hi = mid;
-  }
-  const ChunkTile t = p.v.wide[lo];
-  // (A share inside one tile of three pieces or more: its first piece's
-  // workgroup joins it.)
-  const long long begin = (long long)share.head * units + p.v.wide[share.tile].unit0 + share.u0;
-  if ((long long)h * units + t.unit0 < begin) return;
-
+  const ChunkTile t = p.v.wide[share.end_tile];
+  const int h = share.end_head;
   const int tid = threadIdx.x;
   const int wave = tid >> 6, lane = tid & 63, half = lane >> 5, col = lane & 31;
   const int row = t.row0 + wave * 32 + col, rows = t.n * p.G;

@@ -52,10 +52,11 @@ struct ChunkTile {
 
 // A workgroup's share of a list: units u0 .. of (head, tile), count in all,
 // going on through the following tiles. first: the workgroup that holds the
-// start of that first tile; last: the one that holds the end of the tile the
-// share ends in (w itself where it ends with a whole tile).
+// start of that first tile. The share ends in (end_head, end_tile), whose end
+// workgroup `last` holds: w itself, too, where the tile started before the
+// share (another workgroup then joins its pieces).
 struct ChunkShare {
-  int tile, head, u0, count, first, last, pad0, pad1;
+  int tile, head, u0, count, first, last, end_tile, end_head;
 };
 
 struct ChunkHead {

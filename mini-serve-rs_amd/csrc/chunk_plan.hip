@@ -46,24 +46,27 @@ __device__ __forceinline__ int block_scan(int x, int* s_w, int* sum) {
   return before + inc - x;
 }
 
-// Last index i of a[0..n) with a[i].unit0 <= u (a[0].unit0 = 0).
-__device__ __forceinline__ int tile_of(const ChunkTile* a, int n, int u) {
+// Last index i of a[0..n) with a[i] <= u (a[0] = 0). The first kHeld prefixes
+// are held in LDS: a search through memory is a round trip per step.
+constexpr int kHeld = 4096;
+__device__ __forceinline__ int tile_of(const int* held, const ChunkTile* a, int n, int u) {
   int lo = 0, hi = n;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (a[mid].unit0 <= u) lo = mid; else hi = mid;
+    if ((mid < kHeld ? held[mid] : a[mid].unit0) <= u) lo = mid; else hi = mid;
   }
   return lo;
 }
 
 // Shares of `units` units of each of Hkv heads over at most max_groups
 // workgroups of at least min_units each.
-__device__ int deal(const ChunkTile* tiles, int n, int units, int Hkv, int max_groups,
-                    int min_units, ChunkShare* out) {
+__device__ int deal(const int* held, const ChunkTile* tiles, int n, int units, int Hkv,
+                    int max_groups, int min_units, ChunkShare* out) {
   const long long total = (long long)units * Hkv;
   if (total == 0) return 0;
   const long long want = (total + min_units - 1) / min_units;
   const int groups = (int)(want < max_groups ? want : max_groups);
+  auto unit0 = [&](int i) { return i < n ? (i < kHeld ? held[i] : tiles[i].unit0) : units; };
   for (int w = threadIdx.x; w < groups; w += kPlanThreads) {
     const long long a = total * w / groups, b = total * (w + 1) / groups;
     // The workgroup holding unit x is the largest w' with w' * total / groups <= x.
@@ -71,16 +74,15 @@ __device__ int deal(const ChunkTile* tiles, int n, int units, int Hkv, int max_g
     ChunkShare s;
     s.head = (int)(a / units);
     const int u = (int)(a - (long long)s.head * units);
-    s.tile = tile_of(tiles, n, u);
-    s.u0 = u - tiles[s.tile].unit0;
+    s.tile = tile_of(held, tiles, n, u);
+    s.u0 = u - unit0(s.tile);
     s.count = (int)(b - a);
     s.first = s.u0 ? holder(a - s.u0) : w;
-    const long long e = b - 1;
-    const long long eh = e / units;
-    const int et = tile_of(tiles, n, (int)(e - eh * units));
-    const long long end = eh * units + (et + 1 < n ? tiles[et + 1].unit0 : units);
-    s.last = end > b ? holder(end - 1) : w;
-    s.pad0 = s.pad1 = 0;
+    s.end_head = (int)((b - 1) / units);
+    const long long base = (long long)s.end_head * units;
+    s.end_tile = tile_of(held, tiles, n, (int)(b - 1 - base));
+    const long long end = base + unit0(s.end_tile + 1);
+    s.last = end > b && base + unit0(s.end_tile) >= a ? holder(end - 1) : w;
     out[w] = s;
   }
   return groups;
@@ -89,6 +91,7 @@ __device__ int deal(const ChunkTile* tiles, int n, int units, int Hkv, int max_g
 __global__ __launch_bounds__(kPlanThreads) void chunk_plan_kernel(PlanParams p) {
   __shared__ int s_wide[kMaxChunkSeqs + 1];  // wide tiles before each sequence
   __shared__ int s_w[kPlanWaves];
+  __shared__ int s_thin[kHeld], s_unit[kHeld];  // unit0 of the thin and the wide tiles
   __shared__ unsigned s_flags;
   const int tid = threadIdx.x;
   if (tid == 0) s_flags = 0;
@@ -126,6 +129,7 @@ __global__ __launch_bounds__(kPlanThreads) void chunk_plan_kernel(PlanParams p) 
     if (thin) {
       t.unit0 = u;
       p.v.thin[at] = t;
+      if (at < kHeld) s_thin[at] = u;
     }
     at = block_scan(wide, s_w, &sum) + score_seqs;
     score_seqs += sum;
@@ -167,13 +171,16 @@ __global__ __launch_bounds__(kPlanThreads) void chunk_plan_kernel(PlanParams p) 
     int sum;
     t.unit0 = block_scan(units, s_w, &sum) + wide_units;
     wide_units += sum;
-    if (i < wide_tiles) p.v.wide[i] = t;
+    if (i < wide_tiles) {
+      p.v.wide[i] = t;
+      if (i < kHeld) s_unit[i] = t.unit0;
+    }
   }
   __syncthreads();
 
-  const int tg = deal(p.v.thin, thin_tiles, thin_units, p.Hkv, 2 * p.cus, kThinMinUnits,
+  const int tg = deal(s_thin, p.v.thin, thin_tiles, thin_units, p.Hkv, 2 * p.cus, kThinMinUnits,
                       p.v.thin_share);
-  const int wg = deal(p.v.wide, wide_tiles, wide_units, p.Hkv, p.cus, kWideMinUnits,
+  const int wg = deal(s_unit, p.v.wide, wide_tiles, wide_units, p.Hkv, p.cus, kWideMinUnits,
                       p.v.wide_share);
   if (tid == 0) {
     ChunkHead h;
