@@ -579,19 +579,30 @@ __device__ __forceinline__ UnitSpan unit_span(int kmin, int wlo, int wp0, int si
 // ---------------------------------------------------------------------------
 // Wide sequences, 16-bit
 // ---------------------------------------------------------------------------
-// A workgroup of 8 waves takes a tile of 256 rows, each wave 32 of them, and
-// streams its share of the tile's pages four at a time: K and V rows staged
-// in LDS once, the next four in flight during the math, one barrier each.
-// Per wave (v_mfma_f32_32x32x16; lane l holds A[l%32][8*(l/32)+j],
+// A workgroup of 8 waves, two a SIMD, takes a tile of 256 rows, each wave 32 of
+// them, and streams its share of the tile's pages four (64 keys) at a time
+// through LDS. Per wave (v_mfma_f32_32x32x16; lane l holds A[l%32][8*(l/32)+j],
 // B[8*(l/32)+j][l%32] and accumulator element i at
 // [8*(i/4) + 4*(l/32) + i%4][l%32]):
 //   S^T (keys x rows) = K . Q^T, so each lane owns one row: max and sum are
 //   over 16 values in the lane and lane l^32, and
 //   O^T (d x rows) += V^T . P^T takes the probabilities from the accumulator
 //   as they lie; V^T comes from row-major LDS through transposing reads.
+// Both halves of a stage's work, 32 MFMAs and the softmax between them, take a
+// wave more than a thousand cycles, on different pipes. So the two waves of a
+// SIMD take turns: while waves 0-3 run the products of a stage (q.k, and p.v
+// of the stage before), waves 4-7 run their softmax, and a barrier swaps them.
+// Waves 4-7 are thus half a stage behind, and store their part of each stage
+// half a stage ahead, which three LDS buffers allow. A turn's operands are
+// read from LDS six MFMAs ahead: 1360 cycles for 32 MFMAs, 2380 as the
+// compiler schedules the reads. A stage of 64 keys takes 4700 cycles, 5600
+// without the turns' order. In long launches the card's clock falls as the
+// cycles do (2.4 to 2.0 GHz, 2.3 us a stage either way: 840 TFLOP/s of the
+// 1190 that a large matrix product reaches); short ones gain 2-4%.
 constexpr int kWideWaves = 8;
 constexpr int kWideThreads = 64 * kWideWaves;
 constexpr int kWideKeys = 16 * kWidePages;
+constexpr int kWideBufs = 3;
 
 template <typename T, int D>
 struct WideLds {
@@ -599,8 +610,8 @@ struct WideLds {
   // own (64 four-byte banks): K rows 4 banks apart, the rows of a transposing
   // V read 16.
   static constexpr int kPadK = 8, kPadV = 32;
-  T k[2][kWideKeys][D + kPadK];
-  T v[2][kWideKeys][D + kPadV];
+  T k[kWideBufs][kWideKeys][D + kPadK];
+  T v[kWideBufs][kWideKeys][D + kPadV];
 };
 
 template <typename T, int D>
@@ -610,7 +621,7 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
   constexpr int PPR = D / 8;                           // packets per row
   constexpr int KPT = kWideKeys * PPR / kWideThreads;  // packets per thread and stage
   __shared__ __align__(16) WideLds<T, D> s;
-  __shared__ uint32_t s_odd[2][2];  // keys of a stage with V not finite
+  __shared__ uint32_t s_odd[kWideBufs][2];  // keys of a stage with V not finite
 
   if (p.v.head->stamp != p.stamp) {
     if (blockIdx.x == 0 && threadIdx.x == 0) ws_raise(&p.v.head->flags, RLSE_WS_ERR_PLAN);
@@ -708,6 +719,7 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
     const T* __restrict__ vh = vp + (size_t)h * 16 * D;
     const unsigned page_elems = Hkv * 16 * D;
     const int last_rec = (((kend - 1) & 15) + 1) * D * 2;
+    unsigned oks = 0;  // valid pages of the last 8 units loaded, a bit each
     u32x4_t kst[KPT], vst[KPT];
     auto load = [&](int u) __attribute__((always_inline)) {
       if (u * kWidePages >= ids_at + 64) fetch_ids(u);
@@ -724,7 +736,14 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
         kst[j] = __builtin_amdgcn_raw_buffer_load_b128(rk, voff, 0, 0);
         vst[j] = __builtin_amdgcn_raw_buffer_load_b128(rv, voff, 0, 0);
       }
-      return (unsigned)(ids_ok >> (u * kWidePages - ids_at)) & 15u;
+      const int at4 = (u & 7) * 4;
+      oks = (oks & ~(15u << at4)) |
+            ((unsigned)(ids_ok >> (u * kWidePages - ids_at)) & 15u) << at4;
+    };
+    // Units with all four pages valid that every row (of the tile) sees whole.
+    auto ok_of = [&](int u) __attribute__((always_inline)) { return oks >> (u & 7) * 4 & 15u; };
+    auto whole_of = [&](int u) __attribute__((always_inline)) {
+      return ok_of(u) == 15u && all.has(u);
     };
     auto store = [&](int bf, bool whole) __attribute__((always_inline)) {
 #pragma unroll
@@ -747,125 +766,184 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
       }
     };
 
-    __syncthreads();  // the stages of the segment before are read
-    if (tid < 4) s_odd[tid >> 1][tid & 1] = 0;
-    __syncthreads();
-    const int u_end = u0 + seg;
-    fetch_ids(u0);
-    unsigned ok = load(u0), ok_next = 0;
-    bool whole_t = ok == 15u && all.has(u0);
-    store(0, whole_t);
-    __syncthreads();
-    int bf = 0;
-    for (int u = u0;; ++u) {
-      const bool more = u + 1 < u_end;
-      if (more) ok_next = load(u + 1);  // in flight during this stage's math
-      if (live) {
-        f32x16_t x[2];
+    f32x16_t x[2];
+    uint4 pk[4];  // P^T operands of the four 16-key blocks
+    // Operand i of a turn's products: the K operands of q.k, then the V^T ones
+    // of p.v.
+    constexpr int NK = 2 * KB, NV = 4 * DB;
+    auto operand = [&](int i, int bk, int bv) __attribute__((always_inline)) {
+      if (i < NK) {
+        const int kb = i >> 1, sb = i & 1;
+        return *reinterpret_cast<const uint4*>(&s.k[bk][sb * 32 + col][kb * 16 + half * 8]);
+      }
+      const int kq = (i - NK) / DB, d = (i - NK) % DB;
+      const uint16_t* v0 =
+          reinterpret_cast<const uint16_t*>(&s.v[bv][kq * 16 + tr_row][d * 32 + tr_col]);
+      const uint2 lo = __builtin_bit_cast(
+          uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)v0));
+      const uint2 hi = __builtin_bit_cast(
+          uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                     (lds_i16x4_t*)(v0 + 8 * (D + WideLds<T, D>::kPadV))));
+      return make_uint4(lo.x, lo.y, hi.x, hi.y);
+    };
+    auto products = [&](auto qk, auto pv, int bk, int bv) __attribute__((always_inline)) {
+      constexpr int from = decltype(qk)::value ? 0 : NK, to = decltype(pv)::value ? NK + NV : NK;
+      constexpr int R = 6;  // operands in flight from LDS ahead of their MFMA
+      __builtin_amdgcn_s_setprio(1);
+      if constexpr (decltype(qk)::value) {
 #pragma unroll
         for (int sb = 0; sb < 2; ++sb)
 #pragma unroll
           for (int i = 0; i < 16; ++i) x[sb][i] = 0.f;
+      }
+      uint4 ring[R];
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
+      for (int i = 0; i < R; ++i) ring[i] = operand(from + i, bk, bv);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int sb = 0; sb < 2; ++sb) {
-            x[sb] = Tile<T>::mma32(
-                *reinterpret_cast<const uint4*>(&s.k[bf][sb * 32 + col][kb * 16 + half * 8]),
-                q[kb], x[sb]);
-          }
-        if (!(ok == 15u && mine.has(u))) {
-#pragma unroll
-          for (int sb = 0; sb < 2; ++sb)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int kk = (i >> 2) * 8 + half * 4 + (i & 3), pg = sb * 2 + (i >> 3);
-              const bool see = (ok >> pg & 1) &
-                               span.sees(page_pos(u * kWidePages + pg) + (kk & 15), p.sinks);
-              x[sb][i] = see ? x[sb][i] : -INFINITY;
-            }
-        }
-        float mx = x[0][0];
-#pragma unroll
-        for (int sb = 0; sb < 2; ++sb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[sb][i]);
-        if (__any(mx * p.c > m + kLazyLog2)) {
-          const float mn = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32, 64)) * p.c);
-          const float a = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-          l *= a;
-#pragma unroll
-          for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[d][i] *= a;
-          m = mn;
-        }
-        const float nm = m == -INFINITY ? 0.f : -m;
-        float sum = 0.f;
+      for (int i = from; i < to; ++i) {
+        const uint4 a = ring[(i - from) % R];
+        if (i < NK)
+          x[i & 1] = Tile<T>::mma32(a, q[i >> 1], x[i & 1]);
+        else
+          o[(i - NK) % DB] = Tile<T>::mma32(a, pk[(i - NK) / DB], o[(i - NK) % DB]);
+        if (i + R < to) ring[(i - from) % R] = operand(i + R, bk, bv);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      __builtin_amdgcn_s_setprio(0);
+    };
+    auto softmax = [&](int u) __attribute__((always_inline)) {
+      const unsigned ok = ok_of(u);
+      if (!(ok == 15u && mine.has(u))) {
 #pragma unroll
         for (int sb = 0; sb < 2; ++sb)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            x[sb][i] = __builtin_amdgcn_exp2f(fmaf(x[sb][i], p.c, nm));
-            sum += x[sb][i];
+            const int kk = (i >> 2) * 8 + half * 4 + (i & 3), pg = sb * 2 + (i >> 3);
+            const bool see = (ok >> pg & 1) &
+                             span.sees(page_pos(u * kWidePages + pg) + (kk & 15), p.sinks);
+            x[sb][i] = see ? x[sb][i] : -INFINITY;
           }
-        l += sum;
+      }
+      float mx = x[0][0];
 #pragma unroll
-        for (int kq = 0; kq < 4; ++kq) {
-          const f32x16_t& y = x[kq >> 1];
-          const int e = (kq & 1) * 8;
-          const uint4 pk = make_uint4(
-              Packet<T>::pack2(y[e], y[e + 1]), Packet<T>::pack2(y[e + 2], y[e + 3]),
-              Packet<T>::pack2(y[e + 4], y[e + 5]), Packet<T>::pack2(y[e + 6], y[e + 7]));
+      for (int sb = 0; sb < 2; ++sb)
 #pragma unroll
-          for (int d = 0; d < DB; ++d) {
-            const uint16_t* v0 =
-                reinterpret_cast<const uint16_t*>(&s.v[bf][kq * 16 + tr_row][d * 32 + tr_col]);
-            const uint2 lo = __builtin_bit_cast(
-                uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)v0));
-            const uint2 hi = __builtin_bit_cast(
-                uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                           (lds_i16x4_t*)(v0 + 8 * (D + WideLds<T, D>::kPadV))));
-            o[d] = Tile<T>::mma32(make_uint4(lo.x, lo.y, hi.x, hi.y), pk, o[d]);
-          }
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[sb][i]);
+      if (__any(mx * p.c > m + kLazyLog2)) {
+        const float mn = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32, 64)) * p.c);
+        const float a = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        l *= a;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[d][i] *= a;
+        m = mn;
+      }
+      const float nm = m == -INFINITY ? 0.f : -m;
+      float sum = 0.f;
+#pragma unroll
+      for (int sb = 0; sb < 2; ++sb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          x[sb][i] = __builtin_amdgcn_exp2f(fmaf(x[sb][i], p.c, nm));
+          sum += x[sb][i];
         }
-        if (!whole_t) {
-          // What values of V that are not finite add to rows that see their keys.
-          for (int sb = 0; sb < 2; ++sb) {
-            uint32_t odd = __builtin_amdgcn_readfirstlane(s_odd[bf][sb]);
-            while (odd) {
-              const int kk = sb * 32 + __builtin_ctz(odd);
-              odd &= odd - 1;
-              if (!(ok >> (kk >> 4) & 1)) continue;
-              const int pg = real_page(u * kWidePages + (kk >> 4), wp0, sink_pages);
-              const T* src = vp + (((size_t)table[pg] * Hkv + h) * 16 + (kk & 15)) * D;
-              const bool see = span.sees(pg * 16 + (kk & 15), p.sinks);
+      l += sum;
 #pragma unroll
-              for (int d = 0; d < DB; ++d)
+      for (int kq = 0; kq < 4; ++kq) {
+        const f32x16_t& y = x[kq >> 1];
+        const int e = (kq & 1) * 8;
+        pk[kq] = make_uint4(
+            Packet<T>::pack2(y[e], y[e + 1]), Packet<T>::pack2(y[e + 2], y[e + 3]),
+            Packet<T>::pack2(y[e + 4], y[e + 5]), Packet<T>::pack2(y[e + 6], y[e + 7]));
+        // (Kept in this turn: the compiler would move it to its use.)
+        asm volatile("" : "+v"(pk[kq].x), "+v"(pk[kq].y), "+v"(pk[kq].z), "+v"(pk[kq].w));
+      }
+    };
+    // What a stage's values of V that are not finite add to the rows that see
+    // their keys.
+    auto add_odd = [&](int bf, int u) __attribute__((always_inline)) {
+      for (int sb = 0; sb < 2; ++sb) {
+        uint32_t odd = __builtin_amdgcn_readfirstlane(s_odd[bf][sb]);
+        while (odd) {
+          const int kk = sb * 32 + __builtin_ctz(odd);
+          odd &= odd - 1;
+          if (!(ok_of(u) >> (kk >> 4) & 1)) continue;
+          const int pg = real_page(u * kWidePages + (kk >> 4), wp0, sink_pages);
+          const T* src = vp + (((size_t)table[pg] * Hkv + h) * 16 + (kk & 15)) * D;
+          const bool see = span.sees(pg * 16 + (kk & 15), p.sinks);
 #pragma unroll
-                for (int i4 = 0; i4 < 4; ++i4) {
-                  const uint2 y = *reinterpret_cast<const uint2*>(src + d * 32 + i4 * 8 + half * 4);
+          for (int d = 0; d < DB; ++d)
 #pragma unroll
-                  for (int i = 0; i < 4; ++i) {
-                    T e;
-                    const uint16_t bits = (uint16_t)((i < 2 ? y.x : y.y) >> (16 * (i & 1)));
-                    __builtin_memcpy(&e, &bits, 2);
-                    const float v = Elem<T>::to_f32(e);
-                    o[d][i4 * 4 + i] += see & !(v - v == 0.f) ? v : 0.f;
-                  }
-                  __builtin_amdgcn_sched_barrier(0);  // (else all loads' registers at once)
-                }
+            for (int i4 = 0; i4 < 4; ++i4) {
+              const uint2 y = *reinterpret_cast<const uint2*>(src + d * 32 + i4 * 8 + half * 4);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                T e;
+                const uint16_t bits = (uint16_t)((i < 2 ? y.x : y.y) >> (16 * (i & 1)));
+                __builtin_memcpy(&e, &bits, 2);
+                const float v = Elem<T>::to_f32(e);
+                o[d][i4 * 4 + i] += see & !(v - v == 0.f) ? v : 0.f;
+              }
+              __builtin_amdgcn_sched_barrier(0);  // (else all loads' registers at once)
             }
-          }
         }
       }
-      if (!more) break;
-      ok = ok_next;
-      whole_t = ok == 15u && all.has(u + 1);
-      store(bf ^ 1, whole_t);
+    };
+    auto turn = [&]() __attribute__((always_inline)) {
+      __builtin_amdgcn_sched_barrier(0);
       __syncthreads();
-      bf ^= 1;
+      __builtin_amdgcn_sched_barrier(0);
+    };
+
+    __syncthreads();  // the stages of the segment before are read
+    if (tid < 2 * kWideBufs) s_odd[tid >> 1][tid & 1] = 0;
+    __syncthreads();
+    const int u_end = u0 + seg;
+    fetch_ids(u0);
+    load(u0);
+    store(0, whole_of(u0));
+    if (seg > 1) load(u0 + 1);
+    turn();
+    // Buffer of unit u: (u - u0) % kWideBufs, kept as three rotating indices.
+    int b_prev = 2, b_cur = 0, b_next = 1;
+    const bool behind = wave >= kWideWaves / 2;
+    if (behind) {
+      if (seg > 1) {
+        store(1, whole_of(u0 + 1));
+        if (seg > 2) load(u0 + 2);
+      }
+      turn();
     }
+    for (int u = u0; u < u_end; ++u) {
+      if (live) {
+        if (u > u0)
+          products(std::true_type{}, std::true_type{}, b_cur, b_prev);
+        else
+          products(std::true_type{}, std::false_type{}, b_cur, b_prev);
+        if (u > u0 && !whole_of(u - 1)) add_odd(b_prev, u - 1);
+      }
+      turn();
+      if (live) softmax(u);
+      // Waves 0-3 store unit u + 1, waves 4-7 (half a stage later) u + 2, into
+      // the buffer of unit u - 2 or u - 1, whose last reads are two turns old.
+      const int us = behind ? u + 2 : u + 1;
+      if (us < u_end) {
+        store(behind ? b_prev : b_next, whole_of(us));
+        if (us + 1 < u_end) load(us + 1);
+      }
+      turn();
+      const int b = b_prev;
+      b_prev = b_cur;
+      b_cur = b_next;
+      b_next = b;
+    }
+    if (live) {
+      products(std::false_type{}, std::true_type{}, 0, b_prev);
+      if (!whole_of(u_end - 1)) add_odd(b_prev, u_end - 1);
+    }
+    if (!behind) turn();
 
     // Lane holds O^T rows d = 32 db + 8 (i/4) + 4 half + i%4 of its row.
     const float lsum = l + __shfl_xor(l, 32, 64);
