@@ -157,11 +157,18 @@ __device__ __forceinline__ float inverse_sum(float L) { return L == 0.f ? 0.f : 
 __device__ __forceinline__ float state_lse(float M, float L) {
   return (M + __builtin_amdgcn_logf(L)) * kLn2;
 }
-// N consecutive values of a row, N a multiple of 4.
+// N consecutive values of a row, N 2 or a multiple of 4.
 template <typename T, int N>
 __device__ __forceinline__ void write_row(T* dst, const float* v, float inv) {
+  if constexpr (N == 2) {
+    if constexpr (sizeof(T) == 2)
+      *reinterpret_cast<uint32_t*>(dst) = Packet<T>::pack2(v[0] * inv, v[1] * inv);
+    else
+      *reinterpret_cast<float2*>(dst) = make_float2(v[0] * inv, v[1] * inv);
+    return;
+  }
 #pragma unroll
-  for (int i = 0; i < N; i += 4) {
+  for (int i = 0; i + 3 < N; i += 4) {
     if constexpr (sizeof(T) == 2)
       *reinterpret_cast<uint2*>(dst + i) = make_uint2(Packet<T>::pack2(v[i] * inv, v[i + 1] * inv),
                                                       Packet<T>::pack2(v[i + 2] * inv, v[i + 3] * inv));
@@ -188,8 +195,6 @@ __device__ __forceinline__ RowSpan row_span(int off, int t, int window) {
 // ---------------------------------------------------------------------------
 // Thin sequences
 // ---------------------------------------------------------------------------
-constexpr int kThinWaves = 4;
-constexpr int kThinThreads = 64 * kThinWaves;
 
 // A page of K and V in registers. 16-bit: K in the A-operand layout of
 // 16x16x32 products (lane l: key l % 16, elements 32 r + 8 (l / 16) .. +8 in
@@ -204,32 +209,32 @@ struct PageRegs {
 
 // V rows of a wave's page in LDS, padded: 16-bit rows by 16 elements (the
 // four rows of a transposing read on banks of their own), f32 rows by 4.
-template <typename T, int D>
+template <typename T, int D, int W>
 struct ThinLds {
   static constexpr int kPad = sizeof(T) == 2 ? 16 : 4;
-  T v[kThinWaves][16][D + kPad];
+  T v[W][16][D + kPad];
 };
 
-template <typename T, int D, int RT>
-__global__ __launch_bounds__(kThinThreads, sizeof(T) == 4 && RT == 2 ? 1 : 2) void chunk_thin_kernel(ChunkParams p) {
+template <typename T, int D, int RT, int W>
+__global__ __launch_bounds__(64 * W, 8 / W) void chunk_thin_kernel(ChunkParams p) {
   constexpr int N = PageRegs<T, D>::N;
   constexpr int ES = (int)sizeof(T), PPR = D * ES / 16;  // packets per row
   constexpr int DT = D / 16;
-  constexpr int NBUF = sizeof(T) == 2 && RT == 1 ? 3 : 2;
+  // Pages in registers: one at work, the others in flight (as many as fit).
+  constexpr int NBUF = ES == 2 ? (RT == 1 ? 3 : 2) : D == 128 && RT == 2 ? 1 : 2;
   constexpr int kExRow = D + 4;
-  __shared__ __align__(16) ThinLds<T, D> s;
-  __shared__ __align__(16) float s_ex[kThinWaves][16][kExRow];
-  __shared__ float s_ml[kThinWaves][16][2];
+  __shared__ __align__(16) ThinLds<T, D, W> s;
+  __shared__ __align__(16) float s_ex[W][16][kExRow];
+  __shared__ float s_ml[W][16][2];
   __shared__ int s_last;
 
   if (p.v.head->stamp != p.stamp) {
     if (blockIdx.x == 0 && threadIdx.x == 0) ws_raise(&p.v.head->flags, RLSE_WS_ERR_PLAN);
     return;
   }
-  const int groups = p.v.head->thin_groups, tiles = p.v.head->thin_tiles;
-  if ((int)blockIdx.x >= groups) return;
-  const int w = share_index(blockIdx.x, groups);
-  const ChunkShare share = p.v.thin_share[w];
+  const int tiles = p.v.head->thin_tiles;
+  const ChunkShare share = p.v.thin_share[blockIdx.x];
+  const int w = __builtin_amdgcn_readfirstlane(share.w);
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -241,44 +246,46 @@ __global__ __launch_bounds__(kThinThreads, sizeof(T) == 4 && RT == 2 ? 1 : 2) vo
   const T* __restrict__ vp = static_cast<const T*>(p.v_pool);
 
   int ti = __builtin_amdgcn_readfirstlane(share.tile);
-  int h = __builtin_amdgcn_readfirstlane(share.head);
-  int u0 = __builtin_amdgcn_readfirstlane(share.u0);
   int left = __builtin_amdgcn_readfirstlane(share.count);
-  bool head_piece = u0 > 0;
-  while (left > 0) {
-    const ChunkTile t = p.v.thin[ti];
-    const int n = __builtin_amdgcn_readfirstlane(t.n), off = __builtin_amdgcn_readfirstlane(t.off);
-    const int tok0 = __builtin_amdgcn_readfirstlane(t.tok0);
-    const int wp0 = __builtin_amdgcn_readfirstlane(t.wp0);
-    const int pages = __builtin_amdgcn_readfirstlane(t.pages);
-    const int* __restrict__ table =
-        p.tables + (size_t)__builtin_amdgcn_readfirstlane(t.seq) * p.mbps;
-    const int seg = min(left, pages - u0);
-    const int rows = n * G;
-    const int kend = off + n;
+  if (left == 0) return;
+  bool head_piece = share.u0 > 0;
 
-    // This wave's pages: virtual pages u0 + wave, + kThinWaves, ...
-    const int np = (seg - wave + kThinWaves - 1) / kThinWaves;
-    int ids = -1, pgs = 0, ids_at = 0;
-    auto fetch_ids = [&](int from) __attribute__((always_inline)) {
-      const int i = from + lane;
-      ids = -1;
-      pgs = 0;
-      if (i < np) {
-        pgs = real_page(u0 + wave + i * kThinWaves, wp0, sink_pages);
-        const int id = table[pgs];
-        ids = (unsigned)id < (unsigned)p.num_blocks ? id : -1;
-      }
-      ids_at = from;
-    };
+  // The piece at work: units u0 .. u0 + seg - 1 of tile t for KV head h. This
+  // wave's pages are virtual pages u0 + wave, + W, ..., np of them;
+  // ids and pgs hold 64 of their ids and table places, one a lane.
+  int h, u0, n, off, tok0, wp0, pages, seg, np;
+  const int* __restrict__ table;
+  int ids, pgs, ids_at;
+  uint4 q[RT][N];
+  RowSpan span[RT];
+  auto fetch_ids = [&](int from) __attribute__((always_inline)) {
+    const int i = from + lane;
+    ids = -1;
+    pgs = 0;
+    if (i < np) {
+      pgs = real_page(u0 + wave + i * W, wp0, sink_pages);
+      const int id = table[pgs];
+      ids = (unsigned)id < (unsigned)p.num_blocks ? id : -1;
+    }
+    ids_at = from;
+  };
+  // Requests the page ids and queries of a piece.
+  auto open = [&](const ChunkTile& t, int head, int first) __attribute__((always_inline)) {
+    h = head;
+    u0 = first;
+    n = __builtin_amdgcn_readfirstlane(t.n);
+    off = __builtin_amdgcn_readfirstlane(t.off);
+    tok0 = __builtin_amdgcn_readfirstlane(t.tok0);
+    wp0 = __builtin_amdgcn_readfirstlane(t.wp0);
+    pages = __builtin_amdgcn_readfirstlane(t.pages);
+    table = p.tables + (size_t)__builtin_amdgcn_readfirstlane(t.seq) * p.mbps;
+    seg = min(left, pages - u0);
+    np = (seg - wave + W - 1) / W;
     fetch_ids(0);
-
-    uint4 q[RT][N];
-    RowSpan span[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       const int row = rt * 16 + col;
-      const bool real = row < rows;
+      const bool real = row < n * G;
       const int tok = real ? row / G : 0, g = real ? row - tok * G : 0;
       span[rt] = row_span(off, tok, p.window);
       const T* src = qb + ((size_t)(tok0 + tok) * Hq + h * G + g) * D + quad * (16 / ES);
@@ -287,6 +294,15 @@ __global__ __launch_bounds__(kThinThreads, sizeof(T) == 4 && RT == 2 ? 1 : 2) vo
         q[rt][r] = real ? *reinterpret_cast<const uint4*>(src + r * (64 / ES))
                         : make_uint4(0, 0, 0, 0);
     }
+  };
+  open(share.start, __builtin_amdgcn_readfirstlane(share.head),
+       __builtin_amdgcn_readfirstlane(share.u0));
+
+  while (true) {
+    const int kend = off + n;
+    // The next tile's record, in flight during this one.
+    const int tn = ti + 1 == tiles ? 0 : ti + 1;
+    const ChunkTile tile_next = p.v.thin[tn];
 
     f32x4_t o[RT][DT];
     float m[RT], l[RT];
@@ -450,20 +466,25 @@ __global__ __launch_bounds__(kThinThreads, sizeof(T) == 4 && RT == 2 ? 1 : 2) vo
       }
     }
 
-    // The waves' states meet in LDS, 16 rows at a time. Thread tid finishes
-    // row tid / 16, its dimensions (tid % 16) * D / 16 ...
+    // The waves' states meet in LDS, 16 rows at a time, TPR threads a
+    // row, DPT dimensions each.
     const bool cut = seg < pages;
+    const int rows = n * G, tok_at = tok0, head = h;
+    left -= seg;
+    ti = tn;
+    if (left > 0) open(tile_next, tn == 0 ? h + 1 : h, 0);  // on its way during the join
     float* part = nullptr;
     if (cut)
       part = p.thin_part + (size_t)(2 * w + (head_piece ? 0 : 1)) * kThinRows * (D + 2);
-    const int er = tid >> 4, ed = (tid & 15) * DT;
+    constexpr int TPR = 4 * W, DPT = D / TPR;
+    const int er = tid / TPR, ed = tid % TPR * DPT;
     auto finish = [&](int row, float M, float L, const float* acc)
                       __attribute__((always_inline)) {
       if (row >= rows) return;
       const int tok = row / G;
-      const size_t at = (size_t)(tok0 + tok) * Hq + h * G + row - tok * G;
-      write_row<T, DT>(static_cast<T*>(p.out) + at * D + ed, acc, inverse_sum(L));
-      if (p.lse && (tid & 15) == 0) p.lse[at] = state_lse(M, L);
+      const size_t at = (size_t)(tok_at + tok) * Hq + head * G + row - tok * G;
+      write_row<T, DPT>(static_cast<T*>(p.out) + at * D + ed, acc, inverse_sum(L));
+      if (p.lse && tid % TPR == 0) p.lse[at] = state_lse(M, L);
     };
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -479,17 +500,17 @@ __global__ __launch_bounds__(kThinThreads, sizeof(T) == 4 && RT == 2 ? 1 : 2) vo
       for (int d = 0; d < DT; ++d)
         *reinterpret_cast<f32x4_t*>(&s_ex[wave][col][16 * d + quad * 4]) = o[rt][d];
       __syncthreads();
-      float M = -INFINITY, L = 0.f, acc[DT];
+      float M = -INFINITY, L = 0.f, acc[DPT];
 #pragma unroll
-      for (int i = 0; i < DT; ++i) acc[i] = 0.f;
+      for (int i = 0; i < DPT; ++i) acc[i] = 0.f;
 #pragma unroll
-      for (int k = 0; k < kThinWaves; ++k) M = fmaxf(M, s_ml[k][er][0]);
+      for (int k = 0; k < W; ++k) M = fmaxf(M, s_ml[k][er][0]);
 #pragma unroll
-      for (int k = 0; k < kThinWaves; ++k) {
+      for (int k = 0; k < W; ++k) {
         const float a = state_weight(s_ml[k][er][0], M);
         L += s_ml[k][er][1] * a;
 #pragma unroll
-        for (int i = 0; i < DT; ++i) acc[i] += s_ex[k][er][ed + i] * a;
+        for (int i = 0; i < DPT; ++i) acc[i] += s_ex[k][er][ed + i] * a;
       }
       const int row = rt * 16 + er;
       if (!cut) {
@@ -497,8 +518,8 @@ __global__ __launch_bounds__(kThinThreads, sizeof(T) == 4 && RT == 2 ? 1 : 2) vo
       } else {
         float* dst = part + row * (D + 2);
 #pragma unroll
-        for (int i = 0; i < DT; i += 2) st_pair(dst + ed + i, acc[i], acc[i + 1]);
-        if ((tid & 15) == 0) st_pair(dst + D, M, L);
+        for (int i = 0; i < DPT; i += 2) st_pair(dst + ed + i, acc[i], acc[i + 1]);
+        if (tid % TPR == 0) st_pair(dst + D, M, L);
       }
     }
 
@@ -507,7 +528,7 @@ __global__ __launch_bounds__(kThinThreads, sizeof(T) == 4 && RT == 2 ? 1 : 2) vo
       // result does not depend on who does). Piece stores are agent scope and
       // waited for before the count rises, so no cache holds an older copy.
       const int first = head_piece ? share.first : w;
-      const int npieces = p.v.thin_share[first].last - first + 1;
+      const int npieces = head_piece ? share.pieces : share.last - w + 1;
       wait_vm_stores();
       __syncthreads();
       if (tid == 0)
@@ -519,34 +540,29 @@ __global__ __launch_bounds__(kThinThreads, sizeof(T) == 4 && RT == 2 ? 1 : 2) vo
         for (int r0 = 0; r0 < rows; r0 += 16) {
           const int row = r0 + er;
           if (row >= rows) break;
-          float M = -INFINITY, L = 0.f, acc[DT];
+          float M = -INFINITY, L = 0.f, acc[DPT];
 #pragma unroll
-          for (int i = 0; i < DT; ++i) acc[i] = 0.f;
+          for (int i = 0; i < DPT; ++i) acc[i] = 0.f;
           for (int k = 0; k < npieces; ++k) {
             const float* src = p.thin_part + (size_t)(2 * (first + k) + (k == 0 ? 1 : 0)) *
                                                  kThinRows * (D + 2) + row * (D + 2);
-            float ml[2], a[DT];
+            float ml[2], a[DPT];
             ld_pair(src + D, ml);
 #pragma unroll
-            for (int i = 0; i < DT; i += 2) ld_pair(src + ed + i, a + i);
+            for (int i = 0; i < DPT; i += 2) ld_pair(src + ed + i, a + i);
             const float mn = fmaxf(M, ml[0]);
             const float sa = state_weight(M, mn), sb = state_weight(ml[0], mn);
             L = L * sa + ml[1] * sb;
 #pragma unroll
-            for (int i = 0; i < DT; ++i) acc[i] = acc[i] * sa + a[i] * sb;
+            for (int i = 0; i < DPT; ++i) acc[i] = acc[i] * sa + a[i] * sb;
             M = mn;
           }
           finish(row, M, L, acc);
         }
       }
     }
-    left -= seg;
-    u0 = 0;
+    if (left == 0) break;
     head_piece = false;
-    if (++ti == tiles) {
-      ti = 0;
-      ++h;
-    }
   }
 }
 
@@ -627,10 +643,9 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
     if (blockIdx.x == 0 && threadIdx.x == 0) ws_raise(&p.v.head->flags, RLSE_WS_ERR_PLAN);
     return;
   }
-  const int groups = p.v.head->wide_groups, tiles = p.v.head->wide_tiles;
-  if ((int)blockIdx.x >= groups) return;
-  const int w = share_index(blockIdx.x, groups);
-  const ChunkShare share = p.v.wide_share[w];
+  const int tiles = p.v.head->wide_tiles;
+  const ChunkShare share = p.v.wide_share[blockIdx.x];
+  const int w = __builtin_amdgcn_readfirstlane(share.w);
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -658,8 +673,8 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
   int u0 = __builtin_amdgcn_readfirstlane(share.u0);
   int left = __builtin_amdgcn_readfirstlane(share.count);
   bool head_piece = u0 > 0;
+  ChunkTile t = share.start;
   while (left > 0) {
-    const ChunkTile t = p.v.wide[ti];
     const int n = __builtin_amdgcn_readfirstlane(t.n), off = __builtin_amdgcn_readfirstlane(t.off);
     const int tok0 = __builtin_amdgcn_readfirstlane(t.tok0);
     const int row0 = __builtin_amdgcn_readfirstlane(t.row0);
@@ -979,6 +994,7 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
       ti = 0;
       ++h;
     }
+    if (left > 0) t = p.v.wide[ti];
   }
 }
 
@@ -1014,10 +1030,9 @@ __global__ __launch_bounds__(kWide32Threads, 1) void chunk_wide32_kernel(ChunkPa
     if (blockIdx.x == 0 && threadIdx.x == 0) ws_raise(&p.v.head->flags, RLSE_WS_ERR_PLAN);
     return;
   }
-  const int groups = p.v.head->wide_groups, tiles = p.v.head->wide_tiles;
-  if ((int)blockIdx.x >= groups) return;
-  const int w = share_index(blockIdx.x, groups);
-  const ChunkShare share = p.v.wide_share[w];
+  const int tiles = p.v.head->wide_tiles;
+  const ChunkShare share = p.v.wide_share[blockIdx.x];
+  const int w = __builtin_amdgcn_readfirstlane(share.w);
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -1040,8 +1055,8 @@ __global__ __launch_bounds__(kWide32Threads, 1) void chunk_wide32_kernel(ChunkPa
   int u0 = __builtin_amdgcn_readfirstlane(share.u0);
   int left = __builtin_amdgcn_readfirstlane(share.count);
   bool head_piece = u0 > 0;
+  ChunkTile t = share.start;
   while (left > 0) {
-    const ChunkTile t = p.v.wide[ti];
     const int n = __builtin_amdgcn_readfirstlane(t.n), off = __builtin_amdgcn_readfirstlane(t.off);
     const int tok0 = __builtin_amdgcn_readfirstlane(t.tok0);
     const int row0 = __builtin_amdgcn_readfirstlane(t.row0);
@@ -1277,6 +1292,7 @@ __global__ __launch_bounds__(kWide32Threads, 1) void chunk_wide32_kernel(ChunkPa
       ti = 0;
       ++h;
     }
+    if (left > 0) t = p.v.wide[ti];
   }
 }
 
@@ -1287,11 +1303,9 @@ template <typename T, int D>
 __global__ __launch_bounds__(kPartLanes) void chunk_merge_kernel(ChunkParams p) {
   constexpr int DB = D / 32;
   if (p.v.head->stamp != p.stamp) return;
-  const int w = blockIdx.x / DB, d = blockIdx.x % DB;
-  const int groups = p.v.head->wide_groups;
-  if (w >= groups) return;
-  const ChunkShare share = p.v.wide_share[w];
-  if (share.last == w) return;
+  const ChunkShare share = p.v.wide_share[blockIdx.x / DB];
+  const int w = share.w, d = blockIdx.x % DB;
+  if (share.count == 0 || share.last == w) return;
   const ChunkTile t = p.v.wide[share.end_tile];
   const int h = share.end_head;
   const int tid = threadIdx.x;
@@ -1346,14 +1360,23 @@ ChunkWorkspace chunk_workspace(int max_rows, int D, int cus) {
 }
 
 template <typename T, int D>
-int launch_chunk(const ChunkParams& p, int max_rows, int thin_rows, int cus, hipStream_t stream) {
+int launch_chunk(const ChunkParams& p, int max_rows, int thin_rows, int waves, int cus,
+                 hipStream_t stream) {
   int st = RLSE_OK;
   if (thin_rows > 0) {
-    const dim3 grid(2 * cus), block(kThinThreads);
-    if (max_rows <= 16)
-      hipLaunchKernelGGL((chunk_thin_kernel<T, D, 1>), grid, block, 0, stream, p);
+    auto run = [&](auto rt, auto waves) {
+      constexpr int RT = decltype(rt)::value, W = decltype(waves)::value;
+      hipLaunchKernelGGL((chunk_thin_kernel<T, D, RT, W>), dim3(thin_groups(cus, W)), dim3(64 * W),
+                         0, stream, p);
+    };
+    const std::integral_constant<int, 1> one;
+    const std::integral_constant<int, 2> two;
+    const std::integral_constant<int, 4> four;
+    const std::integral_constant<int, 8> eight;
+    if (waves == 8)
+      max_rows <= 16 ? run(one, eight) : run(two, eight);
     else
-      hipLaunchKernelGGL((chunk_thin_kernel<T, D, 2>), grid, block, 0, stream, p);
+      max_rows <= 16 ? run(one, four) : run(two, four);
     st = launch_status("chunk_thin_kernel");
   }
   if (st || max_rows <= thin_rows) return st;
@@ -1449,7 +1472,8 @@ extern "C" int rlse_chunk_attn(const void* q, const void* k_pool, const void* v_
   auto run = [&](auto t, auto d) {
     using T = decltype(t);
     constexpr int D = decltype(d)::value;
-    return launch_chunk<T, D>(p, max_rows, thin_row_limit(num_seqs, max_rows), cus, s);
+    return launch_chunk<T, D>(p, max_rows, thin_row_limit(num_seqs, max_rows),
+                              thin_waves(num_seqs, num_kv_heads, cus), cus, s);
   };
   const std::integral_constant<int, 64> d64;
   const std::integral_constant<int, 128> d128;

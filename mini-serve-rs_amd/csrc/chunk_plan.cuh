@@ -31,6 +31,11 @@ constexpr int kScorePages = 16;     // pages per unit of the wide key-weight lau
 constexpr int kMaxChunkSeqs = 4096; // prefix tables of the plan launch live in LDS
 constexpr int kThinMinUnits = 8;    // smallest share of a workgroup: pages,
 constexpr int kWideMinUnits = 4;    //   and wide units
+// How far a share's boundary moves to a tile's rather than cut it: a cut costs
+// a thin workgroup about what it streams in the time of 16 pages, a wide one
+// about a unit.
+constexpr int kThinSnap = 16;
+constexpr int kWideSnap = 1;
 
 // Rows of a thin sequence at most in a step of num_seqs sequences of up to
 // max_rows rows. A single sequence that may be wide is taken as wide whatever
@@ -38,6 +43,14 @@ constexpr int kWideMinUnits = 4;    //   and wide units
 __host__ __device__ inline int thin_row_limit(int num_seqs, int max_rows) {
   return num_seqs == 1 && max_rows > kThinRows ? 0 : kThinRows;
 }
+
+// Waves of a thin workgroup, and how many workgroups share the step: eight a
+// compute unit either way. In one workgroup of 8 the waves of a tile meet in
+// LDS; with many tiles two of 4 cover each other's joins.
+__host__ __device__ inline int thin_waves(int num_seqs, int Hkv, int cus) {
+  return (long long)num_seqs * Hkv <= 2LL * cus ? 8 : 4;
+}
+__host__ __device__ inline int thin_groups(int cus, int waves) { return cus * (8 / waves); }
 
 struct ChunkTile {
   int unit0;     // units of this list's tiles before it (of one KV head)
@@ -50,20 +63,25 @@ struct ChunkTile {
   int pages;     // virtual pages
 };
 
-// A workgroup's share of a list: units u0 .. of (head, tile), count in all,
-// going on through the following tiles. first: the workgroup that holds the
-// start of that first tile. The share ends in (end_head, end_tile), whose end
-// workgroup `last` holds: w itself, too, where the tile started before the
-// share (another workgroup then joins its pieces).
+// A workgroup's share of a list, number w: units u0 .. of (head, tile), count
+// in all (0: none), going on through the following tiles. The tile it starts
+// in is copied here, so that a workgroup's first loads all go out together.
+// first: the share that holds that tile's start, pieces: how many shares hold
+// some of it. The share ends in (end_head, end_tile), whose end share `last`
+// holds: w itself, too, where that tile started before the share (another
+// workgroup then joins its pieces).
 struct ChunkShare {
-  int tile, head, u0, count, first, last, end_tile, end_head;
+  int w, head, u0, count, first, pieces, last, tile;
+  ChunkTile start;
+  int end_tile, end_head, pad[14];
 };
+static_assert(sizeof(ChunkShare) == 128, "a share is a cache line");
 
 struct ChunkHead {
   uint32_t flags;  // RLSE_WS_ERR_* of this step
   uint32_t stamp;  // chunk_stamp of the call that built the plan
-  int thin_tiles, thin_units, thin_groups;
-  int wide_tiles, wide_units, wide_groups;
+  int thin_tiles, thin_units;
+  int wide_tiles, wide_units;
   int score_seqs, score_units;  // wide sequences, and their key blocks
 };
 constexpr int kChunkHeadBytes = 256;
@@ -87,7 +105,7 @@ struct ChunkPlanView {
   ChunkTile* thin;    // [num_seqs]
   ChunkTile* score;   // [num_seqs]: wide sequences, all their rows
   ChunkTile* wide;    // [wide_cap]
-  ChunkShare* thin_share;  // [2 * cus]
+  ChunkShare* thin_share;  // [2 * cus], by workgroup
   ChunkShare* wide_share;  // [cus]
 };
 __host__ __device__ inline long long wide_tile_cap(long long total_tokens, int G, int num_seqs) {
@@ -95,19 +113,19 @@ __host__ __device__ inline long long wide_tile_cap(long long total_tokens, int G
 }
 __host__ __device__ inline size_t chunk_plan_bytes(int num_seqs, int total_tokens, int G, int cus) {
   return kChunkHeadBytes +
-         sizeof(ChunkTile) * (size_t)(2LL * num_seqs + wide_tile_cap(total_tokens, G, num_seqs)) +
-         sizeof(ChunkShare) * (size_t)(3 * cus);
+         sizeof(ChunkShare) * (size_t)(3 * cus) +
+         sizeof(ChunkTile) * (size_t)(2LL * num_seqs + wide_tile_cap(total_tokens, G, num_seqs));
 }
 __host__ __device__ inline ChunkPlanView chunk_plan_view(void* plan, int num_seqs,
                                                          int total_tokens, int G, int cus) {
   ChunkPlanView v;
   char* p = static_cast<char*>(plan);
   v.head = reinterpret_cast<ChunkHead*>(p);
-  v.thin = reinterpret_cast<ChunkTile*>(p + kChunkHeadBytes);
+  v.thin_share = reinterpret_cast<ChunkShare*>(p + kChunkHeadBytes);
+  v.wide_share = v.thin_share + 2 * cus;
+  v.thin = reinterpret_cast<ChunkTile*>(v.wide_share + cus);
   v.score = v.thin + num_seqs;
   v.wide = v.score + num_seqs;
-  v.thin_share = reinterpret_cast<ChunkShare*>(v.wide + wide_tile_cap(total_tokens, G, num_seqs));
-  v.wide_share = v.thin_share + 2 * cus;
   return v;
 }
 

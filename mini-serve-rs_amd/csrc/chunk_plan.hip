@@ -17,7 +17,7 @@ struct PlanParams {
   const int* cu;
   const int* lens;
   int num_seqs, total_tokens, max_tokens, G, Hkv, mbps, window, sinks, cus;
-  int thin_rows;
+  int thin_rows, thin_groups;
   uint32_t stamp;
   ChunkPlanView v;
   int wide_cap;
@@ -59,39 +59,84 @@ __device__ __forceinline__ int tile_of(const int* held, const ChunkTile* a, int 
 }
 
 // Shares of `units` units of each of Hkv heads over at most max_groups
-// workgroups of at least min_units each.
-__device__ int deal(const int* held, const ChunkTile* tiles, int n, int units, int Hkv,
-                    int max_groups, int min_units, ChunkShare* out) {
-  const long long total = (long long)units * Hkv;
-  if (total == 0) return 0;
-  const long long want = (total + min_units - 1) / min_units;
-  const int groups = (int)(want < max_groups ? want : max_groups);
+// workgroups of at least min_units each. Equal shares, but a boundary within
+// snap units of a tile's moves there: a tile cut for the sake of a few units
+// costs more than they do. I: an integer type that holds units * Hkv *
+// max_groups; starts: max_groups + 1 of them in LDS.
+constexpr int kMaxShares = 1024;
+template <typename I>
+__device__ void deal(const int* held, const ChunkTile* tiles, int n, int units, int Hkv,
+                     int max_groups, int min_units, int snap, I* starts, ChunkShare* out) {
+  const I total = (I)units * Hkv;
+  const I want = (total + min_units - 1) / min_units;
+  const int groups = (int)(want < (I)max_groups ? want : (I)max_groups);
   auto unit0 = [&](int i) { return i < n ? (i < kHeld ? held[i] : tiles[i].unit0) : units; };
-  for (int w = threadIdx.x; w < groups; w += kPlanThreads) {
-    const long long a = total * w / groups, b = total * (w + 1) / groups;
-    // The workgroup holding unit x is the largest w' with w' * total / groups <= x.
-    auto holder = [&](long long x) { return (int)(((x + 1) * groups - 1) / total); };
-    ChunkShare s;
-    s.head = (int)(a / units);
-    const int u = (int)(a - (long long)s.head * units);
-    s.tile = tile_of(held, tiles, n, u);
-    s.u0 = u - unit0(s.tile);
-    s.count = (int)(b - a);
-    s.first = s.u0 ? holder(a - s.u0) : w;
-    s.end_head = (int)((b - 1) / units);
-    const long long base = (long long)s.end_head * units;
-    s.end_tile = tile_of(held, tiles, n, (int)(b - 1 - base));
-    const long long end = base + unit0(s.end_tile + 1);
-    s.last = end > b && base + unit0(s.end_tile) >= a ? holder(end - 1) : w;
-    out[w] = s;
+  snap = min((I)snap, total / (4 * groups));
+  for (int w = threadIdx.x; w <= groups; w += kPlanThreads) {
+    I x = total * w / groups;
+    if (w > 0 && w < groups) {
+      const int head = (int)(x / units), u = (int)(x - (I)head * units);
+      const int i = tile_of(held, tiles, n, u), lo = unit0(i), hi = unit0(i + 1);
+      if (u - lo <= snap)
+        x -= u - lo;
+      else if (hi - u <= snap)
+        x += hi - u;
+    }
+    starts[w] = x;
   }
-  return groups;
+  __syncthreads();
+  for (int b = threadIdx.x; b < max_groups; b += kPlanThreads) {
+    if (b >= groups) {
+      out[b].count = 0;
+      continue;
+    }
+    ChunkShare s;
+    s.w = share_index(b, groups);
+    const I from = starts[s.w], to = starts[s.w + 1];
+    auto holder = [&](I x) {  // the share that has unit x
+      int w = (int)(x * groups / total);
+      while (starts[w] > x) --w;
+      while (starts[w + 1] <= x) ++w;
+      return w;
+    };
+    s.head = (int)(from / units);
+    const int u = (int)(from - (I)s.head * units);
+    s.tile = tile_of(held, tiles, n, u);
+    s.start = tiles[s.tile];
+    s.u0 = u - unit0(s.tile);
+    s.count = (int)(to - from);
+    s.first = s.u0 ? holder(from - s.u0) : s.w;
+    const I tile_end = from - s.u0 + (unit0(s.tile + 1) - unit0(s.tile));
+    s.pieces = (tile_end > to ? holder(tile_end - 1) : s.w) - s.first + 1;
+    s.end_head = (int)((to - 1) / units);
+    const I base = (I)s.end_head * units;
+    s.end_tile = tile_of(held, tiles, n, (int)(to - 1 - base));
+    const I end = base + unit0(s.end_tile + 1);
+    s.last = end > to && base + unit0(s.end_tile) >= from ? holder(end - 1) : s.w;
+    out[b] = s;
+  }
+  __syncthreads();
+}
+__device__ void deal_shares(const int* held, const ChunkTile* tiles, int n, int units, int Hkv,
+                            int max_groups, int min_units, int snap, unsigned long long* starts,
+                            ChunkShare* out) {
+  if (units == 0) {
+    for (int b = threadIdx.x; b < max_groups; b += kPlanThreads) out[b].count = 0;
+    return;
+  }
+  // (64-bit divisions take a few microseconds here.)
+  if ((unsigned long long)units * Hkv * max_groups < (1ull << 31))
+    deal<unsigned>(held, tiles, n, units, Hkv, max_groups, min_units, snap,
+                   reinterpret_cast<unsigned*>(starts), out);
+  else
+    deal<unsigned long long>(held, tiles, n, units, Hkv, max_groups, min_units, snap, starts, out);
 }
 
 __global__ __launch_bounds__(kPlanThreads) void chunk_plan_kernel(PlanParams p) {
   __shared__ int s_wide[kMaxChunkSeqs + 1];  // wide tiles before each sequence
   __shared__ int s_w[kPlanWaves];
   __shared__ int s_thin[kHeld], s_unit[kHeld];  // unit0 of the thin and the wide tiles
+  __shared__ unsigned long long s_starts[kMaxShares + 1];
   __shared__ unsigned s_flags;
   const int tid = threadIdx.x;
   if (tid == 0) s_flags = 0;
@@ -178,20 +223,18 @@ __global__ __launch_bounds__(kPlanThreads) void chunk_plan_kernel(PlanParams p) 
   }
   __syncthreads();
 
-  const int tg = deal(s_thin, p.v.thin, thin_tiles, thin_units, p.Hkv, 2 * p.cus, kThinMinUnits,
-                      p.v.thin_share);
-  const int wg = deal(s_unit, p.v.wide, wide_tiles, wide_units, p.Hkv, p.cus, kWideMinUnits,
-                      p.v.wide_share);
+  deal_shares(s_thin, p.v.thin, thin_tiles, thin_units, p.Hkv, p.thin_groups, kThinMinUnits,
+              kThinSnap, s_starts, p.v.thin_share);
+  deal_shares(s_unit, p.v.wide, wide_tiles, wide_units, p.Hkv, p.cus, kWideMinUnits, kWideSnap,
+              s_starts, p.v.wide_share);
   if (tid == 0) {
     ChunkHead h;
     h.flags = s_flags;
     h.stamp = p.stamp;
     h.thin_tiles = thin_tiles;
     h.thin_units = thin_units;
-    h.thin_groups = tg;
     h.wide_tiles = wide_tiles;
     h.wide_units = wide_units;
-    h.wide_groups = wg;
     h.score_seqs = score_seqs;
     h.score_units = score_units;
     *p.v.head = h;
@@ -266,6 +309,9 @@ extern "C" int rlse_chunk_plan(const int32_t* cu_tokens, const int32_t* seq_lens
   p.max_tokens = max_tokens;
   p.Hkv = num_kv_heads;
   p.thin_rows = thin_row_limit(num_seqs, max_tokens * p.G);
+  p.thin_groups = thin_groups(p.cus, thin_waves(num_seqs, num_kv_heads, p.cus));
+  if (p.thin_groups > kMaxShares)
+    return fail(RLSE_ERR_INVALID_VALUE, "chunk_plan: %d compute units", p.cus);
   p.mbps = max_blocks_per_seq;
   p.window = window;
   p.sinks = sinks;

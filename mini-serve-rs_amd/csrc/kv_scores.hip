@@ -105,20 +105,17 @@ __device__ __forceinline__ void write_score(const ScoreParams& p, size_t row, in
   if (k < kend) p.scores[row + k] = w + (p.prev && k < off ? p.prev[row + k] : 0.f);
 }
 
-constexpr int kThinWaves = 4;
-constexpr int kThinThreads = 64 * kThinWaves;
 
-template <typename T, int D, int RT>
-__global__ __launch_bounds__(kThinThreads) void score_thin_kernel(ScoreParams p) {
+template <typename T, int D, int RT, int W>
+__global__ __launch_bounds__(64 * W) void score_thin_kernel(ScoreParams p) {
   constexpr int ES = (int)sizeof(T), N = D * ES / 64;
   constexpr int NBUF = 4;
   if (p.v.head->stamp != p.stamp) {
     if (blockIdx.x == 0 && threadIdx.x == 0) ws_raise(&p.v.head->flags, RLSE_WS_ERR_PLAN);
     return;
   }
-  const int groups = p.v.head->thin_groups, tiles = p.v.head->thin_tiles;
-  if ((int)blockIdx.x >= groups) return;
-  const ChunkShare share = p.v.thin_share[share_index(blockIdx.x, groups)];
+  const int tiles = p.v.head->thin_tiles;
+  const ChunkShare share = p.v.thin_share[blockIdx.x];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int col = lane & 15, quad = lane >> 4;
   const int Hq = p.Hq, Hkv = p.Hkv, G = p.G;
@@ -130,8 +127,8 @@ __global__ __launch_bounds__(kThinThreads) void score_thin_kernel(ScoreParams p)
   int h = __builtin_amdgcn_readfirstlane(share.head);
   int u0 = __builtin_amdgcn_readfirstlane(share.u0);
   int left = __builtin_amdgcn_readfirstlane(share.count);
+  ChunkTile t = share.start;
   while (left > 0) {
-    const ChunkTile t = p.v.thin[ti];
     const int n = __builtin_amdgcn_readfirstlane(t.n), off = __builtin_amdgcn_readfirstlane(t.off);
     const int tok0 = __builtin_amdgcn_readfirstlane(t.tok0);
     const int wp0 = __builtin_amdgcn_readfirstlane(t.wp0);
@@ -141,7 +138,7 @@ __global__ __launch_bounds__(kThinThreads) void score_thin_kernel(ScoreParams p)
     const size_t out = ((size_t)seq * Hkv + h) * p.mbps * 16;
     const int seg = min(left, pages - u0);
     const int rows = n * G, kend = off + n;
-    const int np = (seg - wave + kThinWaves - 1) / kThinWaves;  // this wave's pages
+    const int np = (seg - wave + W - 1) / W;  // this wave's pages
 
     int ids = -1, pgs = 0, ids_at = 0;
     auto fetch_ids = [&](int from) __attribute__((always_inline)) {
@@ -149,7 +146,7 @@ __global__ __launch_bounds__(kThinThreads) void score_thin_kernel(ScoreParams p)
       ids = -1;
       pgs = 0;
       if (i < np) {
-        pgs = real_page(u0 + wave + i * kThinWaves, wp0, sink_pages);
+        pgs = real_page(u0 + wave + i * W, wp0, sink_pages);
         const int id = table[pgs];
         ids = (unsigned)id < (unsigned)p.num_blocks ? id : -1;
       }
@@ -240,7 +237,7 @@ __global__ __launch_bounds__(kThinThreads) void score_thin_kernel(ScoreParams p)
         compute(buf[j], i + j);
       }
     }
-    for (int u = u0 + wave; u < u0 + seg; u += kThinWaves)
+    for (int u = u0 + wave; u < u0 + seg; u += W)
       carry_gap(p, out, wp0, sink_pages, u, pages, lane, 64);
     left -= seg;
     u0 = 0;
@@ -248,6 +245,7 @@ __global__ __launch_bounds__(kThinThreads) void score_thin_kernel(ScoreParams p)
       ti = 0;
       ++h;
     }
+    if (left > 0) t = p.v.thin[ti];
   }
 }
 
@@ -473,14 +471,23 @@ __global__ __launch_bounds__(kWideThreads, 2) void score_wide_kernel(ScoreParams
 }
 
 template <typename T, int D>
-int launch_scores(const ScoreParams& p, int max_rows, int thin_rows, int cus, hipStream_t stream) {
+int launch_scores(const ScoreParams& p, int max_rows, int thin_rows, int waves, int cus,
+                  hipStream_t stream) {
   int st = RLSE_OK;
   if (thin_rows > 0) {
-    const dim3 grid(2 * cus), block(kThinThreads);
-    if (max_rows <= 16)
-      hipLaunchKernelGGL((score_thin_kernel<T, D, 1>), grid, block, 0, stream, p);
+    auto run = [&](auto rt, auto waves) {
+      constexpr int RT = decltype(rt)::value, W = decltype(waves)::value;
+      hipLaunchKernelGGL((score_thin_kernel<T, D, RT, W>), dim3(thin_groups(cus, W)), dim3(64 * W),
+                         0, stream, p);
+    };
+    const std::integral_constant<int, 1> one;
+    const std::integral_constant<int, 2> two;
+    const std::integral_constant<int, 4> four;
+    const std::integral_constant<int, 8> eight;
+    if (waves == 8)
+      max_rows <= 16 ? run(one, eight) : run(two, eight);
     else
-      hipLaunchKernelGGL((score_thin_kernel<T, D, 2>), grid, block, 0, stream, p);
+      max_rows <= 16 ? run(one, four) : run(two, four);
     st = launch_status("score_thin_kernel");
   }
   if (st || max_rows <= thin_rows) return st;
@@ -541,7 +548,8 @@ extern "C" int rlse_kv_scores(const void* q, const void* k_pool, const int32_t* 
   auto run = [&](auto t, auto d) {
     using T = decltype(t);
     constexpr int D = decltype(d)::value;
-    return launch_scores<T, D>(p, max_rows, thin_row_limit(num_seqs, max_rows), cus, s);
+    return launch_scores<T, D>(p, max_rows, thin_row_limit(num_seqs, max_rows),
+                               thin_waves(num_seqs, num_kv_heads, cus), cus, s);
   };
   const std::integral_constant<int, 64> d64;
   const std::integral_constant<int, 128> d128;
