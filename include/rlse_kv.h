@@ -443,20 +443,25 @@ int rlse_chunk_plan(const int32_t* cu_tokens, const int32_t* seq_lens, int num_s
  * (its pages' ids are all outside [0, num_blocks)) gives zeros and -inf.
  * Scores that are NaN, and infinite or NaN values of a visible key, reach
  * the rows that see it and no others. f32, bf16 or f16, head_dim 64 or 128,
- * any group size; q, out and pools 16-byte aligned. workspace:
+ * groups of up to 256 heads; q, out and pools 16-byte aligned. workspace:
  * rlse_chunk_workspace_size bytes (grows with none of the lengths), 16-byte
  * aligned, zero-filled once before its first use and then left to the
  * library; one serves every call with the same head shape and at most the
  * max_tokens it was sized for. Calls that share one must be ordered (same
  * stream). Results do not depend on what shares the step with a sequence
- * beyond rounding: its keys are divided among workgroups differently. */
+ * beyond rounding: its keys are divided among workgroups differently.
+ * flags: RLSE_CHUNK_SHARED_PAGES when sequences of the step share pages (forks
+ * of one prefix): the pages of few-token sequences, otherwise read with
+ * non-temporal loads as each is read once, then stay in the caches. The
+ * results are the same either way. */
+#define RLSE_CHUNK_SHARED_PAGES 1
 int rlse_chunk_workspace_size(int num_seqs, int total_tokens, int max_tokens, int num_heads,
                               int num_kv_heads, int head_dim, size_t* bytes);
 int rlse_chunk_attn(const void* q, const void* k_pool, const void* v_pool,
                     const int32_t* block_tables, void* plan, void* out, float* lse, int num_seqs,
                     int total_tokens, int max_tokens, int num_heads, int num_kv_heads,
                     int head_dim, int max_blocks_per_seq, int num_blocks, int window, int sinks,
-                    float scale, int dtype, void* workspace, size_t workspace_bytes,
+                    float scale, int dtype, void* workspace, size_t workspace_bytes, int flags,
                     rlse_stream_t stream);
 
 /* The weight each cached key receives from the step's queries: for every key
@@ -471,12 +476,12 @@ int rlse_chunk_attn(const void* q, const void* k_pool, const void* v_pool,
  * sequences without new tokens, are left as they were. Keys of pages whose
  * ids are out of range receive nothing; a row whose lse is -inf gives
  * nothing. Each sum is formed in one order: the same call gives the same
- * bits. Shapes, plan and dtypes as rlse_chunk_attn. */
+ * bits. Shapes, plan, dtypes and flags as rlse_chunk_attn. */
 int rlse_kv_scores(const void* q, const void* k_pool, const int32_t* block_tables, void* plan,
                    const float* lse, const float* prev, float* scores, int num_seqs,
                    int total_tokens, int max_tokens, int num_heads, int num_kv_heads,
                    int head_dim, int max_blocks_per_seq, int num_blocks, int window, int sinks,
-                   float scale, int dtype, rlse_stream_t stream);
+                   float scale, int dtype, int flags, rlse_stream_t stream);
 
 /* Eviction by accumulated weight, every layer at once. For layer l, sequence
  * b and KV head h with more than `budget` keys, the first `sinks`, the last

@@ -215,11 +215,12 @@ struct ThinLds {
   T v[W][16][D + kPad];
 };
 
-template <typename T, int D, int RT, int W>
+template <typename T, int D, int RT, int W, bool STREAM>
 __global__ __launch_bounds__(64 * W, 8 / W) void chunk_thin_kernel(ChunkParams p) {
   constexpr int N = PageRegs<T, D>::N;
   constexpr int ES = (int)sizeof(T), PPR = D * ES / 16;  // packets per row
   constexpr int DT = D / 16;
+  constexpr int POL = STREAM ? kLoadNonTemporal : 0;
   // Pages in registers: one at work, the others in flight (as many as fit).
   constexpr int NBUF = ES == 2 ? (RT == 1 ? 3 : 2) : D == 128 && RT == 2 ? 1 : 2;
   constexpr int kExRow = D + 4;
@@ -331,9 +332,9 @@ __global__ __launch_bounds__(64 * W, 8 / W) void chunk_thin_kernel(ChunkParams p
 #pragma unroll
       for (int r = 0; r < N; ++r) {
         b.k[r] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(
-                                               rk, col * D * ES + quad * 16 + r * 64, 0, 0));
+                                               rk, col * D * ES + quad * 16 + r * 64, 0, POL));
         b.v[r] = __builtin_bit_cast(
-            uint4, __builtin_amdgcn_raw_buffer_load_b128(rv, (lane + 64 * r) * 16, 0, 0));
+            uint4, __builtin_amdgcn_raw_buffer_load_b128(rv, (lane + 64 * r) * 16, 0, POL));
       }
       b.pos = id < 0 ? -1 : pos;
     };
@@ -543,19 +544,30 @@ __global__ __launch_bounds__(64 * W, 8 / W) void chunk_thin_kernel(ChunkParams p
           float M = -INFINITY, L = 0.f, acc[DPT];
 #pragma unroll
           for (int i = 0; i < DPT; ++i) acc[i] = 0.f;
-          for (int k = 0; k < npieces; ++k) {
-            const float* src = p.thin_part + (size_t)(2 * (first + k) + (k == 0 ? 1 : 0)) *
-                                                 kThinRows * (D + 2) + row * (D + 2);
-            float ml[2], a[DPT];
-            ld_pair(src + D, ml);
+          // kJoin pieces' loads go out together; those past the last read it
+          // again and are not joined.
+          constexpr int kJoin = 4;
+          for (int k0 = 0; k0 < npieces; k0 += kJoin) {
+            float ml[kJoin][2], a[kJoin][DPT];
 #pragma unroll
-            for (int i = 0; i < DPT; i += 2) ld_pair(src + ed + i, a + i);
-            const float mn = fmaxf(M, ml[0]);
-            const float sa = state_weight(M, mn), sb = state_weight(ml[0], mn);
-            L = L * sa + ml[1] * sb;
+            for (int j = 0; j < kJoin; ++j) {
+              const int k = min(k0 + j, npieces - 1);
+              const float* src = p.thin_part + (size_t)(2 * (first + k) + (k == 0 ? 1 : 0)) *
+                                                   kThinRows * (D + 2) + row * (D + 2);
+              ld_pair(src + D, ml[j]);
 #pragma unroll
-            for (int i = 0; i < DPT; ++i) acc[i] = acc[i] * sa + a[i] * sb;
-            M = mn;
+              for (int i = 0; i < DPT; i += 2) ld_pair(src + ed + i, a[j] + i);
+            }
+#pragma unroll
+            for (int j = 0; j < kJoin; ++j) {
+              if (k0 + j >= npieces) break;
+              const float mn = fmaxf(M, ml[j][0]);
+              const float sa = state_weight(M, mn), sb = state_weight(ml[j][0], mn);
+              L = L * sa + ml[j][1] * sb;
+#pragma unroll
+              for (int i = 0; i < DPT; ++i) acc[i] = acc[i] * sa + a[j][i] * sb;
+              M = mn;
+            }
           }
           finish(row, M, L, acc);
         }
@@ -1360,14 +1372,17 @@ ChunkWorkspace chunk_workspace(int max_rows, int D, int cus) {
 }
 
 template <typename T, int D>
-int launch_chunk(const ChunkParams& p, int max_rows, int thin_rows, int waves, int cus,
-                 hipStream_t stream) {
+int launch_chunk(const ChunkParams& p, int max_rows, int thin_rows, int waves, bool shared,
+                 int cus, hipStream_t stream) {
   int st = RLSE_OK;
   if (thin_rows > 0) {
-    auto run = [&](auto rt, auto waves) {
-      constexpr int RT = decltype(rt)::value, W = decltype(waves)::value;
-      hipLaunchKernelGGL((chunk_thin_kernel<T, D, RT, W>), dim3(thin_groups(cus, W)), dim3(64 * W),
-                         0, stream, p);
+    auto run = [&](auto rt, auto w) {
+      constexpr int RT = decltype(rt)::value, W = decltype(w)::value;
+      const dim3 grid(thin_groups(cus, W)), block(64 * W);
+      if (shared)
+        hipLaunchKernelGGL((chunk_thin_kernel<T, D, RT, W, false>), grid, block, 0, stream, p);
+      else
+        hipLaunchKernelGGL((chunk_thin_kernel<T, D, RT, W, true>), grid, block, 0, stream, p);
     };
     const std::integral_constant<int, 1> one;
     const std::integral_constant<int, 2> two;
@@ -1418,7 +1433,8 @@ extern "C" int rlse_chunk_attn(const void* q, const void* k_pool, const void* v_
                                int num_seqs, int total_tokens, int max_tokens, int num_heads,
                                int num_kv_heads, int head_dim, int max_blocks_per_seq,
                                int num_blocks, int window, int sinks, float scale, int dtype,
-                               void* workspace, size_t workspace_bytes, rlse_stream_t stream) {
+                               void* workspace, size_t workspace_bytes, int flags,
+                               rlse_stream_t stream) {
   int st = validate_chunk_shape("chunk_attn", num_seqs, total_tokens, max_tokens, num_heads,
                                 num_kv_heads, max_blocks_per_seq, window, sinks);
   if (st) return st;
@@ -1430,6 +1446,8 @@ extern "C" int rlse_chunk_attn(const void* q, const void* k_pool, const void* v_
     return fail(RLSE_ERR_INVALID_VALUE, "chunk_attn: num_blocks %d", num_blocks);
   if (!(scale > 0.f) || !isfinite(scale))
     return fail(RLSE_ERR_INVALID_VALUE, "chunk_attn: scale must be finite and positive");
+  if (flags & ~RLSE_CHUNK_SHARED_PAGES)
+    return fail(RLSE_ERR_INVALID_VALUE, "chunk_attn: unknown flags 0x%x", flags);
   if (!q || !k_pool || !v_pool || !block_tables || !plan || !out || !workspace)
     return fail(RLSE_ERR_INVALID_VALUE, "chunk_attn: null pointer argument");
   const uintptr_t align = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_pool) |
@@ -1473,7 +1491,8 @@ extern "C" int rlse_chunk_attn(const void* q, const void* k_pool, const void* v_
     using T = decltype(t);
     constexpr int D = decltype(d)::value;
     return launch_chunk<T, D>(p, max_rows, thin_row_limit(num_seqs, max_rows),
-                              thin_waves(num_seqs, num_kv_heads, cus), cus, s);
+                              thin_waves(num_seqs, num_kv_heads, cus),
+                              flags & RLSE_CHUNK_SHARED_PAGES, cus, s);
   };
   const std::integral_constant<int, 64> d64;
   const std::integral_constant<int, 128> d128;

@@ -27,7 +27,7 @@ namespace rlse {
 constexpr int kThinRows = 32;       // rows (tokens * group size) of a thin sequence at most
 constexpr int kWideRows = 256;      // rows per wide tile
 constexpr int kWidePages = 4;       // pages per wide unit
-constexpr int kScorePages = 16;     // pages per unit of the wide key-weight launch
+constexpr int kScorePages = 8;     // pages per unit of the wide key-weight launch
 constexpr int kMaxChunkSeqs = 4096; // prefix tables of the plan launch live in LDS
 constexpr int kThinMinUnits = 8;    // smallest share of a workgroup: pages,
 constexpr int kWideMinUnits = 4;    //   and wide units
@@ -35,6 +35,11 @@ constexpr int kWideMinUnits = 4;    //   and wide units
 // a thin workgroup about what it streams in the time of 16 pages, a wide one
 // about a unit.
 constexpr int kThinSnap = 16;
+// Pages of a thin tile that is not cut while there are workgroups for all: a
+// cut takes 8 us (pieces stored, counted and joined; one token after 700,
+// 16/8 heads of 128: 15.7 us cut, 11.4 whole), as long as 64 f32 pages or more
+// than 100 of 16 bits.
+constexpr int kThinWhole = 64;
 constexpr int kWideSnap = 1;
 
 // Rows of a thin sequence at most in a step of num_seqs sequences of up to
@@ -85,6 +90,19 @@ struct ChunkHead {
   int score_seqs, score_units;  // wide sequences, and their key blocks
 };
 constexpr int kChunkHeadBytes = 256;
+
+// A row's token, row / G, by multiplication: exact for row * G < 2^32 (rows are
+// below 2^23 and G at most kMaxGroup).
+constexpr int kMaxGroup = 256;
+struct RowDiv {
+  unsigned mul;
+  int G;
+  __host__ __device__ explicit RowDiv(int g)
+      : mul(g > 1 ? (unsigned)(0x100000000ull / (unsigned)g + 1) : 0u), G(g) {}
+  __host__ __device__ int token(int row) const {
+    return G == 1 ? row : (int)((unsigned long long)(unsigned)row * mul >> 32);
+  }
+};
 
 // What the plan's users agree on, in one word (FNV-1a over the arguments).
 struct ChunkShape {

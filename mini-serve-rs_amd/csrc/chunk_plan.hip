@@ -59,22 +59,26 @@ __device__ __forceinline__ int tile_of(const int* held, const ChunkTile* a, int 
 }
 
 // Shares of `units` units of each of Hkv heads over at most max_groups
-// workgroups of at least min_units each. Equal shares, but a boundary within
-// snap units of a tile's moves there: a tile cut for the sake of a few units
-// costs more than they do. I: an integer type that holds units * Hkv *
+// workgroups of at least min_units each: equal shares, but a boundary within
+// snap units of a tile's moves there, and with `whole` (n * Hkv <= max_groups)
+// each gets one tile. (A tile cut
+// for the sake of a few units costs more than they do.) I: an integer type that holds units * Hkv *
 // max_groups; starts: max_groups + 1 of them in LDS.
 constexpr int kMaxShares = 1024;
 template <typename I>
 __device__ void deal(const int* held, const ChunkTile* tiles, int n, int units, int Hkv,
-                     int max_groups, int min_units, int snap, I* starts, ChunkShare* out) {
+                     int max_groups, int min_units, int snap, bool whole, I* starts,
+                     ChunkShare* out) {
   const I total = (I)units * Hkv;
   const I want = (total + min_units - 1) / min_units;
-  const int groups = (int)(want < (I)max_groups ? want : (I)max_groups);
+  const int groups = whole ? n * Hkv : (int)(want < (I)max_groups ? want : (I)max_groups);
   auto unit0 = [&](int i) { return i < n ? (i < kHeld ? held[i] : tiles[i].unit0) : units; };
   snap = min((I)snap, total / (4 * groups));
   for (int w = threadIdx.x; w <= groups; w += kPlanThreads) {
     I x = total * w / groups;
-    if (w > 0 && w < groups) {
+    if (whole) {
+      x = w < groups ? (I)(w / n) * units + unit0(w % n) : total;
+    } else if (w > 0 && w < groups) {
       const int head = (int)(x / units), u = (int)(x - (I)head * units);
       const int i = tile_of(held, tiles, n, u), lo = unit0(i), hi = unit0(i + 1);
       if (u - lo <= snap)
@@ -118,18 +122,19 @@ __device__ void deal(const int* held, const ChunkTile* tiles, int n, int units, 
   __syncthreads();
 }
 __device__ void deal_shares(const int* held, const ChunkTile* tiles, int n, int units, int Hkv,
-                            int max_groups, int min_units, int snap, unsigned long long* starts,
-                            ChunkShare* out) {
+                            int max_groups, int min_units, int snap, bool whole,
+                            unsigned long long* starts, ChunkShare* out) {
   if (units == 0) {
     for (int b = threadIdx.x; b < max_groups; b += kPlanThreads) out[b].count = 0;
     return;
   }
   // (64-bit divisions take a few microseconds here.)
   if ((unsigned long long)units * Hkv * max_groups < (1ull << 31))
-    deal<unsigned>(held, tiles, n, units, Hkv, max_groups, min_units, snap,
+    deal<unsigned>(held, tiles, n, units, Hkv, max_groups, min_units, snap, whole,
                    reinterpret_cast<unsigned*>(starts), out);
   else
-    deal<unsigned long long>(held, tiles, n, units, Hkv, max_groups, min_units, snap, starts, out);
+    deal<unsigned long long>(held, tiles, n, units, Hkv, max_groups, min_units, snap, whole, starts,
+                             out);
 }
 
 __global__ __launch_bounds__(kPlanThreads) void chunk_plan_kernel(PlanParams p) {
@@ -138,8 +143,12 @@ __global__ __launch_bounds__(kPlanThreads) void chunk_plan_kernel(PlanParams p) 
   __shared__ int s_thin[kHeld], s_unit[kHeld];  // unit0 of the thin and the wide tiles
   __shared__ unsigned long long s_starts[kMaxShares + 1];
   __shared__ unsigned s_flags;
+  __shared__ int s_longest;  // pages of the longest thin tile
   const int tid = threadIdx.x;
-  if (tid == 0) s_flags = 0;
+  if (tid == 0) {
+    s_flags = 0;
+    s_longest = 0;
+  }
   __syncthreads();
 
   int thin_tiles = 0, thin_units = 0, wide_tiles = 0, score_seqs = 0, score_units = 0;
@@ -175,6 +184,7 @@ __global__ __launch_bounds__(kPlanThreads) void chunk_plan_kernel(PlanParams p) 
       t.unit0 = u;
       p.v.thin[at] = t;
       if (at < kHeld) s_thin[at] = u;
+      atomicMax(&s_longest, t.pages);
     }
     at = block_scan(wide, s_w, &sum) + score_seqs;
     score_seqs += sum;
@@ -224,9 +234,10 @@ __global__ __launch_bounds__(kPlanThreads) void chunk_plan_kernel(PlanParams p) 
   __syncthreads();
 
   deal_shares(s_thin, p.v.thin, thin_tiles, thin_units, p.Hkv, p.thin_groups, kThinMinUnits,
-              kThinSnap, s_starts, p.v.thin_share);
+              kThinSnap, (long long)thin_tiles * p.Hkv <= p.thin_groups && s_longest <= kThinWhole,
+              s_starts, p.v.thin_share);
   deal_shares(s_unit, p.v.wide, wide_tiles, wide_units, p.Hkv, p.cus, kWideMinUnits, kWideSnap,
-              s_starts, p.v.wide_share);
+              false, s_starts, p.v.wide_share);
   if (tid == 0) {
     ChunkHead h;
     h.flags = s_flags;
@@ -254,6 +265,8 @@ int validate_chunk_shape(const char* what, int num_seqs, int total_tokens, int m
   if (Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0)
     return fail(RLSE_ERR_INVALID_VALUE, "%s: num_heads %d not a multiple of num_kv_heads %d", what,
                 Hq, Hkv);
+  if (Hq / Hkv > kMaxGroup)
+    return fail(RLSE_ERR_INVALID_VALUE, "%s: group size %d above %d", what, Hq / Hkv, kMaxGroup);
   if ((long long)total_tokens * Hq > 0x7fffffffLL / 256)
     return fail(RLSE_ERR_INVALID_VALUE, "%s: total_tokens * num_heads too large", what);
   if (mbps <= 0 || mbps > (1 << 24))

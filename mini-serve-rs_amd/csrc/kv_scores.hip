@@ -15,8 +15,9 @@
 //  - thin sequences (at most 32 rows): HBM bound on K. A wave takes a page at
 //    a time, 16 keys of all rows on 16x16 MFMAs.
 //  - wide ones: bound by the exponentials (16 a lane and 32x32 tile, at a
-//    quarter of the VALU's rate) beside the MFMAs. A workgroup holds 256 keys
-//    in registers and streams the rows through LDS, 64 (f32: 32) at a time.
+//    quarter of the VALU's rate) beside the MFMAs. A workgroup holds 128 keys
+//    in registers and streams the rows through LDS, 64 (f32: 32) at a time;
+//    three of them share a compute unit, to cover each other's loads.
 #include <math.h>
 
 #include "chunk_plan.cuh"
@@ -44,6 +45,7 @@ struct ScoreParams {
   uint32_t stamp;
   int Hq, Hkv, G, mbps, num_blocks, window, sinks;
   float c;  // scale * log2(e)
+  RowDiv div{1};
 };
 
 template <typename T>
@@ -100,13 +102,13 @@ __device__ __forceinline__ void carry_gap(const ScoreParams& p, size_t row, int 
   for (int k = a + thread; k < b; k += threads)
     p.scores[row + k] = p.prev ? p.prev[row + k] : 0.f;
 }
-__device__ __forceinline__ void write_score(const ScoreParams& p, size_t row, int k, int off,
-                                            int kend, float w) {
-  if (k < kend) p.scores[row + k] = w + (p.prev && k < off ? p.prev[row + k] : 0.f);
+// What key k (of a sequence with `off` older ones) had before.
+__device__ __forceinline__ float had(const ScoreParams& p, size_t row, int k, int off) {
+  return p.prev && k < off ? p.prev[row + k] : 0.f;
 }
 
 
-template <typename T, int D, int RT, int W>
+template <typename T, int D, int RT, int W, bool STREAM>
 __global__ __launch_bounds__(64 * W) void score_thin_kernel(ScoreParams p) {
   constexpr int ES = (int)sizeof(T), N = D * ES / 64;
   constexpr int NBUF = 4;
@@ -183,6 +185,7 @@ __global__ __launch_bounds__(64 * W) void score_thin_kernel(ScoreParams p) {
 
     struct Page {
       uint4 k[N];
+      float had;  // what its keys had before, one a lane
       int id, pos;
     };
     auto load = [&](Page& b, int i) __attribute__((always_inline)) {
@@ -196,7 +199,9 @@ __global__ __launch_bounds__(64 * W) void score_thin_kernel(ScoreParams p) {
 #pragma unroll
       for (int r = 0; r < N; ++r)
         b.k[r] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(
-                                               rk, col * D * ES + quad * 16 + r * 64, 0, 0));
+                                               rk, col * D * ES + quad * 16 + r * 64, 0,
+                                               STREAM ? kLoadNonTemporal : 0));
+      b.had = i < np ? had(p, out, b.pos + col, off) : 0.f;
     };
     auto compute = [&](const Page& b, int i) __attribute__((always_inline)) {
       if (i >= np) return;  // (uniform)
@@ -224,7 +229,7 @@ __global__ __launch_bounds__(64 * W) void score_thin_kernel(ScoreParams p) {
         w += __shfl_xor(w, 16, 64);
         w += __shfl_xor(w, 32, 64);
       }
-      if (lane < 16) write_score(p, out, b.pos + col, off, kend, w);
+      if (lane < 16 && b.pos + col < kend) p.scores[out + b.pos + col] = w + b.had;
     };
 
     Page buf[NBUF];
@@ -249,12 +254,12 @@ __global__ __launch_bounds__(64 * W) void score_thin_kernel(ScoreParams p) {
   }
 }
 
-constexpr int kWideWaves = 8;
+constexpr int kWideWaves = 4;
 constexpr int kWideThreads = 64 * kWideWaves;
 constexpr int kScoreKeys = 16 * kScorePages;  // keys a workgroup holds
 
 template <typename T, int D>
-__global__ __launch_bounds__(kWideThreads, 2) void score_wide_kernel(ScoreParams p) {
+__global__ __launch_bounds__(kWideThreads, 3) void score_wide_kernel(ScoreParams p) {
   constexpr int ES = (int)sizeof(T);
   constexpr int KB = D * ES / 32;          // 16-byte packets of a lane's key
   constexpr int KS = ES == 2 ? 2 : 1;      // 32-key blocks per wave
@@ -284,6 +289,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void score_wide_kernel(ScoreParams
   const int kg = wave % KG, rg = wave / KG;
   const int Hq = p.Hq, Hkv = p.Hkv, G = p.G;
   const int sink_pages = (p.sinks + 15) >> 4;
+  const RowDiv div = p.div;
   const T* __restrict__ qb = static_cast<const T*>(p.q);
   const T* __restrict__ kp = static_cast<const T*>(p.k_pool);
 
@@ -352,7 +358,17 @@ __global__ __launch_bounds__(kWideThreads, 2) void score_wide_kernel(ScoreParams
     float sum[KS];
 #pragma unroll
     for (int i = 0; i < KS; ++i) sum[i] = 0.f;
+    // What the key that this thread will write had before.
+    float before = 0.f;
+    if (tid < kScoreKeys && vfirst + (tid >> 4) <= vlast)
+      before = had(p, out, real_page(vfirst + (tid >> 4), wp0, sink_pages) * 16 + (tid & 15), off);
 
+    // Row r of this head's: token r / G, head r % G of the group.
+    const T* __restrict__ qh = qb + ((size_t)tok0 * Hq + h * G) * D;
+    const float* __restrict__ lh = p.lse + (size_t)tok0 * Hq + h * G;
+    auto place = [&](int row) __attribute__((always_inline)) {
+      return row + div.token(row) * (Hq - G);
+    };
     u32x4_t qst[QPT];
     float lst = 0.f;
     int kst = 0;
@@ -360,18 +376,14 @@ __global__ __launch_bounds__(kWideThreads, 2) void score_wide_kernel(ScoreParams
 #pragma unroll
       for (int j = 0; j < QPT; ++j) {
         const int pk = tid + j * kWideThreads;
-        const int row = r0 + pk / PPR, dc = pk % PPR;
-        const int tok = row / G;
-        qst[j] = u32x4_t{0, 0, 0, 0};
-        if (row < rows)
-          qst[j] = *reinterpret_cast<const u32x4_t*>(
-              qb + ((size_t)(tok0 + tok) * Hq + h * G + row - tok * G) * D + dc * (16 / ES));
+        const int row = min(r0 + pk / PPR, rows - 1), dc = pk % PPR;
+        qst[j] = *reinterpret_cast<const u32x4_t*>(qh + (size_t)place(row) * D + dc * (16 / ES));
       }
       if (tid < ROWS) {
-        const int row = r0 + tid, tok = row / G;
-        lst = row < rows ? row_lse(p.lse[(size_t)(tok0 + tok) * Hq + h * G + row - tok * G])
-                         : INFINITY;
-        kst = off + tok;
+        // (Rows past the last read it again, without weight.)
+        const int row = min(r0 + tid, rows - 1);
+        lst = r0 + tid < rows ? row_lse(lh[place(row)]) : INFINITY;
+        kst = off + div.token(row);
       }
     };
     auto store = [&](int bf) __attribute__((always_inline)) {
@@ -396,7 +408,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void score_wide_kernel(ScoreParams
         if (more) load(r0 + ROWS);
         // This wave's rows, and what they see of its keys.
         const int ra = r0 + rg * 32, rb = min(ra + 31, rows - 1);
-        const int kmax_lo = off + min(ra, rows - 1) / G, kmax_hi = off + rb / G;
+        const int kmax_lo = off + div.token(min(ra, rows - 1)), kmax_hi = off + div.token(rb);
         const bool none =
             ra >= rows || first_key > kmax_hi ||
             (p.window > 0 && last_key <= kmax_lo - p.window && first_key >= p.sinks);
@@ -462,7 +474,8 @@ __global__ __launch_bounds__(kWideThreads, 2) void score_wide_kernel(ScoreParams
         float w = s_sum[0][tid];
 #pragma unroll
         for (int i = 1; i < RG; ++i) w += s_sum[i][tid];
-        write_score(p, out, real_page(vi, wp0, sink_pages) * 16 + (tid & 15), off, kend, w);
+        const int key = real_page(vi, wp0, sink_pages) * 16 + (tid & 15);
+        if (key < kend) p.scores[out + key] = w + before;
       }
     }
     carry_gap(p, out, wp0, sink_pages, u, (pages + kScorePages - 1) / kScorePages, tid,
@@ -471,14 +484,17 @@ __global__ __launch_bounds__(kWideThreads, 2) void score_wide_kernel(ScoreParams
 }
 
 template <typename T, int D>
-int launch_scores(const ScoreParams& p, int max_rows, int thin_rows, int waves, int cus,
-                  hipStream_t stream) {
+int launch_scores(const ScoreParams& p, int max_rows, int thin_rows, int waves, bool shared,
+                  int cus, hipStream_t stream) {
   int st = RLSE_OK;
   if (thin_rows > 0) {
-    auto run = [&](auto rt, auto waves) {
-      constexpr int RT = decltype(rt)::value, W = decltype(waves)::value;
-      hipLaunchKernelGGL((score_thin_kernel<T, D, RT, W>), dim3(thin_groups(cus, W)), dim3(64 * W),
-                         0, stream, p);
+    auto run = [&](auto rt, auto w) {
+      constexpr int RT = decltype(rt)::value, W = decltype(w)::value;
+      const dim3 grid(thin_groups(cus, W)), block(64 * W);
+      if (shared)
+        hipLaunchKernelGGL((score_thin_kernel<T, D, RT, W, false>), grid, block, 0, stream, p);
+      else
+        hipLaunchKernelGGL((score_thin_kernel<T, D, RT, W, true>), grid, block, 0, stream, p);
     };
     const std::integral_constant<int, 1> one;
     const std::integral_constant<int, 2> two;
@@ -491,7 +507,7 @@ int launch_scores(const ScoreParams& p, int max_rows, int thin_rows, int waves, 
     st = launch_status("score_thin_kernel");
   }
   if (st || max_rows <= thin_rows) return st;
-  hipLaunchKernelGGL((score_wide_kernel<T, D>), dim3(2 * cus), dim3(kWideThreads), 0, stream, p);
+  hipLaunchKernelGGL((score_wide_kernel<T, D>), dim3(3 * cus), dim3(kWideThreads), 0, stream, p);
   return launch_status("score_wide_kernel");
 }
 
@@ -505,7 +521,7 @@ extern "C" int rlse_kv_scores(const void* q, const void* k_pool, const int32_t* 
                               int num_seqs, int total_tokens, int max_tokens, int num_heads,
                               int num_kv_heads, int head_dim, int max_blocks_per_seq,
                               int num_blocks, int window, int sinks, float scale, int dtype,
-                              rlse_stream_t stream) {
+                              int flags, rlse_stream_t stream) {
   int st = validate_chunk_shape("kv_scores", num_seqs, total_tokens, max_tokens, num_heads,
                                 num_kv_heads, max_blocks_per_seq, window, sinks);
   if (st) return st;
@@ -517,6 +533,8 @@ extern "C" int rlse_kv_scores(const void* q, const void* k_pool, const int32_t* 
     return fail(RLSE_ERR_INVALID_VALUE, "kv_scores: num_blocks %d", num_blocks);
   if (!(scale > 0.f) || !isfinite(scale))
     return fail(RLSE_ERR_INVALID_VALUE, "kv_scores: scale must be finite and positive");
+  if (flags & ~RLSE_CHUNK_SHARED_PAGES)
+    return fail(RLSE_ERR_INVALID_VALUE, "kv_scores: unknown flags 0x%x", flags);
   if (!q || !k_pool || !block_tables || !plan || !lse || !scores)
     return fail(RLSE_ERR_INVALID_VALUE, "kv_scores: null pointer argument");
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_pool) |
@@ -543,13 +561,15 @@ extern "C" int rlse_kv_scores(const void* q, const void* k_pool, const int32_t* 
   p.window = window;
   p.sinks = sinks;
   p.c = scale * kLog2E;
+  p.div = RowDiv(p.G);
   const int max_rows = max_tokens * p.G;
   const hipStream_t s = as_stream(stream);
   auto run = [&](auto t, auto d) {
     using T = decltype(t);
     constexpr int D = decltype(d)::value;
     return launch_scores<T, D>(p, max_rows, thin_row_limit(num_seqs, max_rows),
-                               thin_waves(num_seqs, num_kv_heads, cus), cus, s);
+                               thin_waves(num_seqs, num_kv_heads, cus),
+                               flags & RLSE_CHUNK_SHARED_PAGES, cus, s);
   };
   const std::integral_constant<int, 64> d64;
   const std::integral_constant<int, 128> d128;

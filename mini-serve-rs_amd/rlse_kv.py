@@ -46,6 +46,7 @@ ERR_BUFFER_TOO_SMALL = 10003
 ERR_TOKEN_LIMIT = 10004
 ERR_DEVICE_TIMEOUT = 10005
 DECODE_STREAM = 1
+CHUNK_SHARED_PAGES = 1
 WS_ERR_MERGE_TIMEOUT = 1
 WS_ERR_LENGTH = 2
 WS_ERR_PREFIX = 4
@@ -214,8 +215,8 @@ _SIGS = {
     "rlse_chunk_plan_size": (_i, [_i, _i, _i, _i, ctypes.POINTER(_sz)]),
     "rlse_chunk_plan": (_i, [_vp, _vp] + [_i] * 8 + [_vp, _sz, _vp]),
     "rlse_chunk_workspace_size": (_i, [_i, _i, _i, _i, _i, _i, ctypes.POINTER(_sz)]),
-    "rlse_chunk_attn": (_i, [_vp] * 7 + [_i] * 10 + [_f, _i, _vp, _sz, _vp]),
-    "rlse_kv_scores": (_i, [_vp] * 7 + [_i] * 10 + [_f, _i, _vp]),
+    "rlse_chunk_attn": (_i, [_vp] * 7 + [_i] * 10 + [_f, _i, _vp, _sz, _i, _vp]),
+    "rlse_kv_scores": (_i, [_vp] * 7 + [_i] * 10 + [_f, _i, _i, _vp]),
     "rlse_kv_evict": (_i, [_vp, _vp, _ll, _i, _vp, _vp, _vp, _ll] + [_vp] * 4 + [_i] * 10 + [_vp]),
     "rlse_rmsnorm": (_i, [_vp, _vp, _vp, _i, _i, _f, _i, _vp]),
     "rlse_rope_tables": (_i, [_d, _i, _i, _i, _vp, _vp]),
@@ -959,21 +960,25 @@ def chunk_workspace_size(num_seqs: int, total_tokens: int, max_tokens: int, num_
 def chunk_attn(q, k_pool, v_pool, block_tables, plan, out, lse, num_seqs: int, total_tokens: int,
                max_tokens: int, num_heads: int, num_kv_heads: int, head_dim: int,
                max_blocks_per_seq: int, num_blocks: int, window: int, sinks: int, scale: float,
-               dtype, workspace, workspace_bytes: int, stream=None) -> None:
+               dtype, workspace, workspace_bytes: int, stream=None,
+               shared_pages: bool = False) -> None:
     """Attention of a ragged step's new tokens over their sequences' pages,
     every key up to their own or a sliding window and sinks; lse (f32
-    [total_tokens][num_heads], may be None) receives the log-sum-exp."""
+    [total_tokens][num_heads], may be None) receives the log-sum-exp.
+    shared_pages (RLSE_CHUNK_SHARED_PAGES): sequences of the step share pages,
+    which are then kept in the caches."""
     _check(load().rlse_chunk_attn(_ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(block_tables),
                                   _ptr(plan), _ptr(out), _ptr(lse), num_seqs, total_tokens,
                                   max_tokens, num_heads, num_kv_heads, head_dim,
                                   max_blocks_per_seq, num_blocks, window, sinks, scale, _dt(dtype),
-                                  _ptr(workspace), workspace_bytes, _stream(stream)))
+                                  _ptr(workspace), workspace_bytes,
+                                  CHUNK_SHARED_PAGES if shared_pages else 0, _stream(stream)))
 
 
 def kv_scores(q, k_pool, block_tables, plan, lse, prev, scores, num_seqs: int, total_tokens: int,
               max_tokens: int, num_heads: int, num_kv_heads: int, head_dim: int,
               max_blocks_per_seq: int, num_blocks: int, window: int, sinks: int, scale: float,
-              dtype, stream=None) -> None:
+              dtype, stream=None, shared_pages: bool = False) -> None:
     """The weight each cached key receives from a ragged step's queries (f32
     [num_seqs][num_kv_heads][max_blocks_per_seq*16]), from the lse of the
     step's chunk_attn, added to prev (None: counted anew; scores itself: in
@@ -981,7 +986,8 @@ def kv_scores(q, k_pool, block_tables, plan, lse, prev, scores, num_seqs: int, t
     _check(load().rlse_kv_scores(_ptr(q), _ptr(k_pool), _ptr(block_tables), _ptr(plan), _ptr(lse),
                                  _ptr(prev), _ptr(scores), num_seqs, total_tokens, max_tokens,
                                  num_heads, num_kv_heads, head_dim, max_blocks_per_seq,
-                                 num_blocks, window, sinks, scale, _dt(dtype), _stream(stream)))
+                                 num_blocks, window, sinks, scale, _dt(dtype),
+                                 CHUNK_SHARED_PAGES if shared_pages else 0, _stream(stream)))
 
 
 def kv_evict(k_pool, v_pool, layer_stride_elems: int, num_layers: int, block_tables, seq_lens,

@@ -13,12 +13,13 @@ def _plan(kv, **a):
 def _attn(kv, ptr=16, **a):
     return kv.load().rlse_chunk_attn(ptr, 16, 16, 16, 16, 16, None, a["n"], a["total"], a["most"],
                                      a["hq"], a["hkv"], a["d"], a["mbps"], a["nb"], a["window"],
-                                     a["sinks"], a["scale"], a["dtype"], 16, 1 << 40, None)
+                                     a["sinks"], a["scale"], a["dtype"], 16, 1 << 40,
+                                     a.get("flags", 0), None)
 
 
 SHAPES = [dict(n=0), dict(n=4097), dict(total=0), dict(most=0), dict(most=11), dict(hq=12),
           dict(hq=0), dict(hkv=0), dict(mbps=0), dict(mbps=1 << 25), dict(window=-1),
-          dict(sinks=-1), dict(total=1 << 24, hq=64)]
+          dict(sinks=-1), dict(total=1 << 24, hq=64), dict(hq=514, hkv=2)]
 
 
 @pytest.mark.parametrize("change", SHAPES, ids=str)
@@ -30,7 +31,8 @@ def test_shapes(kv, change):
 
 
 @pytest.mark.parametrize("change", [dict(d=96), dict(dtype=7), dict(nb=0), dict(scale=0.0),
-                                    dict(scale=float("nan")), dict(scale=float("inf"))], ids=str)
+                                    dict(scale=float("nan")), dict(scale=float("inf")),
+                                    dict(flags=2)], ids=str)
 def test_attention_arguments(kv, change):
     assert _attn(kv, **{**GOOD, **change}) == kv.ERR_INVALID_VALUE
     assert "chunk_attn" in kv.last_error()
@@ -53,11 +55,12 @@ def test_pointers(kv):
 def _scores(kv, ptr=16, **a):
     return kv.load().rlse_kv_scores(ptr, 16, 16, 16, 16, None, 16, a["n"], a["total"], a["most"],
                                     a["hq"], a["hkv"], a["d"], a["mbps"], a["nb"], a["window"],
-                                    a["sinks"], a["scale"], a["dtype"], None)
+                                    a["sinks"], a["scale"], a["dtype"],
+                                    a.get("flags", 0), None)
 
 
 @pytest.mark.parametrize("change", SHAPES + [dict(d=96), dict(dtype=7), dict(nb=0),
-                                             dict(scale=0.0)], ids=str)
+                                             dict(scale=0.0), dict(flags=4)], ids=str)
 def test_score_arguments(kv, change):
     assert _scores(kv, **{**GOOD, **change}) == kv.ERR_INVALID_VALUE
     assert "kv_scores" in kv.last_error()
