@@ -88,7 +88,7 @@ __device__ __forceinline__ float row_lse(float lse) {
 }
 // Whether a row whose own key is at kmax sees key k.
 __device__ __forceinline__ bool row_sees(int k, int kmax, int window, int sinks) {
-  return k <= kmax && (window <= 0 || k > kmax - window || k < sinks);
+  return (k <= kmax) & ((window <= 0) | (k > kmax - window) | (k < sinks));  // (no branches)
 }
 
 // Keys between the sinks' pages and the window's, which no row sees, keep
@@ -364,7 +364,9 @@ __global__ __launch_bounds__(kWideThreads, 3) void score_wide_kernel(ScoreParams
       before = had(p, out, real_page(vfirst + (tid >> 4), wp0, sink_pages) * 16 + (tid & 15), off);
 
     // Row r of this head's: token r / G, head r % G of the group.
-    const T* __restrict__ qh = qb + ((size_t)tok0 * Hq + h * G) * D;
+    const auto rq = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<T*>(qb + ((size_t)tok0 * Hq + h * G) * D), 0,
+        (int)(((unsigned)(n - 1) * Hq + G) * (D * ES)), kBufferWord3);
     const float* __restrict__ lh = p.lse + (size_t)tok0 * Hq + h * G;
     auto place = [&](int row) __attribute__((always_inline)) {
       return row + div.token(row) * (Hq - G);
@@ -376,8 +378,9 @@ __global__ __launch_bounds__(kWideThreads, 3) void score_wide_kernel(ScoreParams
 #pragma unroll
       for (int j = 0; j < QPT; ++j) {
         const int pk = tid + j * kWideThreads;
-        const int row = min(r0 + pk / PPR, rows - 1), dc = pk % PPR;
-        qst[j] = *reinterpret_cast<const u32x4_t*>(qh + (size_t)place(row) * D + dc * (16 / ES));
+        // (Rows past the last lie past the descriptor's end: zeros.)
+        qst[j] = __builtin_amdgcn_raw_buffer_load_b128(
+            rq, (int)((unsigned)place(r0 + pk / PPR) * (D * ES) + pk % PPR * 16), 0, 0);
       }
       if (tid < ROWS) {
         // (Rows past the last read it again, without weight.)
@@ -428,30 +431,30 @@ __global__ __launch_bounds__(kWideThreads, 3) void score_wide_kernel(ScoreParams
           const bool whole = valid && last_key <= kmax_lo && last_key < kend && rb == ra + 31 &&
                              (p.window <= 0 || first_key > kmax_hi - p.window ||
                               last_key < p.sinks);
+// Accumulator element e is row 8 (e/4) + 4 half + e%4 of the 32.
+          float l[16];
 #pragma unroll
-          for (int g4 = 0; g4 < 4; ++g4) {
-            const int r = rg * 32 + g4 * 8 + half * 4;
-            const float4 l4 = *reinterpret_cast<const float4*>(&s_lse[bf][r]);
-            const float l[4] = {l4.x, l4.y, l4.z, l4.w};
-            if (whole) {
+          for (int e = 0; e < 16; e += 4)
+            *reinterpret_cast<float4*>(l + e) = *reinterpret_cast<const float4*>(
+                &s_lse[bf][rg * 32 + e * 2 + half * 4]);
+          if (whole) {
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
+            for (int e = 0; e < 16; ++e)
 #pragma unroll
-                for (int i = 0; i < KS; ++i)
-                  sum[i] += __builtin_amdgcn_exp2f(fmaf(x[i][g4 * 4 + j], p.c, -l[j]));
-            } else {
-              const int4 m4 = *reinterpret_cast<const int4*>(&s_kmax[bf][r]);
-              const int m[4] = {m4.x, m4.y, m4.z, m4.w};
+              for (int i = 0; i < KS; ++i)
+                sum[i] += __builtin_amdgcn_exp2f(fmaf(x[i][e], p.c, -l[e]));
+          } else {
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
+            for (int e = 0; e < 16; ++e) {
+              const int r = rg * 32 + (e >> 2) * 8 + half * 4 + (e & 3);
+              const int own = s_kmax[bf][r];
 #pragma unroll
-                for (int i = 0; i < KS; ++i) {
-                  const float e = __builtin_amdgcn_exp2f(fmaf(x[i][g4 * 4 + j], p.c, -l[j]));
-                  sum[i] += r0 + r + j < rows && here[i] &&
-                                    row_sees(key[i], m[j], p.window, p.sinks)
-                                ? e
-                                : 0.f;
-                }
+              for (int i = 0; i < KS; ++i) {
+                const float w = __builtin_amdgcn_exp2f(fmaf(x[i][e], p.c, -l[e]));
+                const bool see = (r0 + r < rows) & here[i] &
+                                 row_sees(key[i], own, p.window, p.sinks);
+                sum[i] += see ? w : 0.f;
+              }
             }
           }
         }
