@@ -311,12 +311,10 @@ __global__ __launch_bounds__(kWideThreads, 3) void score_wide_kernel(ScoreParams
     const size_t out = ((size_t)seq * Hkv + h) * p.mbps * 16;
     const int rows = n * G, kend = off + n;
 
-    // This lane's keys (one per 32-key block) and, for the wave, the pages
-    // of all its keys.
+    // This lane's keys (one per 32-key block).
     int key[KS];
-    bool here[KS];
+    unsigned reach[KS];  // rows see key when their own is at key .. key + reach
     uint4 k[KS][KB];
-    int pos[2 * KS];
     bool valid = true;
     int first_key = 0x7fffffff, last_key = -1;
 #pragma unroll
@@ -325,21 +323,24 @@ __global__ __launch_bounds__(kWideThreads, 3) void score_wide_kernel(ScoreParams
       const int pg = real_page(min(vi, pages - 1), wp0, sink_pages);
       const int id = table[pg];
       const bool ok = vi < pages && (unsigned)id < (unsigned)p.num_blocks;
-      pos[i] = vi < pages ? pg * 16 : -1;
       valid = valid && ok;
       if (ok) {
         first_key = min(first_key, pg * 16);
         last_key = max(last_key, pg * 16 + 15);
       }
       if ((col >> 4) == (i & 1)) {
-        key[i >> 1] = vi < pages ? pg * 16 + (col & 15) : kend;
-        here[i >> 1] = ok && key[i >> 1] < kend;
+        const int at = pg * 16 + (col & 15);
+        const bool here = ok && at < kend;
+        key[i >> 1] = here ? at : 0x7fffffff;
+        reach[i >> 1] = !here ? 0u
+                        : p.window > 0 && at >= p.sinks ? (unsigned)p.window - 1u
+                                                        : 0x7fffffffu;
         const T* src = kp + (((size_t)(ok ? id : 0) * Hkv + h) * 16 + (col & 15)) * D;
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
           // 16-bit: elements 16 b + 8 half ..; f32: half * D/2 + 4 b ..
-          const int at = ES == 2 ? b * 16 + half * 8 : half * (D / 2) + b * 4;
-          k[i >> 1][b] = here[i >> 1] ? *reinterpret_cast<const uint4*>(src + at)
+          const int e = ES == 2 ? b * 16 + half * 8 : half * (D / 2) + b * 4;
+          k[i >> 1][b] = here ? *reinterpret_cast<const uint4*>(src + e)
                                       : make_uint4(0, 0, 0, 0);
         }
       }
@@ -383,10 +384,10 @@ __global__ __launch_bounds__(kWideThreads, 3) void score_wide_kernel(ScoreParams
             rq, (int)((unsigned)place(r0 + pk / PPR) * (D * ES) + pk % PPR * 16), 0, 0);
       }
       if (tid < ROWS) {
-        // (Rows past the last read it again, without weight.)
+        // (Rows past the last read it again; they see no key.)
         const int row = min(r0 + tid, rows - 1);
-        lst = r0 + tid < rows ? row_lse(lh[place(row)]) : INFINITY;
-        kst = off + div.token(row);
+        lst = lh[place(row)];
+        kst = r0 + tid < rows ? off + div.token(row) : -1;
       }
     };
     auto store = [&](int bf) __attribute__((always_inline)) {
@@ -396,7 +397,7 @@ __global__ __launch_bounds__(kWideThreads, 3) void score_wide_kernel(ScoreParams
         *reinterpret_cast<u32x4_t*>(&s_q[bf][pk / PPR][pk % PPR * (16 / ES)]) = qst[j];
       }
       if (tid < ROWS) {
-        s_lse[bf][tid] = lst;
+        s_lse[bf][tid] = kst < 0 ? INFINITY : row_lse(lst);
         s_kmax[bf][tid] = kst;
       }
     };
@@ -432,29 +433,34 @@ __global__ __launch_bounds__(kWideThreads, 3) void score_wide_kernel(ScoreParams
                              (p.window <= 0 || first_key > kmax_hi - p.window ||
                               last_key < p.sinks);
 // Accumulator element e is row 8 (e/4) + 4 half + e%4 of the 32.
-          float l[16];
-#pragma unroll
-          for (int e = 0; e < 16; e += 4)
-            *reinterpret_cast<float4*>(l + e) = *reinterpret_cast<const float4*>(
-                &s_lse[bf][rg * 32 + e * 2 + half * 4]);
+          const float* ls = &s_lse[bf][rg * 32 + half * 4];
           if (whole) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-#pragma unroll
-              for (int i = 0; i < KS; ++i)
-                sum[i] += __builtin_amdgcn_exp2f(fmaf(x[i][e], p.c, -l[e]));
-          } else {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const int r = rg * 32 + (e >> 2) * 8 + half * 4 + (e & 3);
-              const int own = s_kmax[bf][r];
+            for (int e4 = 0; e4 < 16; e4 += 4) {
+              const float4 l = *reinterpret_cast<const float4*>(ls + e4 * 2);
 #pragma unroll
               for (int i = 0; i < KS; ++i) {
-                const float w = __builtin_amdgcn_exp2f(fmaf(x[i][e], p.c, -l[e]));
-                const bool see = (r0 + r < rows) & here[i] &
-                                 row_sees(key[i], own, p.window, p.sinks);
-                sum[i] += see ? w : 0.f;
+                sum[i] += __builtin_amdgcn_exp2f(fmaf(x[i][e4], p.c, -l.x));
+                sum[i] += __builtin_amdgcn_exp2f(fmaf(x[i][e4 + 1], p.c, -l.y));
+                sum[i] += __builtin_amdgcn_exp2f(fmaf(x[i][e4 + 2], p.c, -l.z));
+                sum[i] += __builtin_amdgcn_exp2f(fmaf(x[i][e4 + 3], p.c, -l.w));
               }
+            }
+          } else {
+            const int* ms = &s_kmax[bf][rg * 32 + half * 4];
+#pragma unroll
+            for (int e4 = 0; e4 < 16; e4 += 4) {
+              const float4 l4 = *reinterpret_cast<const float4*>(ls + e4 * 2);
+              const int4 m4 = *reinterpret_cast<const int4*>(ms + e4 * 2);
+              const float l[4] = {l4.x, l4.y, l4.z, l4.w};
+              const int own[4] = {m4.x, m4.y, m4.z, m4.w};
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < KS; ++i) {
+                  const float w = __builtin_amdgcn_exp2f(fmaf(x[i][e4 + j], p.c, -l[j]));
+                  sum[i] += (unsigned)(own[j] - key[i]) <= reach[i] ? w : 0.f;
+                }
             }
           }
         }
