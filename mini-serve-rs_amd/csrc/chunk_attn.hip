@@ -95,7 +95,8 @@ struct ChunkParams {
   uint32_t stamp;
   float* thin_part;    // [2 * groups][kThinRows * (D + 2)]
   uint32_t* thin_done; // [groups]: pieces of the tile cut at a share's end
-  float4* wide_part;   // [2 * groups][wide_part_slots(D)]
+  float* wide_part;    // [2 * groups][wide_part_floats(D)]
+  uint32_t* wide_done; // [groups]: pieces of two-piece tiles left so far
   int Hq, Hkv, G, mbps, num_blocks, window, sinks;
   float c;             // scale * log2(e)
 };
@@ -296,7 +297,7 @@ __global__ __launch_bounds__(64 * W, 8 / W) void chunk_thin_kernel(ChunkParams p
                         : make_uint4(0, 0, 0, 0);
     }
   };
-  open(share.start, __builtin_amdgcn_readfirstlane(share.head),
+  open(share.at, __builtin_amdgcn_readfirstlane(share.head),
        __builtin_amdgcn_readfirstlane(share.u0));
 
   while (true) {
@@ -579,9 +580,9 @@ __global__ __launch_bounds__(64 * W, 8 / W) void chunk_thin_kernel(ChunkParams p
 }
 
 constexpr int kPartLanes = 2 * kWideRows;  // two lanes a row
-// float4 slots of a wide tile's partial state: the row's 4 D/32 of a lane, and
-// its (m, l).
-constexpr int wide_part_slots(int D) { return (D / 8 + 1) * kPartLanes; }
+// Floats of a wide tile's partial state: per lane 4 D/32 fours of its row, and
+// (m, l).
+constexpr int wide_part_floats(int D) { return (D / 8 + 1) * 4 * kPartLanes; }
 
 // The units (of kWidePages pages, 64 keys) of a wide tile whose keys some rows
 // all see: from lo to hi - 1, and the first `sunk` among the sinks. kmin: the
@@ -602,6 +603,104 @@ __device__ __forceinline__ UnitSpan unit_span(int kmin, int wlo, int wp0, int si
   s.hi = max(0, ((kmin + 1) >> 4) - wp0 + skip) / P;
   s.sunk = min(sinks / (16 * P), wp0 > 0 ? sink_pages / P : s.hi);
   return s;
+}
+
+// What becomes of a wide workgroup's piece of a tile: units to be joined with
+// others' before it (head) or after it (tail), or the whole tile. The lane
+// holds O^T rows d = 32 db + 8 (i/4) + 4 half + i%4 of its row (at `at` in q
+// and out), its max and its whole sum.
+//
+// A tile of two pieces is the end of one share and the start of the next. A
+// workgroup takes its share from the end, so the first piece is done early and
+// the second late: the second's workgroup finds the first waiting and joins it
+// from its registers. Nobody waits: a piece that finds no other is left in
+// memory and counted, and the one counted second joins. (The joined bits are
+// the same either way.) Pieces of a tile cut more than once are left for
+// chunk_merge_kernel, where several workgroups join each. Against a merge of
+// every cut tile in a launch of its own: attn_mixed 168 -> FILLME us.
+template <typename T, int D>
+__device__ __forceinline__ void wide_finish(const ChunkParams& p, const ChunkShare& share, int w,
+                                            bool head, bool tail, bool live, bool real, size_t at,
+                                            f32x16_t (&o)[D / 32], float m, float lsum) {
+  constexpr int DB = D / 32;
+  __shared__ int s_counted;
+  const int tid = threadIdx.x, half = (tid & 63) >> 5;
+  bool done = !head && !tail;
+  if (!done) {
+    const int first = head ? share.first : w;
+    const int pieces = head ? share.pieces : share.last - w + 1;
+    uint32_t* count = p.wide_done + first;
+    auto slot = [&](int of, bool tail_piece) {
+      return p.wide_part + (size_t)(2 * of + (tail_piece ? 1 : 0)) * wide_part_floats(D) + 4 * tid;
+    };
+    bool join = false;
+    if (pieces == 2 && head) {
+      if (tid == 0) s_counted = (int)ld_word(count);
+      __syncthreads();
+      join = s_counted == 1;
+      __syncthreads();
+    }
+    if (!join) {
+      // Slot k of thread tid: four floats, 1 KB of consecutive bytes a wave.
+      float* part = slot(w, !head);
+      if (live) {
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; i += 2)
+            st_pair(part + (d * 4 + i / 4) * 4 * kPartLanes + i % 4, o[d][i], o[d][i + 1]);
+        st_pair(part + 4 * DB * 4 * kPartLanes, m, lsum);
+      }
+      if (pieces == 2) {
+        wait_vm_stores();
+        __syncthreads();
+        if (tid == 0)
+          s_counted = (int)__hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED,
+                                                  __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        join = s_counted == 1;
+      }
+    }
+    if (join) {
+      if (tid == 0) st_word(count, 0u);
+      if (live) {
+        const float* part = head ? slot(first, true) : slot(w + 1, false);
+        float ml[2];
+        ld_pair(part + 4 * DB * 4 * kPartLanes, ml);
+        const float M = fmaxf(m, ml[0]);
+        // a: the first piece's weight, b: the second's.
+        const float mine = state_weight(m, M), other = state_weight(ml[0], M);
+        const float a = head ? other : mine, b = head ? mine : other;
+        auto joined = [&](float own, float read) __attribute__((always_inline)) {
+          return fmaf(head ? read : own, a, mul_rn(head ? own : read, b));
+        };
+        lsum = joined(lsum, ml[1]);
+        m = M;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            float x[2];
+            ld_pair(part + (d * 4 + i / 4) * 4 * kPartLanes + i % 4, x);
+            o[d][i] = joined(o[d][i], x[0]);
+            o[d][i + 1] = joined(o[d][i + 1], x[1]);
+          }
+      }
+      done = true;
+    }
+  }
+  if (done && real) {
+    T* dst = static_cast<T*>(p.out) + at * D;
+    const float inv = inverse_sum(lsum);
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int i4 = 0; i4 < 4; ++i4) {
+        const float v[4] = {o[d][i4 * 4], o[d][i4 * 4 + 1], o[d][i4 * 4 + 2], o[d][i4 * 4 + 3]};
+        write_row<T, 4>(dst + d * 32 + i4 * 8 + half * 4, v, inv);
+      }
+    if (p.lse && half == 0) p.lse[at] = state_lse(m, lsum);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -680,12 +779,12 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
   const int tr_g = lane >> 4, tr_j = (lane & 15) >> 2, tr_a = lane & 3;
   const int tr_row = (tr_g >> 1) * 4 + tr_j, tr_col = (tr_g & 1) * 16 + tr_a * 4;
 
-  int ti = __builtin_amdgcn_readfirstlane(share.tile);
-  int h = __builtin_amdgcn_readfirstlane(share.head);
-  int u0 = __builtin_amdgcn_readfirstlane(share.u0);
+  // The share's tiles from its last to its first (see wide_finish).
+  int ti = __builtin_amdgcn_readfirstlane(share.end_tile);
+  int h = __builtin_amdgcn_readfirstlane(share.end_head);
+  int u_end = __builtin_amdgcn_readfirstlane(share.end_u);
   int left = __builtin_amdgcn_readfirstlane(share.count);
-  bool head_piece = u0 > 0;
-  ChunkTile t = share.start;
+  ChunkTile t = share.at;
   while (left > 0) {
     const int n = __builtin_amdgcn_readfirstlane(t.n), off = __builtin_amdgcn_readfirstlane(t.off);
     const int tok0 = __builtin_amdgcn_readfirstlane(t.tok0);
@@ -695,7 +794,7 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
     const int* __restrict__ table =
         p.tables + (size_t)__builtin_amdgcn_readfirstlane(t.seq) * p.mbps;
     const int units = (pages + kWidePages - 1) / kWidePages;
-    const int seg = min(left, units - u0);
+    const int seg = min(left, u_end), u0 = u_end - seg;
     const int rows = n * G;
     const int last_row = min(rows, row0 + kWideRows) - 1;
     const int kend = off + last_row / G + 1;  // keys the tile's rows see end here
@@ -911,7 +1010,7 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
                 const uint16_t bits = (uint16_t)((i < 2 ? y.x : y.y) >> (16 * (i & 1)));
                 __builtin_memcpy(&e, &bits, 2);
                 const float v = Elem<T>::to_f32(e);
-                o[d][i4 * 4 + i] += see & !(v - v == 0.f) ? v : 0.f;
+                o[d][i4 * 4 + i] += (see & !(v - v == 0.f)) ? v : 0.f;
               }
               __builtin_amdgcn_sched_barrier(0);  // (else all loads' registers at once)
             }
@@ -927,7 +1026,6 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
     __syncthreads();  // the stages of the segment before are read
     if (tid < 2 * kWideBufs) s_odd[tid >> 1][tid & 1] = 0;
     __syncthreads();
-    const int u_end = u0 + seg;
     fetch_ids(u0);
     load(u0);
     store(0, whole_of(u0));
@@ -972,41 +1070,17 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
     }
     if (!behind) turn();
 
-    // Lane holds O^T rows d = 32 db + 8 (i/4) + 4 half + i%4 of its row.
-    const float lsum = l + __shfl_xor(l, 32, 64);
-    if (seg == units) {
-      if (wrow + col < rows) {
-        T* dst = static_cast<T*>(p.out) + at * D;
-        const float inv = inverse_sum(lsum);
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-          for (int i4 = 0; i4 < 4; ++i4) {
-            const float v[4] = {o[d][i4 * 4], o[d][i4 * 4 + 1], o[d][i4 * 4 + 2],
-                                o[d][i4 * 4 + 3]};
-            write_row<T, 4>(dst + d * 32 + i4 * 8 + half * 4, v, inv);
-          }
-        if (p.lse && half == 0) p.lse[at] = state_lse(m, lsum);
-      }
-    } else if (live) {
-      float4* part = p.wide_part +
-                     (size_t)(2 * w + (head_piece ? 0 : 1)) * wide_part_slots(D) + tid;
-#pragma unroll
-      for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int i4 = 0; i4 < 4; ++i4)
-          part[(d * 4 + i4) * kPartLanes] = make_float4(o[d][i4 * 4], o[d][i4 * 4 + 1],
-                                                        o[d][i4 * 4 + 2], o[d][i4 * 4 + 3]);
-      part[4 * DB * kPartLanes] = make_float4(m, lsum, 0.f, 0.f);
-    }
+    wide_finish<T, D>(p, share, w, u0 > 0, u_end < units, live, wrow + col < rows, at, o, m,
+                      l + __shfl_xor(l, 32, 64));
     left -= seg;
-    u0 = 0;
-    head_piece = false;
-    if (++ti == tiles) {
-      ti = 0;
-      ++h;
+    if (ti-- == 0) {
+      ti = tiles - 1;
+      --h;
     }
-    if (left > 0) t = p.v.wide[ti];
+    if (left > 0) {
+      t = p.v.wide[ti];
+      u_end = (__builtin_amdgcn_readfirstlane(t.pages) + kWidePages - 1) / kWidePages;
+    }
   }
 }
 
@@ -1062,12 +1136,12 @@ __global__ __launch_bounds__(kWide32Threads, 1) void chunk_wide32_kernel(ChunkPa
   const int voff = (kk0 & 15) * D * 4 + dc * 16;
   const int pg0 = __builtin_amdgcn_readfirstlane(kk0 >> 4);
 
-  int ti = __builtin_amdgcn_readfirstlane(share.tile);
-  int h = __builtin_amdgcn_readfirstlane(share.head);
-  int u0 = __builtin_amdgcn_readfirstlane(share.u0);
+  // The share's tiles from its last to its first (see wide_finish).
+  int ti = __builtin_amdgcn_readfirstlane(share.end_tile);
+  int h = __builtin_amdgcn_readfirstlane(share.end_head);
+  int u_end = __builtin_amdgcn_readfirstlane(share.end_u);
   int left = __builtin_amdgcn_readfirstlane(share.count);
-  bool head_piece = u0 > 0;
-  ChunkTile t = share.start;
+  ChunkTile t = share.at;
   while (left > 0) {
     const int n = __builtin_amdgcn_readfirstlane(t.n), off = __builtin_amdgcn_readfirstlane(t.off);
     const int tok0 = __builtin_amdgcn_readfirstlane(t.tok0);
@@ -1077,7 +1151,7 @@ __global__ __launch_bounds__(kWide32Threads, 1) void chunk_wide32_kernel(ChunkPa
     const int* __restrict__ table =
         p.tables + (size_t)__builtin_amdgcn_readfirstlane(t.seq) * p.mbps;
     const int units = (pages + kWidePages - 1) / kWidePages;
-    const int seg = min(left, units - u0);
+    const int seg = min(left, u_end), u0 = u_end - seg;
     const int rows = n * G;
     const int last_row = min(rows, row0 + kWideRows) - 1;
     const int kend = off + last_row / G + 1;  // keys the tile's rows see end here
@@ -1168,7 +1242,6 @@ __global__ __launch_bounds__(kWide32Threads, 1) void chunk_wide32_kernel(ChunkPa
     __syncthreads();  // the stages of the segment before are read
     if (tid < 4) s_odd[tid >> 1][tid & 1] = 0;
     __syncthreads();
-    const int u_end = u0 + seg;
     fetch_ids(u0);
     unsigned ok = load(u0), ok_next = 0;
     bool whole_t = ok == 15u && all.has(u0);
@@ -1270,54 +1343,30 @@ __global__ __launch_bounds__(kWide32Threads, 1) void chunk_wide32_kernel(ChunkPa
       bf ^= 1;
     }
 
-    // Lane holds O^T rows d = 32 db + 8 (i/4) + 4 half + i%4 of its row.
-    const float lsum = l + __shfl_xor(l, 32, 64);
-    if (seg == units) {
-      if (wrow + col < rows) {
-        float* dst = static_cast<float*>(p.out) + at * D;
-        const float inv = inverse_sum(lsum);
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-          for (int i4 = 0; i4 < 4; ++i4) {
-            const float v[4] = {o[d][i4 * 4], o[d][i4 * 4 + 1], o[d][i4 * 4 + 2],
-                                o[d][i4 * 4 + 3]};
-            write_row<float, 4>(dst + d * 32 + i4 * 8 + half * 4, v, inv);
-          }
-        if (p.lse && half == 0) p.lse[at] = state_lse(m, lsum);
-      }
-    } else if (live) {
-      float4* part = p.wide_part +
-                     (size_t)(2 * w + (head_piece ? 0 : 1)) * wide_part_slots(D) + tid;
-#pragma unroll
-      for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int i4 = 0; i4 < 4; ++i4)
-          part[(d * 4 + i4) * kPartLanes] = make_float4(o[d][i4 * 4], o[d][i4 * 4 + 1],
-                                                        o[d][i4 * 4 + 2], o[d][i4 * 4 + 3]);
-      part[4 * DB * kPartLanes] = make_float4(m, lsum, 0.f, 0.f);
-    }
+    wide_finish<float, D>(p, share, w, u0 > 0, u_end < units, live, wrow + col < rows, at, o, m,
+                          l + __shfl_xor(l, 32, 64));
     left -= seg;
-    u0 = 0;
-    head_piece = false;
-    if (++ti == tiles) {
-      ti = 0;
-      ++h;
+    if (ti-- == 0) {
+      ti = tiles - 1;
+      --h;
     }
-    if (left > 0) t = p.v.wide[ti];
+    if (left > 0) {
+      t = p.v.wide[ti];
+      u_end = (__builtin_amdgcn_readfirstlane(t.pages) + kWidePages - 1) / kWidePages;
+    }
   }
 }
 
-// Joins the pieces of the wide tiles that the shares cut: workgroup (w, d)
-// dimension block d of the tile that workgroup w's share ends in, if others
-// hold the rest of it. The pieces combine online in their order.
+// Joins the wide tiles that were cut into three pieces or more: workgroup (b, d)
+// dimension block d of the tile that workgroup b's share ends in, if it starts
+// there. The pieces combine online in their order.
 template <typename T, int D>
 __global__ __launch_bounds__(kPartLanes) void chunk_merge_kernel(ChunkParams p) {
   constexpr int DB = D / 32;
   if (p.v.head->stamp != p.stamp) return;
   const ChunkShare share = p.v.wide_share[blockIdx.x / DB];
   const int w = share.w, d = blockIdx.x % DB;
-  if (share.count == 0 || share.last == w) return;
+  if (share.count == 0 || share.last < w + 2) return;  // three pieces or more
   const ChunkTile t = p.v.wide[share.end_tile];
   const int h = share.end_head;
   const int tid = threadIdx.x;
@@ -1328,8 +1377,9 @@ __global__ __launch_bounds__(kPartLanes) void chunk_merge_kernel(ChunkParams p) 
 #pragma unroll
   for (int i = 0; i < 16; ++i) acc[i] = 0.f;
   for (int k = w; k <= share.last; ++k) {
-    const float4* part = p.wide_part +
-                         (size_t)(2 * k + (k == w ? 1 : 0)) * wide_part_slots(D) + tid;
+    const float4* part = reinterpret_cast<const float4*>(
+                             p.wide_part + (size_t)(2 * k + (k == w ? 1 : 0)) * wide_part_floats(D)) +
+                         tid;
     const float4 ml = part[4 * DB * kPartLanes];
     float4 a[4];
 #pragma unroll
@@ -1356,18 +1406,19 @@ __global__ __launch_bounds__(kPartLanes) void chunk_merge_kernel(ChunkParams p) 
 }
 
 // Workspace: header (word 0 unused by these kernels' errors, which the plan
-// holds), the thin tiles' piece counts, then the pieces.
+// holds), the tiles' piece counts, then the pieces.
 struct ChunkWorkspace {
-  size_t done, thin, wide, bytes;
+  size_t done, wide_done, thin, wide, bytes;
 };
 ChunkWorkspace chunk_workspace(int max_rows, int D, int cus) {
   ChunkWorkspace ws;
   ws.done = 256;
-  ws.thin = ws.done + ((size_t)2 * cus * sizeof(uint32_t) + 255) / 256 * 256;
+  ws.wide_done = ws.done + (size_t)2 * cus * sizeof(uint32_t);
+  ws.thin = ws.done + ((size_t)3 * cus * sizeof(uint32_t) + 255) / 256 * 256;
   ws.wide = ws.thin + (size_t)4 * cus * kThinRows * (D + 2) * sizeof(float);
   ws.bytes = ws.wide;
   if (max_rows > kThinRows)
-    ws.bytes += (size_t)2 * cus * wide_part_slots(D) * sizeof(float4);
+    ws.bytes += (size_t)2 * cus * wide_part_floats(D) * sizeof(float);
   return ws;
 }
 
@@ -1478,7 +1529,8 @@ extern "C" int rlse_chunk_attn(const void* q, const void* k_pool, const void* v_
                          max_blocks_per_seq, window, sinks, cus});
   p.thin_done = reinterpret_cast<uint32_t*>(base + ws.done);
   p.thin_part = reinterpret_cast<float*>(base + ws.thin);
-  p.wide_part = reinterpret_cast<float4*>(base + ws.wide);
+  p.wide_part = reinterpret_cast<float*>(base + ws.wide);
+  p.wide_done = reinterpret_cast<uint32_t*>(base + ws.wide_done);
   p.Hq = num_heads;
   p.Hkv = num_kv_heads;
   p.mbps = max_blocks_per_seq;

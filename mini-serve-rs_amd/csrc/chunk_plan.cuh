@@ -68,17 +68,17 @@ struct ChunkTile {
   int pages;     // virtual pages
 };
 
-// A workgroup's share of a list, number w: units u0 .. of (head, tile), count
-// in all (0: none), going on through the following tiles. The tile it starts
-// in is copied here, so that a workgroup's first loads all go out together.
-// first: the share that holds that tile's start, pieces: how many shares hold
-// some of it. The share ends in (end_head, end_tile), whose end share `last`
-// holds: w itself, too, where that tile started before the share (another
-// workgroup then joins its pieces).
+// A workgroup's share of a list, number w: units u0 .. of (head, tile) to unit
+// end_u - 1 of (end_head, end_tile), count in all (0: none). The tile it works
+// on first -- the thin kernels start at the share's start, the wide ones at its
+// end -- is copied here (`at`), so that a workgroup's first loads all go out
+// together. first: the share that holds the start tile's start, pieces: how
+// many shares hold some of that tile. last: the share that holds the end
+// tile's end; w itself, too, where that tile started before the share.
 struct ChunkShare {
   int w, head, u0, count, first, pieces, last, tile;
-  ChunkTile start;
-  int end_tile, end_head, pad[14];
+  ChunkTile at;
+  int end_tile, end_head, end_u, pad[13];
 };
 static_assert(sizeof(ChunkShare) == 128, "a share is a cache line");
 

@@ -67,8 +67,8 @@ __device__ __forceinline__ int tile_of(const int* held, const ChunkTile* a, int 
 constexpr int kMaxShares = 1024;
 template <typename I>
 __device__ void deal(const int* held, const ChunkTile* tiles, int n, int units, int Hkv,
-                     int max_groups, int min_units, int snap, bool whole, I* starts,
-                     ChunkShare* out) {
+                     int max_groups, int min_units, int snap, bool whole, bool from_end,
+                     I* starts, ChunkShare* out) {
   const I total = (I)units * Hkv;
   const I want = (total + min_units - 1) / min_units;
   const int groups = whole ? n * Hkv : (int)(want < (I)max_groups ? want : (I)max_groups);
@@ -106,7 +106,6 @@ __device__ void deal(const int* held, const ChunkTile* tiles, int n, int units, 
     s.head = (int)(from / units);
     const int u = (int)(from - (I)s.head * units);
     s.tile = tile_of(held, tiles, n, u);
-    s.start = tiles[s.tile];
     s.u0 = u - unit0(s.tile);
     s.count = (int)(to - from);
     s.first = s.u0 ? holder(from - s.u0) : s.w;
@@ -117,24 +116,26 @@ __device__ void deal(const int* held, const ChunkTile* tiles, int n, int units, 
     s.end_tile = tile_of(held, tiles, n, (int)(to - 1 - base));
     const I end = base + unit0(s.end_tile + 1);
     s.last = end > to && base + unit0(s.end_tile) >= from ? holder(end - 1) : s.w;
+    s.end_u = (int)(to - base - unit0(s.end_tile));
+    s.at = tiles[from_end ? s.end_tile : s.tile];
     out[b] = s;
   }
   __syncthreads();
 }
 __device__ void deal_shares(const int* held, const ChunkTile* tiles, int n, int units, int Hkv,
                             int max_groups, int min_units, int snap, bool whole,
-                            unsigned long long* starts, ChunkShare* out) {
+                            bool from_end, unsigned long long* starts, ChunkShare* out) {
   if (units == 0) {
     for (int b = threadIdx.x; b < max_groups; b += kPlanThreads) out[b].count = 0;
     return;
   }
   // (64-bit divisions take a few microseconds here.)
   if ((unsigned long long)units * Hkv * max_groups < (1ull << 31))
-    deal<unsigned>(held, tiles, n, units, Hkv, max_groups, min_units, snap, whole,
+    deal<unsigned>(held, tiles, n, units, Hkv, max_groups, min_units, snap, whole, from_end,
                    reinterpret_cast<unsigned*>(starts), out);
   else
-    deal<unsigned long long>(held, tiles, n, units, Hkv, max_groups, min_units, snap, whole, starts,
-                             out);
+    deal<unsigned long long>(held, tiles, n, units, Hkv, max_groups, min_units, snap, whole,
+                             from_end, starts, out);
 }
 
 __global__ __launch_bounds__(kPlanThreads) void chunk_plan_kernel(PlanParams p) {
@@ -235,9 +236,9 @@ __global__ __launch_bounds__(kPlanThreads) void chunk_plan_kernel(PlanParams p) 
 
   deal_shares(s_thin, p.v.thin, thin_tiles, thin_units, p.Hkv, p.thin_groups, kThinMinUnits,
               kThinSnap, (long long)thin_tiles * p.Hkv <= p.thin_groups && s_longest <= kThinWhole,
-              s_starts, p.v.thin_share);
+              false, s_starts, p.v.thin_share);
   deal_shares(s_unit, p.v.wide, wide_tiles, wide_units, p.Hkv, p.cus, kWideMinUnits, kWideSnap,
-              false, s_starts, p.v.wide_share);
+              false, true, s_starts, p.v.wide_share);
   if (tid == 0) {
     ChunkHead h;
     h.flags = s_flags;

@@ -129,7 +129,7 @@ __global__ __launch_bounds__(64 * W) void score_thin_kernel(ScoreParams p) {
   int h = __builtin_amdgcn_readfirstlane(share.head);
   int u0 = __builtin_amdgcn_readfirstlane(share.u0);
   int left = __builtin_amdgcn_readfirstlane(share.count);
-  ChunkTile t = share.start;
+  ChunkTile t = share.at;
   while (left > 0) {
     const int n = __builtin_amdgcn_readfirstlane(t.n), off = __builtin_amdgcn_readfirstlane(t.off);
     const int tok0 = __builtin_amdgcn_readfirstlane(t.tok0);
