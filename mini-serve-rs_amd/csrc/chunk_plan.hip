@@ -23,27 +23,38 @@ struct PlanParams {
   int wide_cap;
 };
 
-// Exclusive prefix of x over the workgroup, and its sum (s_w: kPlanWaves ints).
-__device__ __forceinline__ int block_scan(int x, int* s_w, int* sum) {
+// Exclusive prefixes of the N values x over the workgroup, and their sums
+// (s_w: kPlanWaves * N ints). (One pass for all: the round trips count here.)
+template <int N>
+__device__ __forceinline__ void block_scan(int (&x)[N], int (*s_w)[N], int (&sum)[N]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int inc = x;
+  int inc[N];
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(inc, o, 64);
-    if (lane >= o) inc += y;
-  }
-  __syncthreads();
-  if (lane == 63) s_w[wave] = inc;
-  __syncthreads();
-  int before = 0, all = 0;
+  for (int i = 0; i < N; ++i) inc[i] = x[i];
 #pragma unroll
-  for (int i = 0; i < kPlanWaves; ++i) {
-    const int s = s_w[i];
-    before += i < wave ? s : 0;
-    all += s;
+  for (int o = 1; o < 64; o <<= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int y = __shfl_up(inc[i], o, 64);
+      if (lane >= o) inc[i] += y;
+    }
+  __syncthreads();
+  if (lane == 63)
+#pragma unroll
+    for (int i = 0; i < N; ++i) s_w[wave][i] = inc[i];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    int before = 0, all = 0;
+#pragma unroll
+    for (int k = 0; k < kPlanWaves; ++k) {
+      const int s = s_w[k][i];
+      before += k < wave ? s : 0;
+      all += s;
+    }
+    sum[i] = all;
+    x[i] = before + inc[i] - x[i];
   }
-  *sum = all;
-  return before + inc - x;
 }
 
 // Last index i of a[0..n) with a[i] <= u (a[0] = 0). The first kHeld prefixes
@@ -58,29 +69,44 @@ __device__ __forceinline__ int tile_of(const int* held, const ChunkTile* a, int 
   return lo;
 }
 
-// Shares of `units` units of each of Hkv heads over at most max_groups
-// workgroups of at least min_units each: equal shares, but a boundary within
+// A list's shares: `units` units of each of Hkv heads over at most max_groups
+// workgroups of at least min_units each, equal shares, but a boundary within
 // snap units of a tile's moves there, and with `whole` (n * Hkv <= max_groups)
-// each gets one tile. (A tile cut
-// for the sake of a few units costs more than they do.) I: an integer type that holds units * Hkv *
-// max_groups; starts: max_groups + 1 of them in LDS.
+// each gets one tile. (A tile cut for the sake of a few units costs more than
+// they do.) Worked out by kDealThreads threads, t among them; starts:
+// max_groups + 1 numbers in LDS. I: an integer type that holds units * Hkv *
+// max_groups.
 constexpr int kMaxShares = 1024;
+constexpr int kDealThreads = kPlanThreads / 2;
+struct DealList {
+  const int* held;
+  const ChunkTile* tiles;
+  int n, units, max_groups, min_units, snap;
+  bool whole, from_end;
+  ChunkShare* out;
+  __device__ int unit0(int i) const {
+    return i < n ? (i < kHeld ? held[i] : tiles[i].unit0) : units;
+  }
+};
 template <typename I>
-__device__ void deal(const int* held, const ChunkTile* tiles, int n, int units, int Hkv,
-                     int max_groups, int min_units, int snap, bool whole, bool from_end,
-                     I* starts, ChunkShare* out) {
-  const I total = (I)units * Hkv;
-  const I want = (total + min_units - 1) / min_units;
-  const int groups = whole ? n * Hkv : (int)(want < (I)max_groups ? want : (I)max_groups);
-  auto unit0 = [&](int i) { return i < n ? (i < kHeld ? held[i] : tiles[i].unit0) : units; };
-  snap = min((I)snap, total / (4 * groups));
-  for (int w = threadIdx.x; w <= groups; w += kPlanThreads) {
+__device__ int deal_groups(const DealList& d, int Hkv) {
+  if (d.whole) return d.n * Hkv;
+  const I want = ((I)d.units * Hkv + d.min_units - 1) / d.min_units;
+  return (int)(want < (I)d.max_groups ? want : (I)d.max_groups);
+}
+template <typename I>
+__device__ void deal_starts(const DealList& d, int Hkv, int t, I* starts) {
+  const I total = (I)d.units * Hkv;
+  if (total == 0) return;
+  const int groups = deal_groups<I>(d, Hkv);
+  const int snap = (int)min((I)d.snap, total / (4 * groups));
+  for (int w = t; w <= groups; w += kDealThreads) {
     I x = total * w / groups;
-    if (whole) {
-      x = w < groups ? (I)(w / n) * units + unit0(w % n) : total;
+    if (d.whole) {
+      x = w < groups ? (I)(w / d.n) * d.units + d.unit0(w % d.n) : total;
     } else if (w > 0 && w < groups) {
-      const int head = (int)(x / units), u = (int)(x - (I)head * units);
-      const int i = tile_of(held, tiles, n, u), lo = unit0(i), hi = unit0(i + 1);
+      const int head = (int)(x / d.units), u = (int)(x - (I)head * d.units);
+      const int i = tile_of(d.held, d.tiles, d.n, u), lo = d.unit0(i), hi = d.unit0(i + 1);
       if (u - lo <= snap)
         x -= u - lo;
       else if (hi - u <= snap)
@@ -88,61 +114,50 @@ __device__ void deal(const int* held, const ChunkTile* tiles, int n, int units, 
     }
     starts[w] = x;
   }
-  __syncthreads();
-  for (int b = threadIdx.x; b < max_groups; b += kPlanThreads) {
+}
+template <typename I>
+__device__ void deal_shares(const DealList& d, int Hkv, int t, const I* starts) {
+  const I total = (I)d.units * Hkv;
+  const int groups = total ? deal_groups<I>(d, Hkv) : 0;
+  for (int b = t; b < d.max_groups; b += kDealThreads) {
     if (b >= groups) {
-      out[b].count = 0;
+      d.out[b].count = 0;
       continue;
     }
     ChunkShare s;
     s.w = share_index(b, groups);
     const I from = starts[s.w], to = starts[s.w + 1];
+    const int units = d.units;
+    s.head = (int)(from / units);
+    const int u = (int)(from - (I)s.head * units);
+    s.tile = tile_of(d.held, d.tiles, d.n, u);
+    s.end_head = (int)((to - 1) / units);
+    const I base = (I)s.end_head * units;
+    s.end_tile = tile_of(d.held, d.tiles, d.n, (int)(to - 1 - base));
+    s.at = d.tiles[d.from_end ? s.end_tile : s.tile];
     auto holder = [&](I x) {  // the share that has unit x
-      int w = (int)(x * groups / total);
+      int w = d.whole ? s.w : (int)(x * groups / total);
       while (starts[w] > x) --w;
       while (starts[w + 1] <= x) ++w;
       return w;
     };
-    s.head = (int)(from / units);
-    const int u = (int)(from - (I)s.head * units);
-    s.tile = tile_of(held, tiles, n, u);
-    s.u0 = u - unit0(s.tile);
+    s.u0 = u - d.unit0(s.tile);
     s.count = (int)(to - from);
     s.first = s.u0 ? holder(from - s.u0) : s.w;
-    const I tile_end = from - s.u0 + (unit0(s.tile + 1) - unit0(s.tile));
+    const I tile_end = from - s.u0 + (d.unit0(s.tile + 1) - d.unit0(s.tile));
     s.pieces = (tile_end > to ? holder(tile_end - 1) : s.w) - s.first + 1;
-    s.end_head = (int)((to - 1) / units);
-    const I base = (I)s.end_head * units;
-    s.end_tile = tile_of(held, tiles, n, (int)(to - 1 - base));
-    const I end = base + unit0(s.end_tile + 1);
-    s.last = end > to && base + unit0(s.end_tile) >= from ? holder(end - 1) : s.w;
-    s.end_u = (int)(to - base - unit0(s.end_tile));
-    s.at = tiles[from_end ? s.end_tile : s.tile];
-    out[b] = s;
+    const I end = base + d.unit0(s.end_tile + 1);
+    s.last = end > to && base + d.unit0(s.end_tile) >= from ? holder(end - 1) : s.w;
+    s.end_u = (int)(to - base - d.unit0(s.end_tile));
+    d.out[b] = s;
   }
-  __syncthreads();
-}
-__device__ void deal_shares(const int* held, const ChunkTile* tiles, int n, int units, int Hkv,
-                            int max_groups, int min_units, int snap, bool whole,
-                            bool from_end, unsigned long long* starts, ChunkShare* out) {
-  if (units == 0) {
-    for (int b = threadIdx.x; b < max_groups; b += kPlanThreads) out[b].count = 0;
-    return;
-  }
-  // (64-bit divisions take a few microseconds here.)
-  if ((unsigned long long)units * Hkv * max_groups < (1ull << 31))
-    deal<unsigned>(held, tiles, n, units, Hkv, max_groups, min_units, snap, whole, from_end,
-                   reinterpret_cast<unsigned*>(starts), out);
-  else
-    deal<unsigned long long>(held, tiles, n, units, Hkv, max_groups, min_units, snap, whole,
-                             from_end, starts, out);
 }
 
 __global__ __launch_bounds__(kPlanThreads) void chunk_plan_kernel(PlanParams p) {
   __shared__ int s_wide[kMaxChunkSeqs + 1];  // wide tiles before each sequence
-  __shared__ int s_w[kPlanWaves];
+  __shared__ int s_w[kPlanWaves][5], s_w1[kPlanWaves][1];
   __shared__ int s_thin[kHeld], s_unit[kHeld];  // unit0 of the thin and the wide tiles
-  __shared__ unsigned long long s_starts[kMaxShares + 1];
+  __shared__ unsigned long long s_starts[2][kMaxShares + 1];
   __shared__ unsigned s_flags;
   __shared__ int s_longest;  // pages of the longest thin tile
   const int tid = threadIdx.x;
@@ -176,28 +191,26 @@ __global__ __launch_bounds__(kPlanThreads) void chunk_plan_kernel(PlanParams p) 
         blocks = wide ? (t.pages + kScorePages - 1) / kScorePages : 0;
       }
     }
-    int sum;
-    int at = block_scan(thin, s_w, &sum) + thin_tiles;
-    thin_tiles += sum;
-    int u = block_scan(thin ? t.pages : 0, s_w, &sum) + thin_units;
-    thin_units += sum;
+    int x[5] = {thin, thin ? t.pages : 0, wide, blocks, tiles}, sum[5];
+    block_scan(x, s_w, sum);
     if (thin) {
-      t.unit0 = u;
+      const int at = x[0] + thin_tiles;
+      t.unit0 = x[1] + thin_units;
       p.v.thin[at] = t;
-      if (at < kHeld) s_thin[at] = u;
+      if (at < kHeld) s_thin[at] = t.unit0;
       atomicMax(&s_longest, t.pages);
     }
-    at = block_scan(wide, s_w, &sum) + score_seqs;
-    score_seqs += sum;
-    u = block_scan(blocks, s_w, &sum) + score_units;
-    score_units += sum;
     if (wide) {
-      t.unit0 = u;
+      const int at = x[2] + score_seqs;
+      t.unit0 = x[3] + score_units;
       p.v.score[at] = t;
+      s_wide[at] = x[4] + wide_tiles;
     }
-    const int w0 = block_scan(tiles, s_w, &sum) + wide_tiles;
-    wide_tiles += sum;
-    if (wide) s_wide[at] = w0;
+    thin_tiles += sum[0];
+    thin_units += sum[1];
+    score_seqs += sum[2];
+    score_units += sum[3];
+    wide_tiles += sum[4];
   }
   if (wide_tiles > p.wide_cap) {  // cu_tokens overlap
     wide_tiles = p.wide_cap;
@@ -224,9 +237,10 @@ __global__ __launch_bounds__(kPlanThreads) void chunk_plan_kernel(PlanParams p) 
       tile_pages(t.off, t.row0 / p.G, last / p.G, p.window, p.sinks, &t.wp0, &t.pages);
       units = (t.pages + kWidePages - 1) / kWidePages;
     }
-    int sum;
-    t.unit0 = block_scan(units, s_w, &sum) + wide_units;
-    wide_units += sum;
+    int x[1] = {units}, sum[1];
+    block_scan(x, s_w1, sum);
+    t.unit0 = x[0] + wide_units;
+    wide_units += sum[0];
     if (i < wide_tiles) {
       p.v.wide[i] = t;
       if (i < kHeld) s_unit[i] = t.unit0;
@@ -234,11 +248,32 @@ __global__ __launch_bounds__(kPlanThreads) void chunk_plan_kernel(PlanParams p) 
   }
   __syncthreads();
 
-  deal_shares(s_thin, p.v.thin, thin_tiles, thin_units, p.Hkv, p.thin_groups, kThinMinUnits,
-              kThinSnap, (long long)thin_tiles * p.Hkv <= p.thin_groups && s_longest <= kThinWhole,
-              false, s_starts, p.v.thin_share);
-  deal_shares(s_unit, p.v.wide, wide_tiles, wide_units, p.Hkv, p.cus, kWideMinUnits, kWideSnap,
-              false, true, s_starts, p.v.wide_share);
+  // The thin list's shares by the first half of the threads, the wide one's
+  // by the second.
+  const bool second = tid >= kDealThreads;
+  DealList d;
+  d.held = second ? s_unit : s_thin;
+  d.tiles = second ? p.v.wide : p.v.thin;
+  d.n = second ? wide_tiles : thin_tiles;
+  d.units = second ? wide_units : thin_units;
+  d.max_groups = second ? p.cus : p.thin_groups;
+  d.min_units = second ? kWideMinUnits : kThinMinUnits;
+  d.snap = second ? kWideSnap : kThinSnap;
+  d.whole = !second && (long long)thin_tiles * p.Hkv <= p.thin_groups && s_longest <= kThinWhole;
+  d.from_end = second;
+  d.out = second ? p.v.wide_share : p.v.thin_share;
+  const int t = tid & (kDealThreads - 1);
+  unsigned long long* starts = s_starts[second];
+  // (64-bit divisions take a few microseconds here.)
+  if ((unsigned long long)max(thin_units, wide_units) * p.Hkv * p.thin_groups < (1ull << 31)) {
+    deal_starts(d, p.Hkv, t, reinterpret_cast<unsigned*>(starts));
+    __syncthreads();
+    deal_shares(d, p.Hkv, t, reinterpret_cast<const unsigned*>(starts));
+  } else {
+    deal_starts(d, p.Hkv, t, starts);
+    __syncthreads();
+    deal_shares(d, p.Hkv, t, static_cast<const unsigned long long*>(starts));
+  }
   if (tid == 0) {
     ChunkHead h;
     h.flags = s_flags;
