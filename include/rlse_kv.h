@@ -418,7 +418,8 @@ int rlse_prefill_attn(const void* q, const void* k_pool, const void* v_pool,
 /* given them back). Rows of q and out outside every sequence are left   */
 /* as they were.                                                         */
 /*                                                                      */
-/* num_seqs <= 4096; total_tokens: rows of q at least cu_tokens[num_seqs]; */
+/* num_seqs <= 4096, max_blocks_per_seq <= 2^17 (2 M tokens), total_tokens * */
+/* num_heads < 2^23; total_tokens: rows of q, at least cu_tokens[num_seqs]; */
 /* max_tokens: the most new tokens of a sequence, or a bound on it (1 for */
 /* a decode step). A sequence with more, or with seq_lens below its new  */
 /* tokens or above max_blocks_per_seq*16, or with offsets that descend or */
@@ -442,7 +443,7 @@ int rlse_chunk_plan(const int32_t* cu_tokens, const int32_t* seq_lens, int num_s
  * the logarithm of the sum of e^(scale q.k) over them. A row that sees no key
  * (its pages' ids are all outside [0, num_blocks)) gives zeros and -inf.
  * Scores that are NaN, and infinite or NaN values of a visible key, reach
- * the rows that see it and no others. f32, bf16 or f16, head_dim 64 or 128,
+ * the rows that see it and no others. out overlaps no other buffer. f32, bf16 or f16, head_dim 64 or 128,
  * groups of up to 256 heads; q, out and pools 16-byte aligned. workspace:
  * rlse_chunk_workspace_size bytes (grows with none of the lengths), 16-byte
  * aligned, zero-filled once before its first use and then left to the
@@ -494,7 +495,7 @@ int rlse_kv_scores(const void* q, const void* k_pool, const int32_t* block_table
  * l*layer_stride_elems), their weights to new_scores (same layout as scores,
  * not overlapping it), their old slots to keep [num_layers][num_seqs]
  * [num_kv_heads][budget] (int32; -1 behind the last), and new_lens[b] =
- * min(seq_lens[b], budget). RoPE stays as it was applied: a caller gives new
+ * min(seq_lens[b], budget) (not overlapping seq_lens). RoPE stays as it was applied: a caller gives new
  * tokens their true positions (rlse_rope) and appends them at the new slots
  * (rlse_kv_append).
  * Nothing the call reads is written, so pages shared by several sequences or

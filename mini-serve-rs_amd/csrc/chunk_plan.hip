@@ -305,8 +305,10 @@ int validate_chunk_shape(const char* what, int num_seqs, int total_tokens, int m
     return fail(RLSE_ERR_INVALID_VALUE, "%s: group size %d above %d", what, Hq / Hkv, kMaxGroup);
   if ((long long)total_tokens * Hq > 0x7fffffffLL / 256)
     return fail(RLSE_ERR_INVALID_VALUE, "%s: total_tokens * num_heads too large", what);
-  if (mbps <= 0 || mbps > (1 << 24))
-    return fail(RLSE_ERR_INVALID_VALUE, "%s: max_blocks_per_seq %d outside 1..2^24", what, mbps);
+  // (A list's units, at most 2^15 + num_seqs wide tiles of a quarter of the
+  // pages each, are counted in 31 bits.)
+  if (mbps <= 0 || mbps > (1 << 17))
+    return fail(RLSE_ERR_INVALID_VALUE, "%s: max_blocks_per_seq %d outside 1..2^17", what, mbps);
   if ((long long)mbps * num_seqs > 0x7fffffffLL)
     return fail(RLSE_ERR_INVALID_VALUE, "%s: num_seqs * max_blocks_per_seq too large", what);
   if (window < 0 || sinks < 0 || sinks > (1 << 28))

@@ -22,6 +22,12 @@ int launch_status(const char* what);
 // Compute-unit count of the current device (cached per device).
 int device_cu_count(int* cus);
 
+// Whether [a, a + an) and [b, b + bn) share a byte.
+inline bool overlap(const void* a, size_t an, const void* b, size_t bn) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y ? y - x < an : x - y < bn;
+}
+
 inline hipStream_t as_stream(rlse_stream_t s) { return reinterpret_cast<hipStream_t>(s); }
 
 // Current bound on a cross-workgroup merge's wait, in 100 MHz wall-clock

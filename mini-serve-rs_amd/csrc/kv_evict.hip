@@ -288,8 +288,12 @@ extern "C" int rlse_kv_evict(void* k_pool, void* v_pool, long long layer_stride_
   if (!k_pool || !v_pool || !block_tables || !seq_lens || !scores || !new_tables || !new_lens ||
       !new_scores || !keep)
     return fail(RLSE_ERR_INVALID_VALUE, "kv_evict: null pointer argument");
-  if (scores == new_scores)
-    return fail(RLSE_ERR_INVALID_VALUE, "kv_evict: new_scores is scores");
+  const size_t sbytes =
+      (num_layers > 1 ? (size_t)(num_layers - 1) * score_layer_stride + row : (size_t)row) * 4;
+  if (overlap(scores, sbytes, new_scores, sbytes))
+    return fail(RLSE_ERR_INVALID_VALUE, "kv_evict: new_scores overlaps scores");
+  if (overlap(seq_lens, (size_t)num_seqs * 4, new_lens, (size_t)num_seqs * 4))
+    return fail(RLSE_ERR_INVALID_VALUE, "kv_evict: new_lens overlaps seq_lens");
   if ((reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(v_pool)) & 15)
     return fail(RLSE_ERR_INVALID_VALUE, "kv_evict: a pool is not 16-byte aligned");
   EvictParams p{};

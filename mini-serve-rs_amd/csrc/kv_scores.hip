@@ -107,10 +107,10 @@ __device__ __forceinline__ float had(const ScoreParams& p, size_t row, int k, in
   return p.prev && k < off ? p.prev[row + k] : 0.f;
 }
 
-
 template <typename T, int D, int RT, int W, bool STREAM>
 __global__ __launch_bounds__(64 * W) void score_thin_kernel(ScoreParams p) {
   constexpr int ES = (int)sizeof(T), N = D * ES / 64;
+  // Pages in registers: one at work, the others in flight.
   constexpr int NBUF = 4;
   if (p.v.head->stamp != p.stamp) {
     if (blockIdx.x == 0 && threadIdx.x == 0) ws_raise(&p.v.head->flags, RLSE_WS_ERR_PLAN);
@@ -156,22 +156,22 @@ __global__ __launch_bounds__(64 * W) void score_thin_kernel(ScoreParams p) {
     };
     fetch_ids(0);
 
-    // Queries in the A-operand layout (lane l: row l % 16), and the rows of
-    // this lane's accumulator elements: row 4 (l / 16) + i.
+    // Queries in the A-operand layout (lane l: row l % 16; past the last row
+    // that row again, for zeros times an infinite key are NaN), and the rows of
+    // this lane's accumulator elements: row 4 (l / 16) + i, of no weight (lse
+    // +inf) past the last.
     uint4 q[RT][N];
     float lse[RT][4];
     int kmax[RT][4];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       {
-        const int row = rt * 16 + col;
-        const bool real = row < rows;
-        const int tok = real ? row / G : 0, g = real ? row - tok * G : 0;
+        const int row = min(rt * 16 + col, rows - 1);
+        const int tok = row / G, g = row - tok * G;
         const T* src = qb + ((size_t)(tok0 + tok) * Hq + h * G + g) * D + quad * (16 / ES);
 #pragma unroll
         for (int r = 0; r < N; ++r)
-          q[rt][r] = real ? *reinterpret_cast<const uint4*>(src + r * (64 / ES))
-                          : make_uint4(0, 0, 0, 0);
+          q[rt][r] = *reinterpret_cast<const uint4*>(src + r * (64 / ES));
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -432,7 +432,7 @@ __global__ __launch_bounds__(kWideThreads, 3) void score_wide_kernel(ScoreParams
           const bool whole = valid && last_key <= kmax_lo && last_key < kend && rb == ra + 31 &&
                              (p.window <= 0 || first_key > kmax_hi - p.window ||
                               last_key < p.sinks);
-// Accumulator element e is row 8 (e/4) + 4 half + e%4 of the 32.
+          // Accumulator element e is row 8 (e/4) + 4 half + e%4 of the 32.
           const float* ls = &s_lse[bf][rg * 32 + half * 4];
           if (whole) {
 #pragma unroll
@@ -549,6 +549,9 @@ extern "C" int rlse_kv_scores(const void* q, const void* k_pool, const int32_t* 
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_pool) |
        reinterpret_cast<uintptr_t>(plan)) & 15)
     return fail(RLSE_ERR_INVALID_VALUE, "kv_scores: a buffer is not 16-byte aligned");
+  const size_t floats = (size_t)num_seqs * num_kv_heads * max_blocks_per_seq * 16;
+  if (prev && prev != scores && overlap(prev, floats * 4, scores, floats * 4))
+    return fail(RLSE_ERR_INVALID_VALUE, "kv_scores: prev overlaps scores and is not scores");
   int cus = 0;
   st = device_cu_count(&cus);
   if (st) return st;

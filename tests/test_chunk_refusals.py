@@ -18,8 +18,8 @@ def _attn(kv, ptr=16, **a):
 
 
 SHAPES = [dict(n=0), dict(n=4097), dict(total=0), dict(most=0), dict(most=11), dict(hq=12),
-          dict(hq=0), dict(hkv=0), dict(mbps=0), dict(mbps=1 << 25), dict(window=-1),
-          dict(sinks=-1), dict(total=1 << 24, hq=64), dict(hq=514, hkv=2)]
+          dict(hq=0), dict(hkv=0), dict(mbps=0), dict(mbps=1 << 25), dict(mbps=(1 << 17) + 1),
+          dict(window=-1), dict(sinks=-1), dict(total=1 << 24, hq=64), dict(hq=514, hkv=2)]
 
 
 @pytest.mark.parametrize("change", SHAPES, ids=str)
@@ -53,7 +53,7 @@ def test_pointers(kv):
 
 
 def _scores(kv, ptr=16, **a):
-    return kv.load().rlse_kv_scores(ptr, 16, 16, 16, 16, None, 16, a["n"], a["total"], a["most"],
+    return kv.load().rlse_kv_scores(ptr, 16, 16, 16, 16, a.get("prev"), 4096, a["n"], a["total"], a["most"],
                                     a["hq"], a["hkv"], a["d"], a["mbps"], a["nb"], a["window"],
                                     a["sinks"], a["scale"], a["dtype"],
                                     a.get("flags", 0), None)
@@ -73,13 +73,14 @@ def test_score_pointers(kv):
     assert "aligned" in kv.last_error()
 
 
-EVICT = dict(k=16, stride=64 * 8 * 16 * 128, layers=2, scores=16, sstride=2 * 8 * 128, new=32,
+EVICT = dict(k=16, stride=64 * 8 * 16 * 128, layers=2, scores=16, sstride=2 * 8 * 128,
+             new=1 << 20, lens=16, nlens=24,
              n=2, hkv=8, d=128, mbps=8, nbps=2, nb=64, budget=20, sinks=2, recent=3, dtype=1)
 
 
 def _evict(kv, **a):
-    return kv.load().rlse_kv_evict(a["k"], 16, a["stride"], a["layers"], 16, 16, a["scores"],
-                                   a["sstride"], 16, 16, a["new"], 16, a["n"], a["hkv"], a["d"],
+    return kv.load().rlse_kv_evict(a["k"], 16, a["stride"], a["layers"], 16, a["lens"],
+                                   a["scores"], a["sstride"], 16, a["nlens"], a["new"], 16, a["n"], a["hkv"], a["d"],
                                    a["mbps"], a["nbps"], a["nb"], a["budget"], a["sinks"],
                                    a["recent"], a["dtype"], None)
 
@@ -89,7 +90,22 @@ def _evict(kv, **a):
     dict(budget=0), dict(budget=33), dict(budget=129, nbps=20), dict(sinks=-1), dict(recent=-1),
     dict(sinks=18), dict(dtype=5), dict(sstride=2047), dict(stride=64 * 8 * 16 * 128 - 1),
     dict(stride=64 * 8 * 16 * 128 + 1), dict(k=None), dict(k=24), dict(new=16),
+    dict(new=16 + 2 * 2 * 8 * 128 * 4 - 4), dict(scores=(1 << 20) + 64), dict(nlens=16),
+    dict(nlens=20), dict(lens=28),
     dict(layers=1 << 20, n=4096, sstride=1 << 40)], ids=str)
 def test_evict_arguments(kv, change):
     assert _evict(kv, **{**EVICT, **change}) == kv.ERR_INVALID_VALUE
     assert "kv_evict" in kv.last_error()
+
+
+def test_overlaps_name_their_reason(kv):
+    for change in (dict(new=16), dict(new=16 + 2 * 2 * 8 * 128 * 4 - 4),
+                   dict(scores=(1 << 20) + 64)):
+        _evict(kv, **{**EVICT, **change})
+        assert "new_scores overlaps" in kv.last_error()
+    for change in (dict(nlens=16), dict(nlens=20), dict(lens=28)):
+        _evict(kv, **{**EVICT, **change})
+        assert "new_lens overlaps" in kv.last_error()
+    for prev in (4092, 4100, 4096 + 4 * GOOD["n"] * GOOD["hkv"] * GOOD["mbps"] * 16 - 4):
+        assert _scores(kv, **{**GOOD, "prev": prev}) == kv.ERR_INVALID_VALUE
+        assert "prev overlaps" in kv.last_error()

@@ -162,3 +162,54 @@ def test_pool_offsets_past_32_bits(kv):
     for b in range(2):
         n = step.lens[b]
         assert_within(got[b, :, :n], want[b, :, :n], tol[b, :, :n], f"sequence {b}")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("new", [1, 3, 70])
+def test_key_of_score_minus_infinity(kv, new, dtype):
+    """A visible key whose score is -inf in every row has no weight, and the
+    others theirs."""
+    step = Step(39, dtype, (6, 2, 64), [new, new], [200, 75])
+    step.q[..., 7] = 1.0
+    for b, at in ((0, 3), (0, 37), (1, 70)):
+        step.k[step.tables[b, at // 16], :, at % 16, 7] = -math.inf
+    want_lse = torch.zeros(step.total, 6)
+    for b in range(2):
+        rows = slice(step.cu[b], step.cu[b + 1])
+        for j in range(6):
+            s = step.q[rows, j].double() @ step.keys(step.k, b, j // 3).T * step.scale
+            want_lse[rows, j] = s.masked_fill(~step.visible(b), -math.inf).logsumexp(-1).float()
+    step.upload().plan(kv)
+    got = scores(kv, step, want_lse.to(DEV)).cpu()
+    for b, at in ((0, 3), (0, 37), (1, 70)):
+        assert (got[b, :, at] == 0).all()
+        step.k[step.tables[b, at // 16], :, at % 16, 7] = -1e4 if dtype != "f32" else -1e5
+    want, tol = step_scores(step, want_lse)
+    for b in range(2):
+        n = step.lens[b]
+        keys = torch.isfinite(step.keys(step.k, b, 0)).all(-1)
+        assert keys.all()
+        assert_within(got[b, :, :n], want[b, :, :n], tol[b, :, :n], f"sequence {b}")
+
+
+def test_flag_for_shared_pages(kv):
+    step = Step(40, "bf16", (16, 8, 128), [1, 2, 40], [300, 310, 320])
+    step.tables[1:, :18] = step.tables[0, :18]
+    step.upload().plan(kv)
+    _, lse = step.run(kv)
+    got, d = scores(kv, step, lse), step.dev
+    other = torch.full_like(got, 7.0)
+    kv.kv_scores(d["q"], d["k"], d["tables"], d["plan"], lse, None, other, *step.shape(),
+                 shared_pages=True)
+    assert torch.equal(got, other)
+    want, tol = step_scores(step, lse.cpu())
+    for b in range(3):
+        n = step.lens[b]
+        assert_within(got[b, :, :n], want[b, :, :n], tol[b, :, :n], f"sequence {b}")
+
+
+def test_many_sequences(kv):
+    """More sequences than workgroups."""
+    step = Step(41, "bf16", (4, 2, 64), [i % 3 for i in range(700)],
+                [(i * 37) % 90 for i in range(700)])
+    check(kv, step, "many")
