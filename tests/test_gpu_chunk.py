@@ -347,3 +347,73 @@ def test_refuses_a_small_workspace(kv):
     with pytest.raises(kv.RlseError, match="plan"):
         kv.chunk_plan(step.dev["cu"], step.dev["lens"], step.n, step.total, step.most, step.hq,
                       step.hkv, step.mbps, 0, 0, small, small.numel())
+
+
+def test_flag_for_shared_pages(kv):
+    """Sequences forked from one prefix; the flag changes no bit."""
+    step = Step(22, "bf16", (16, 8, 128), [1, 1, 4, 50], [200, 210, 220, 230])
+    step.tables[1:, :12] = step.tables[0, :12]
+    step.upload().plan(kv)
+    check(step, kv, "forks")
+    d, ws = step.dev, step.workspace(kv)
+    out, lse = step.run(kv, ws)
+    other, olse = torch.full_like(out, 7.0), torch.full_like(lse, 7.0)
+    kv.chunk_attn(d["q"], d["k"], d["v"], d["tables"], d["plan"], other, olse, *step.shape(), ws,
+                  ws.numel(), shared_pages=True)
+    assert torch.equal(out, other) and torch.equal(lse, olse)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_one_workspace_and_the_same_bits_again(kv, dtype):
+    """Steps of many kinds through one workspace, over and over: a tile's pieces
+    give the same bits whichever workgroup joins them."""
+    steps = [Step(23 + i, dtype, (14, 2, 64), *args).upload().plan(kv) for i, args in enumerate([
+        ([90, 200, 37, 150, 61], [40, 300, 0, 77, 1200]),
+        ([1] * 7, [30, 9000, 100, 2000, 7, 64, 511]),
+        ([300], [0]),
+        ([41] * 9, [333] * 9, 200, 4),
+    ])]
+    ws = max((s.workspace(kv) for s in steps), key=lambda w: w.numel())
+    first = [s.run(kv, ws) for s in steps]
+    for s, (out, lse) in zip(steps, first):
+        want, wlse, tol, ltol = s.attention()
+        assert_within(out, want, tol, "out")
+        assert_within(lse, wlse, ltol, "lse")
+    for _ in range(30):
+        for s, (out, lse) in zip(steps, first):
+            again, alse = s.run(kv, ws)
+            assert torch.equal(out, again) and torch.equal(lse, alse)
+
+
+@pytest.mark.parametrize("heads", [(6, 6, 64), (33, 3, 128), (256, 1, 64)],
+                         ids=lambda h: "x".join(map(str, h)))
+def test_odd_groups(kv, heads):
+    step = Step(27, "bf16", heads, [1, 3, 20], [50, 0, 70], 30, 2).upload().plan(kv)
+    check(step, kv, "odd groups")
+
+
+def test_many_sequences(kv):
+    """More sequences than workgroups: several tiles each, some empty."""
+    new = [i % 3 for i in range(700)]
+    cached = [(i * 37) % 90 for i in range(700)]
+    step = Step(28, "f16", (4, 2, 64), new, cached).upload().plan(kv)
+    check(step, kv, "many")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("new", [2, 70])
+def test_a_value_of_little_weight_still_reaches_its_rows(kv, new, dtype):
+    """The last token's V is infinite and its weight below the type's smallest:
+    its own row has the infinity, those before it do not."""
+    step = Step(29, dtype, (4, 2, 64), [new], [24])
+    step.q[..., 0] = 30.0
+    step.k[..., 0] = 4.0
+    at = step.lens[0] - 1
+    step.k[step.tables[0, at // 16], :, at % 16, 0] = -2.0
+    want, wlse, tol, ltol = step.attention()
+    step.v[step.tables[0, at // 16], :, at % 16, 9] = math.inf
+    want[new - 1, :, 9] = math.inf
+    step.upload().plan(kv)
+    out, lse = step.run(kv)
+    assert_within(out, want, tol, "out")
+    assert_within(lse, wlse, ltol, "lse")
