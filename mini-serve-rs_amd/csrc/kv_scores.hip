@@ -257,6 +257,7 @@ __global__ __launch_bounds__(64 * W) void score_thin_kernel(ScoreParams p) {
 constexpr int kWideWaves = 4;
 constexpr int kWideThreads = 64 * kWideWaves;
 constexpr int kScoreKeys = 16 * kScorePages;  // keys a workgroup holds
+constexpr int kBlockRows = 128;  // a block's beginning and end cost about as many rows
 
 template <typename T, int D>
 __global__ __launch_bounds__(kWideThreads, 3) void score_wide_kernel(ScoreParams p) {
@@ -273,16 +274,15 @@ __global__ __launch_bounds__(kWideThreads, 3) void score_wide_kernel(ScoreParams
   __shared__ __align__(16) float s_lse[2][ROWS];
   __shared__ __align__(16) int s_kmax[2][ROWS];
   __shared__ float s_sum[RG][kScoreKeys];
+  __shared__ __align__(16) int s_rows[kWideThreads];
+  __shared__ int s_order[kWideThreads];
+  static_assert(kWideThreads == 256 && kMaxChunkSeqs < 1 << 23, "an order packs both");
 
   if (p.v.head->stamp != p.stamp) {
     if (blockIdx.x == 0 && threadIdx.x == 0) ws_raise(&p.v.head->flags, RLSE_WS_ERR_PLAN);
     return;
   }
   const int units = p.v.head->score_units, seqs = p.v.head->score_seqs;
-  const long long total = (long long)units * p.Hkv;
-  const int groups = (int)min((long long)gridDim.x, total);
-  if ((int)blockIdx.x >= groups) return;
-  const int wg = share_index(blockIdx.x, groups);
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int half = lane >> 5, col = lane & 31;
@@ -293,13 +293,83 @@ __global__ __launch_bounds__(kWideThreads, 3) void score_wide_kernel(ScoreParams
   const T* __restrict__ qb = static_cast<const T*>(p.q);
   const T* __restrict__ kp = static_cast<const T*>(p.k_pool);
 
-  for (long long unit = total * wg / groups; unit < total * (wg + 1) / groups; ++unit) {
-    const int h = (int)(unit / units), ub = (int)(unit - (long long)h * units);
+  // The sequence of a key block (of one head).
+  auto tile_at = [&](int ub) __attribute__((always_inline)) {
     int lo = 0, hi = seqs;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (p.v.score[mid].unit0 <= ub) lo = mid; else hi = mid;
     }
+    return lo;
+  };
+  // Rows that see a key of block u: from the first key's own token to the last
+  // one whose window reaches the last key (sinks: to the end).
+  auto rows_of = [&](const ChunkTile& t, int u, int* r_lo, int* r_hi)
+                     __attribute__((always_inline)) {
+    const int vfirst = u * kScorePages, vlast = min(vfirst + kScorePages, t.pages) - 1;
+    const int pos0 = real_page(vfirst, t.wp0, sink_pages) * 16;
+    const int pos1 = real_page(vlast, t.wp0, sink_pages) * 16 + 15;
+    int t_hi = t.n - 1;
+    if (p.window > 0 && pos0 >= p.sinks)
+      t_hi = (int)min((long long)t_hi, (long long)pos1 + p.window - 1 - t.off);
+    *r_lo = max(0, pos0 - t.off) * G / ROWS * ROWS;
+    *r_hi = (t_hi + 1) * G;
+  };
+
+  // The blocks of all KV heads, heads outermost, lie in eight contiguous runs,
+  // one for each XCD (workgroup b runs on XCD b % 8). Every compute unit of it
+  // holds three workgroups, at places c, c + its units, and so on; a run of up
+  // to kWideThreads blocks is sorted by the rows they meet, and dealt to and
+  // fro over the compute units, so that each gets about the same. (In order of
+  // their keys, 2 chunks of 2000 tokens under a window of 4096 with sinks gave
+  // some 382 stages of rows where the mean was 269: 254 us, 219 dealt so.)
+  const long long total = (long long)units * p.Hkv;
+  const long long run0 = total * (blockIdx.x & 7) >> 3;
+  const int run = (int)((total * ((blockIdx.x & 7) + 1) >> 3) - run0);
+  const int place = blockIdx.x >> 3, places = ((int)gridDim.x + 7 - (blockIdx.x & 7)) >> 3;
+  const int columns = (places + 2) / 3;
+  if (run == 0) return;
+  // Block i of the run is block (rem0 + i) % units of head h0 + (rem0 + i) / units.
+  const int h0 = (int)(run0 / units);
+  const unsigned rem0 = (unsigned)(run0 - (long long)h0 * units);
+  const bool sorted = run <= kWideThreads;
+  if (sorted) {
+    int rows = 0, lo = 0;
+    if (tid < run) {
+      const int ub = (int)((rem0 + tid) % (unsigned)units);
+      lo = tile_at(ub);
+      const ChunkTile t = p.v.score[lo];
+      int r_lo, r_hi;
+      rows_of(t, ub - t.unit0, &r_lo, &r_hi);
+      rows = max(r_hi - r_lo, 0) + kBlockRows;
+    }
+    s_rows[tid] = rows;  // (0 past the run's end)
+    __syncthreads();
+    int rank = 0;
+    for (int i = 0; i < run; i += 4) {
+      const int4 r = *reinterpret_cast<const int4*>(s_rows + i);
+      rank += (r.x > rows) | ((r.x == rows) & (i < tid));
+      rank += (r.y > rows) | ((r.y == rows) & (i + 1 < tid));
+      rank += (r.z > rows) | ((r.z == rows) & (i + 2 < tid));
+      rank += (r.w > rows) | ((r.w == rows) & (i + 3 < tid));
+    }
+    if (tid < run) s_order[rank] = lo << 8 | tid;
+    __syncthreads();
+  }
+
+  for (int round = place / columns;; round += 3) {
+    if (round * columns >= run) break;
+    int at = round * columns + (round & 1 ? columns - 1 - place % columns : place % columns);
+    if (at >= run) continue;
+    int lo = -1;
+    if (sorted) {
+      const int order = __builtin_amdgcn_readfirstlane(s_order[at]);
+      lo = order >> 8;
+      at = order & 255;
+    }
+    const int h = h0 + (int)((rem0 + at) / (unsigned)units);
+    const int ub = (int)((rem0 + at) % (unsigned)units);
+    if (lo < 0) lo = tile_at(ub);
     const ChunkTile t = p.v.score[lo];
     const int n = __builtin_amdgcn_readfirstlane(t.n), off = __builtin_amdgcn_readfirstlane(t.off);
     const int tok0 = __builtin_amdgcn_readfirstlane(t.tok0);
@@ -311,54 +381,22 @@ __global__ __launch_bounds__(kWideThreads, 3) void score_wide_kernel(ScoreParams
     const size_t out = ((size_t)seq * Hkv + h) * p.mbps * 16;
     const int rows = n * G, kend = off + n;
 
-    // This lane's keys (one per 32-key block).
-    int key[KS];
-    unsigned reach[KS];  // rows see key when their own is at key .. key + reach
-    uint4 k[KS][KB];
-    bool valid = true;
-    int first_key = 0x7fffffff, last_key = -1;
+    // (Page ids, rows and keys are requested before any is waited for.)
+    // Page of this lane's key in each of the wave's 32-key blocks.
+    int id[KS], pg[KS];
 #pragma unroll
-    for (int i = 0; i < 2 * KS; ++i) {
-      const int vi = u * kScorePages + kg * 2 * KS + i;
-      const int pg = real_page(min(vi, pages - 1), wp0, sink_pages);
-      const int id = table[pg];
-      const bool ok = vi < pages && (unsigned)id < (unsigned)p.num_blocks;
-      valid = valid && ok;
-      if (ok) {
-        first_key = min(first_key, pg * 16);
-        last_key = max(last_key, pg * 16 + 15);
-      }
-      if ((col >> 4) == (i & 1)) {
-        const int at = pg * 16 + (col & 15);
-        const bool here = ok && at < kend;
-        key[i >> 1] = here ? at : 0x7fffffff;
-        reach[i >> 1] = !here ? 0u
-                        : p.window > 0 && at >= p.sinks ? (unsigned)p.window - 1u
-                                                        : 0x7fffffffu;
-        const T* src = kp + (((size_t)(ok ? id : 0) * Hkv + h) * 16 + (col & 15)) * D;
-#pragma unroll
-        for (int b = 0; b < KB; ++b) {
-          // 16-bit: elements 16 b + 8 half ..; f32: half * D/2 + 4 b ..
-          const int e = ES == 2 ? b * 16 + half * 8 : half * (D / 2) + b * 4;
-          k[i >> 1][b] = here ? *reinterpret_cast<const uint4*>(src + e)
-                                      : make_uint4(0, 0, 0, 0);
-        }
-      }
+    for (int i = 0; i < KS; ++i) {
+      const int vi = u * kScorePages + (kg * KS + i) * 2 + (col >> 4);
+      pg[i] = real_page(min(vi, pages - 1), wp0, sink_pages);
+      id[i] = table[pg[i]];
+      if (vi >= pages || (unsigned)id[i] >= (unsigned)p.num_blocks) id[i] = -1;
     }
-    // Rows that see a key of the workgroup: from the first key's own token to
-    // the last one whose window reaches the last key (sinks: to the end).
     const int vfirst = u * kScorePages, vlast = min(vfirst + kScorePages, pages) - 1;
-    const int pos0 = real_page(vfirst, wp0, sink_pages) * 16;
-    const int pos1 = real_page(vlast, wp0, sink_pages) * 16 + 15;
-    const int t_lo = max(0, pos0 - off);
-    int t_hi = n - 1;
-    if (p.window > 0 && pos0 >= p.sinks)
-      t_hi = (int)min((long long)t_hi, (long long)pos1 + p.window - 1 - off);
-    const int r_lo = t_lo * G / ROWS * ROWS, r_hi = (t_hi + 1) * G;
+    int r_lo, r_hi;
+    rows_of(t, u, &r_lo, &r_hi);
+    r_lo = __builtin_amdgcn_readfirstlane(r_lo);
+    r_hi = __builtin_amdgcn_readfirstlane(r_hi);
 
-    float sum[KS];
-#pragma unroll
-    for (int i = 0; i < KS; ++i) sum[i] = 0.f;
     // What the key that this thread will write had before.
     float before = 0.f;
     if (tid < kScoreKeys && vfirst + (tid >> 4) <= vlast)
@@ -369,7 +407,7 @@ __global__ __launch_bounds__(kWideThreads, 3) void score_wide_kernel(ScoreParams
         const_cast<T*>(qb + ((size_t)tok0 * Hq + h * G) * D), 0,
         (int)(((unsigned)(n - 1) * Hq + G) * (D * ES)), kBufferWord3);
     const float* __restrict__ lh = p.lse + (size_t)tok0 * Hq + h * G;
-    auto place = [&](int row) __attribute__((always_inline)) {
+    auto row_at = [&](int row) __attribute__((always_inline)) {
       return row + div.token(row) * (Hq - G);
     };
     u32x4_t qst[QPT];
@@ -381,12 +419,12 @@ __global__ __launch_bounds__(kWideThreads, 3) void score_wide_kernel(ScoreParams
         const int pk = tid + j * kWideThreads;
         // (Rows past the last lie past the descriptor's end: zeros.)
         qst[j] = __builtin_amdgcn_raw_buffer_load_b128(
-            rq, (int)((unsigned)place(r0 + pk / PPR) * (D * ES) + pk % PPR * 16), 0, 0);
+            rq, (int)((unsigned)row_at(r0 + pk / PPR) * (D * ES) + pk % PPR * 16), 0, 0);
       }
       if (tid < ROWS) {
         // (Rows past the last read it again; they see no key.)
         const int row = min(r0 + tid, rows - 1);
-        lst = lh[place(row)];
+        lst = lh[row_at(row)];
         kst = r0 + tid < rows ? off + div.token(row) : -1;
       }
     };
@@ -401,9 +439,46 @@ __global__ __launch_bounds__(kWideThreads, 3) void score_wide_kernel(ScoreParams
         s_kmax[bf][tid] = kst;
       }
     };
+    if (r_lo < r_hi) load(r_lo);
+
+    int key[KS];
+    unsigned reach[KS];  // rows see key when their own is at key .. key + reach
+    uint4 k[KS][KB];
+    bool valid = true;
+    int first_key = 0x7fffffff, last_key = -1;
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      const uint64_t ok = __ballot(id[i] >= 0);
+#pragma unroll
+      for (int j = 0; j < 32; j += 16) {
+        const int pos = __builtin_amdgcn_readlane(pg[i], j) * 16;
+        if (ok >> j & 1) {
+          first_key = min(first_key, pos);
+          last_key = max(last_key, pos + 15);
+        } else {
+          valid = false;
+        }
+      }
+      const int at = pg[i] * 16 + (col & 15);
+      const bool here = id[i] >= 0 && at < kend;
+      key[i] = here ? at : 0x7fffffff;
+      reach[i] = !here ? 0u
+                 : p.window > 0 && at >= p.sinks ? (unsigned)p.window - 1u
+                                                 : 0x7fffffffu;
+      const T* src = kp + (((size_t)max(id[i], 0) * Hkv + h) * 16 + (col & 15)) * D;
+#pragma unroll
+      for (int b = 0; b < KB; ++b) {
+        // 16-bit: elements 16 b + 8 half ..; f32: half * D/2 + 4 b ..
+        const int e = ES == 2 ? b * 16 + half * 8 : half * (D / 2) + b * 4;
+        k[i][b] = here ? *reinterpret_cast<const uint4*>(src + e) : make_uint4(0, 0, 0, 0);
+      }
+    }
+
+    float sum[KS];
+#pragma unroll
+    for (int i = 0; i < KS; ++i) sum[i] = 0.f;
     __syncthreads();  // the stages of the unit before are read
     if (r_lo < r_hi) {
-      load(r_lo);
       store(0);
       __syncthreads();
       int bf = 0;
@@ -422,12 +497,24 @@ __global__ __launch_bounds__(kWideThreads, 3) void score_wide_kernel(ScoreParams
           for (int i = 0; i < KS; ++i)
 #pragma unroll
             for (int e = 0; e < 16; ++e) x[i][e] = 0.f;
+          // Rows come from LDS four products ahead (as the compiler schedules the
+          // reads: 3% slower).
+          auto operand = [&](int b) __attribute__((always_inline)) {
+            const int at = ES == 2 ? b * 16 + half * 8 : half * (D / 2) + b * 4;
+            return *reinterpret_cast<const uint4*>(&s_q[bf][rg * 32 + col][at]);
+          };
+          constexpr int R = 4;
+          uint4 ring[R];
+#pragma unroll
+          for (int b = 0; b < R; ++b) ring[b] = operand(b);
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int b = 0; b < KB; ++b) {
-            const int at = ES == 2 ? b * 16 + half * 8 : half * (D / 2) + b * 4;
-            const uint4 a = *reinterpret_cast<const uint4*>(&s_q[bf][rg * 32 + col][at]);
+            const uint4 a = ring[b % R];
 #pragma unroll
             for (int i = 0; i < KS; ++i) x[i] = mma32<T>(a, k[i][b], x[i]);
+            if (b + R < KB) ring[b % R] = operand(b + R);
+            __builtin_amdgcn_sched_barrier(0);
           }
           const bool whole = valid && last_key <= kmax_lo && last_key < kend && rb == ra + 31 &&
                              (p.window <= 0 || first_key > kmax_hi - p.window ||

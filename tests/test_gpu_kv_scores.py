@@ -213,3 +213,11 @@ def test_many_sequences(kv):
     step = Step(41, "bf16", (4, 2, 64), [i % 3 for i in range(700)],
                 [(i * 37) % 90 for i in range(700)])
     check(kv, step, "many")
+
+
+@pytest.mark.parametrize("window", [(0, 0), (40, 3)])
+def test_many_chunks(kv, window):
+    """More key blocks than are sorted by the rows they meet."""
+    step = Step(42, "bf16", (16, 8, 64), [17 + i % 20 for i in range(330)],
+                [(i * 37) % 200 for i in range(330)], *window)
+    check(kv, step, "many chunks")
