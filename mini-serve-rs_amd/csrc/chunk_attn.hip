@@ -46,6 +46,7 @@ typedef short i16x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) i16x4_t lds_i16x4_t;
+typedef __attribute__((address_space(3))) void lds_void_t;
 
 // 16-bit tiles: 16x16x32 and 32x32x16 products of 16-byte operands, and
 // 16x16x16 ones of 8-byte operands.
@@ -148,6 +149,19 @@ __device__ __forceinline__ void ld_pair(const float* p, float* out) {
                                        __HIP_MEMORY_SCOPE_AGENT);
   out[0] = __uint_as_float((uint32_t)v);
   out[1] = __uint_as_float((uint32_t)(v >> 32));
+}
+
+// Requests 16 bytes a lane through a buffer descriptor, to lds + 16 * lane (lds
+// the same for the wave).
+__device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t r, void* lds, int off) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void_t*)lds, 16, off, 0, 0, 0);
+#endif
+}
+// Waits for the wave's LDS accesses.
+__device__ __forceinline__ void wait_lds() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(15 | 7 << 4 | 3 << 14);
 }
 
 // The weight of a partial state of max m under the joint max M (both -inf:
@@ -739,12 +753,16 @@ constexpr int kWideBufs = 3;
 
 template <typename T, int D>
 struct WideLds {
-  // Row strides that put the rows one read takes together on banks of their
-  // own (64 four-byte banks): K rows 4 banks apart, the rows of a transposing
-  // V read 16.
-  static constexpr int kPadK = 8, kPadV = 32;
-  T k[kWideBufs][kWideKeys][D + kPadK];
-  T v[kWideBufs][kWideKeys][D + kPadV];
+  T k[kWideBufs][kWideKeys][D];
+  T v[kWideBufs][kWideKeys][D];
+  // Packet (16 bytes) c of a row lies at place c ^ turn: rows that one read
+  // takes together are on banks of their own (64 four-byte banks). K: 8
+  // consecutive rows, one packet of each; V (transposing reads): 4 consecutive
+  // rows, the same four packets of each.
+  static __device__ __forceinline__ int turn_k(int row) { return row & (D / 8 - 1); }
+  static __device__ __forceinline__ int turn_v(int row) {
+    return D == 128 ? (row & 3) << 2 : (row & 2) << 1;
+  }
 };
 
 template <typename T, int D>
@@ -773,11 +791,13 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
   const T* __restrict__ kp = static_cast<const T*>(p.k_pool);
   const T* __restrict__ vp = static_cast<const T*>(p.v_pool);
 
-  // Packet j of this thread in a stage: key kk0 + j * kWideThreads / PPR,
-  // chunk dc of its row; its page is the same for the wave.
+  // Place j of this thread in a stage: key kk0 + j * kWideThreads / PPR, place
+  // dc of its row; its page is the same for the wave, whose places are 1 KB of
+  // consecutive LDS.
   const int kk0 = tid / PPR, dc = tid % PPR;
   constexpr int kStep = kWideThreads / PPR;  // 32 or 64 keys
-  const int voff = (kk0 & 15) * D * 2 + dc * 16;
+  const int koff = (kk0 & 15) * D * 2 + (dc ^ WideLds<T, D>::turn_k(kk0)) * 16;
+  const int voff = (kk0 & 15) * D * 2 + (dc ^ WideLds<T, D>::turn_v(kk0)) * 16;
   const int pg0 = __builtin_amdgcn_readfirstlane(kk0 >> 4);
 
   // Transposing V reads: within a 16-lane group lane 4j + a points at key row
@@ -852,8 +872,7 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
     const unsigned page_elems = Hkv * 16 * D;
     const int last_rec = (((kend - 1) & 15) + 1) * D * 2;
     unsigned oks = 0;  // valid pages of the last 8 units loaded, a bit each
-    u32x4_t kst[KPT], vst[KPT];
-    auto load = [&](int u) __attribute__((always_inline)) {
+    auto load = [&](int u, int bf) __attribute__((always_inline)) {
       if (u * kWidePages >= ids_at + 64) fetch_ids(u);
 #pragma unroll
       for (int j = 0; j < KPT; ++j) {
@@ -865,8 +884,9 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
                                                           kBufferWord3);
         const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(vh + base), 0, rec,
                                                           kBufferWord3);
-        kst[j] = __builtin_amdgcn_raw_buffer_load_b128(rk, voff, 0, 0);
-        vst[j] = __builtin_amdgcn_raw_buffer_load_b128(rv, voff, 0, 0);
+        const int kk = wave * (64 / PPR) + j * kStep;
+        load_lds(rk, &s.k[bf][kk][0], koff);
+        load_lds(rv, &s.v[bf][kk][0], voff);
       }
       const int at4 = (u & 7) * 4;
       oks = (oks & ~(15u << at4)) |
@@ -877,27 +897,34 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
     auto whole_of = [&](int u) __attribute__((always_inline)) {
       return ok_of(u) == 15u && all.has(u);
     };
-    auto store = [&](int bf, bool whole) __attribute__((always_inline)) {
+    // Waits for this thread's part of unit u; where not all of the unit is
+    // seen, its values of V that are not finite become zeros and are noted.
+    auto arrive = [&](int u, int bf) __attribute__((always_inline)) {
+      wait_vm_stores();
+      if (whole_of(u)) return;
 #pragma unroll
       for (int j = 0; j < KPT; ++j) {
         const int kk = kk0 + j * kStep;
-        if (!whole) {
-          bool odd = false;
+        u32x4_t* at = reinterpret_cast<u32x4_t*>(&s.v[bf][kk][dc * 8]);
+        u32x4_t y = *at;
+        bool odd = false;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            constexpr uint32_t inf = Tile<T>::kInf;
-            const uint32_t x = vst[j][i];
-            const bool lo = (x & inf) == inf, hi = (x & inf << 16) == inf << 16;
-            odd = odd | lo | hi;
-            vst[j][i] = x & (lo ? 0xffff0000u : ~0u) & (hi ? 0xffffu : ~0u);
-          }
-          if (odd) atomicOr(&s_odd[bf][kk >> 5], 1u << (kk & 31));
+        for (int i = 0; i < 4; ++i) {
+          constexpr uint32_t inf = Tile<T>::kInf;
+          const uint32_t x = y[i];
+          const bool lo = (x & inf) == inf, hi = (x & inf << 16) == inf << 16;
+          odd = odd | lo | hi;
+          y[i] = x & (lo ? 0xffff0000u : ~0u) & (hi ? 0xffffu : ~0u);
         }
-        *reinterpret_cast<u32x4_t*>(&s.k[bf][kk][dc * 8]) = kst[j];
-        *reinterpret_cast<u32x4_t*>(&s.v[bf][kk][dc * 8]) = vst[j];
+        if (odd) {
+          *at = y;
+          atomicOr(&s_odd[bf][kk >> 5], 1u << (kk & 31));
+        }
       }
     };
 
+    // Buffer of unit u: (u - u0) % kWideBufs, kept as three rotating indices.
+    int b_prev = 2, b_cur = 0, b_next = 1;
     f32x16_t x[2];
     uint4 pk[4];  // P^T operands of the four 16-key blocks
     // Operand i of a turn's products: the K operands of q.k, then the V^T ones
@@ -906,19 +933,20 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
     auto operand = [&](int i, int bk, int bv) __attribute__((always_inline)) {
       if (i < NK) {
         const int kb = i >> 1, sb = i & 1;
-        return *reinterpret_cast<const uint4*>(&s.k[bk][sb * 32 + col][kb * 16 + half * 8]);
+        return *reinterpret_cast<const uint4*>(
+            &s.k[bk][sb * 32 + col][((kb * 2 + half) ^ WideLds<T, D>::turn_k(col)) * 8]);
       }
       const int kq = (i - NK) / DB, d = (i - NK) % DB;
-      const uint16_t* v0 =
-          reinterpret_cast<const uint16_t*>(&s.v[bv][kq * 16 + tr_row][d * 32 + tr_col]);
+      const uint16_t* v0 = reinterpret_cast<const uint16_t*>(
+          &s.v[bv][kq * 16 + tr_row][((d * 32 + tr_col) ^ WideLds<T, D>::turn_v(tr_row) * 8)]);
       const uint2 lo = __builtin_bit_cast(
           uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)v0));
       const uint2 hi = __builtin_bit_cast(
           uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                     (lds_i16x4_t*)(v0 + 8 * (D + WideLds<T, D>::kPadV))));
+                     (lds_i16x4_t*)(v0 + 8 * D)));
       return make_uint4(lo.x, lo.y, hi.x, hi.y);
     };
-    auto products = [&](auto qk, auto pv, int bk, int bv) __attribute__((always_inline)) {
+    auto products = [&](auto qk, auto pv, int bk, int bv, int ul) __attribute__((always_inline)) {
       constexpr int from = decltype(qk)::value ? 0 : NK, to = decltype(pv)::value ? NK + NV : NK;
       constexpr int R = 6;  // operands in flight from LDS ahead of their MFMA
       __builtin_amdgcn_s_setprio(1);
@@ -940,6 +968,7 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
         else
           o[(i - NK) % DB] = Tile<T>::mma32(a, pk[(i - NK) / DB], o[(i - NK) % DB]);
         if (i + R < to) ring[(i - from) % R] = operand(i + R, bk, bv);
+        if (i + R == to && ul < u_end) load(ul, b_next);
         __builtin_amdgcn_sched_barrier(0);
       }
       __builtin_amdgcn_s_setprio(0);
@@ -1025,7 +1054,9 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
     };
     auto turn = [&]() __attribute__((always_inline)) {
       __builtin_amdgcn_sched_barrier(0);
-      __syncthreads();
+      wait_lds();
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
       __builtin_amdgcn_sched_barrier(0);
     };
 
@@ -1033,37 +1064,29 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
     if (tid < 2 * kWideBufs) s_odd[tid >> 1][tid & 1] = 0;
     __syncthreads();
     fetch_ids(u0);
-    load(u0);
-    store(0, whole_of(u0));
-    if (seg > 1) load(u0 + 1);
+    load(u0, 0);
+    arrive(u0, 0);
     turn();
-    // Buffer of unit u: (u - u0) % kWideBufs, kept as three rotating indices.
-    int b_prev = 2, b_cur = 0, b_next = 1;
     const bool behind = wave >= kWideWaves / 2;
     if (behind) {
-      if (seg > 1) {
-        store(1, whole_of(u0 + 1));
-        if (seg > 2) load(u0 + 2);
-      }
+      if (seg > 1) load(u0 + 1, 1);
       turn();
+      // (Waves 0-3 loaded theirs in this turn and wait for it in the next.)
     }
     for (int u = u0; u < u_end; ++u) {
+      if (!live && !behind && u + 1 < u_end) load(u + 1, b_next);
       if (live) {
         if (u > u0)
-          products(std::true_type{}, std::true_type{}, b_cur, b_prev);
+          products(std::true_type{}, std::true_type{}, b_cur, b_prev, behind ? u_end : u + 1);
         else
-          products(std::true_type{}, std::false_type{}, b_cur, b_prev);
+          products(std::true_type{}, std::false_type{}, b_cur, b_prev, behind ? u_end : u + 1);
         if (u > u0 && !whole_of(u - 1)) add_odd(b_prev, u - 1);
       }
+      if (behind && u + 1 < u_end) arrive(u + 1, b_next);
       turn();
+      if (behind && u + 2 < u_end) load(u + 2, b_prev);
       if (live) softmax(u);
-      // Waves 0-3 store unit u + 1, waves 4-7 (half a stage later) u + 2, into
-      // the buffer of unit u - 2 or u - 1, whose last reads are two turns old.
-      const int us = behind ? u + 2 : u + 1;
-      if (us < u_end) {
-        store(behind ? b_prev : b_next, whole_of(us));
-        if (us + 1 < u_end) load(us + 1);
-      }
+      if (!behind && u + 1 < u_end) arrive(u + 1, b_next);
       turn();
       const int b = b_prev;
       b_prev = b_cur;
@@ -1071,7 +1094,7 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
       b_next = b;
     }
     if (live) {
-      products(std::false_type{}, std::true_type{}, 0, b_prev);
+      products(std::false_type{}, std::true_type{}, 0, b_prev, u_end);
       if (!whole_of(u_end - 1)) add_odd(b_prev, u_end - 1);
     }
     if (!behind) turn();
