@@ -14,7 +14,7 @@
 //  - thin (at most 32 rows: decode steps, drafts): HBM bound. A wave streams
 //    its own pages, 16 keys at a time, and every key meets all rows at once
 //    (S^T = K.Q^T on 16x16 MFMAs with K straight from memory in the operand
-//    layout); the four waves of a workgroup meet at the tile's end.
+//    layout); the waves of a workgroup meet at the tile's end.
 //  - wide: MFMA bound. Eight waves of 32 rows share 64 keys staged in LDS.
 // Softmax statistics, sums and accumulators are f32; probabilities are
 // rounded to the K/V type for the product with V (2^-9 relative in bf16, as
@@ -739,13 +739,17 @@ __device__ __forceinline__ void wide_finish(const ChunkParams& p, const ChunkSha
 // wave more than a thousand cycles, on different pipes. So the two waves of a
 // SIMD take turns: while waves 0-3 run the products of a stage (q.k, and p.v
 // of the stage before), waves 4-7 run their softmax, and a barrier swaps them.
-// Waves 4-7 are thus half a stage behind, and store their part of each stage
-// half a stage ahead, which three LDS buffers allow. A turn's operands are
-// read from LDS six MFMAs ahead: 1360 cycles for 32 MFMAs, 2380 as the
-// compiler schedules the reads. A stage of 64 keys takes 4700 cycles, 5600
-// without the turns' order. In long launches the card's clock falls as the
-// cycles do (2.4 to 2.0 GHz, 2.3 us a stage either way: 840 TFLOP/s of the
-// 1190 that a large matrix product reaches); short ones gain 2-4%.
+// Waves 4-7 are thus half a stage behind. A stage's keys and values go straight
+// to LDS, each wave's part a turn or two before it is used, which three
+// buffers allow (through registers, stored between the turns: 778 us for the
+// prompts below). A turn's operands are read from LDS six MFMAs ahead: 1360
+// cycles for 32 MFMAs, 2380 as the compiler schedules the reads.
+// Two prompts of 4096 tokens after 0-6000, 32/8 heads of 128 in bf16: 700 us,
+// 970 TFLOP/s of the 1194 that a large matrix product reaches here. A stage of
+// 64 keys takes 4030 cycles (products 1850, softmax 1470, the rest loads,
+// waits and barriers) at a clock that long launches bring down to 1.76 GHz
+// (1.94 in one of 290 us): what they draw bounds them, so that a turn
+// shortened by a tenth gains a few per cent.
 constexpr int kWideWaves = 8;
 constexpr int kWideThreads = 64 * kWideWaves;
 constexpr int kWideKeys = 16 * kWidePages;
