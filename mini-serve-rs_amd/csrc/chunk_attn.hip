@@ -14,7 +14,12 @@
 //  - thin (at most 32 rows: decode steps, drafts): HBM bound. A wave streams
 //    its own pages, 16 keys at a time, and every key meets all rows at once
 //    (S^T = K.Q^T on 16x16 MFMAs with K straight from memory in the operand
-//    layout); the waves of a workgroup meet at the tile's end.
+//    layout); the waves of a workgroup meet at the tile's end. 48 tokens after
+//    4096-32768 keys, 32/8 heads of 128 in f16: 554 us, 6.5 TB/s; 32 tokens under a
+//    window of 1024, 16/8 heads: 25 us, of which 20 are HBM's; one token after 700:
+//    12 us, a chain of loads. Pages are read with non-temporal loads unless the
+//    caller says that sequences share them: 32 tokens after 4000 keys 81 us, 91
+//    cacheable; with one table for all, 44 and 42.
 //  - wide: MFMA bound. Eight waves of 32 rows share 64 keys staged in LDS.
 // Softmax statistics, sums and accumulators are f32; probabilities are
 // rounded to the K/V type for the product with V (2^-9 relative in bf16, as
@@ -741,12 +746,11 @@ __device__ __forceinline__ void wide_finish(const ChunkParams& p, const ChunkSha
 // of the stage before), waves 4-7 run their softmax, and a barrier swaps them.
 // Waves 4-7 are thus half a stage behind. A stage's keys and values go straight
 // to LDS, each wave's part a turn or two before it is used, which three
-// buffers allow (through registers, stored between the turns: 778 us for the
-// prompts below). A turn's operands are read from LDS six MFMAs ahead: 1360
+// buffers allow (through registers, stored between the turns: 5% slower). A turn's operands are read from LDS six MFMAs ahead: 1360
 // cycles for 32 MFMAs, 2380 as the compiler schedules the reads.
-// Two prompts of 4096 tokens after 0-6000, 32/8 heads of 128 in bf16: 700 us,
-// 970 TFLOP/s of the 1194 that a large matrix product reaches here. A stage of
-// 64 keys takes 4030 cycles (products 1850, softmax 1470, the rest loads,
+// Two prompts of 4096 tokens after 0-6000, 32/8 heads of 128 in bf16: 740-780 us,
+// 870-915 TFLOP/s of the 1194 that a large matrix product reaches here. A stage
+// of 64 keys takes 4030 cycles (products 1850, softmax 1470, the rest loads,
 // waits and barriers) at a clock that long launches bring down to 1.76 GHz
 // (1.94 in one of 290 us): what they draw bounds them, so that a turn
 // shortened by a tenth gains a few per cent.
@@ -1120,6 +1124,8 @@ __global__ __launch_bounds__(kWideThreads, 1) void chunk_wide_kernel(ChunkParams
 // ---------------------------------------------------------------------------
 // Wide sequences, f32
 // ---------------------------------------------------------------------------
+// 1024 tokens after 2048, 32/8 heads of 128: 345 us, 125 TFLOP/s of the 154 that a
+// large f32 matrix product reaches here.
 // The same products on v_mfma_f32_32x32x2_f32, whose rate bounds them: lane half
 // h contracts dimension h*D/2 + j at step j of S^T = K . Q^T, and step j of
 // O^T += V^T . P^T pairs the two keys that the lane halves hold in accumulator

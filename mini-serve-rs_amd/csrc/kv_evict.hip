@@ -10,7 +10,9 @@
 //    weight is found by three histograms (11, 11 and 10 bits) of the weights'
 //    order-preserving bit patterns, then the kept keys are numbered by ballots
 //    in key order: weights above it, and of those equal to it the first ones.
-//    No float arithmetic, and integer counts only: the answer is exact.
+//    No float arithmetic, and integer counts only: the answer is exact. Bound by
+//    the barriers between its passes: 8 us for one head of 1500 keys, 58 us for
+//    3584 heads of 1500-4096.
 //  - Move: HBM bound, a copy of rows picked by index, with non-temporal loads
 //    and stores, for nothing is read twice (Qwen3-0.6B, 28 layers of 16
 //    sequences cut to 1024 keys, 3.8 GB: 682 us, 5.5 TB/s; 737 us cacheable,

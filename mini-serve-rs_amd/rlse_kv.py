@@ -12,6 +12,10 @@ reference's operator and cache APIs by name and behaviour:
 * ``kv_append`` / ``kv_gather`` / ``kv_scatter`` / ``kv_copy_blocks`` --
   Attention::append_kv and get/set_kv_snapshot (qwen2.rs:349-377, 547-574).
 * ``paged_gqa_decode`` -- decode_attention_gqa_zero_copy (qwen2.rs:177-203).
+* ``chunk_plan`` / ``chunk_attn`` / ``kv_scores`` / ``kv_evict`` -- ragged steps
+  of long contexts (no counterpart in the reference): attention of any number
+  of new tokens per sequence with a sliding window and sinks, the weight every
+  cached key receives, and the cut of a cache to its heaviest keys.
 * ``rmsnorm`` / ``rope`` / ``qk_norm_rope_append`` -- RmsNorm::forward,
   apply_rotary_emb_qkv and the front half of Attention::forward
   (qwen2.rs:56-142, 291-313).
