@@ -191,8 +191,9 @@ __device__ __forceinline__ void write_row(T* dst, const float* v, float inv) {
 #pragma unroll
   for (int i = 0; i + 3 < N; i += 4) {
     if constexpr (sizeof(T) == 2)
-      *reinterpret_cast<uint2*>(dst + i) = make_uint2(Packet<T>::pack2(v[i] * inv, v[i + 1] * inv),
-                                                      Packet<T>::pack2(v[i + 2] * inv, v[i + 3] * inv));
+      *reinterpret_cast<uint2*>(dst + i) =
+          make_uint2(Packet<T>::pack2(v[i] * inv, v[i + 1] * inv),
+                     Packet<T>::pack2(v[i + 2] * inv, v[i + 3] * inv));
     else
       *reinterpret_cast<float4*>(dst + i) =
           make_float4(v[i] * inv, v[i + 1] * inv, v[i + 2] * inv, v[i + 3] * inv);
@@ -746,8 +747,9 @@ __device__ __forceinline__ void wide_finish(const ChunkParams& p, const ChunkSha
 // of the stage before), waves 4-7 run their softmax, and a barrier swaps them.
 // Waves 4-7 are thus half a stage behind. A stage's keys and values go straight
 // to LDS, each wave's part a turn or two before it is used, which three
-// buffers allow (through registers, stored between the turns: 5% slower). A turn's operands are read from LDS six MFMAs ahead: 1360
-// cycles for 32 MFMAs, 2380 as the compiler schedules the reads.
+// buffers allow (through registers, stored between the turns: 5% slower). A
+// turn's operands are read from LDS six MFMAs ahead (as the compiler schedules
+// the reads, a turn of products took 1.75 times as long).
 // Two prompts of 4096 tokens after 0-6000, 32/8 heads of 128 in bf16: 740-780 us,
 // 870-915 TFLOP/s of the 1194 that a large matrix product reaches here. A stage
 // of 64 keys takes 4030 cycles (products 1850, softmax 1470, the rest loads,
@@ -1416,9 +1418,9 @@ __global__ __launch_bounds__(kPartLanes) void chunk_merge_kernel(ChunkParams p) 
 #pragma unroll
   for (int i = 0; i < 16; ++i) acc[i] = 0.f;
   for (int k = w; k <= share.last; ++k) {
-    const float4* part = reinterpret_cast<const float4*>(
-                             p.wide_part + (size_t)(2 * k + (k == w ? 1 : 0)) * wide_part_floats(D)) +
-                         tid;
+    const size_t slot = 2 * k + (k == w ? 1 : 0);
+    const float4* part =
+        reinterpret_cast<const float4*>(p.wide_part + slot * wide_part_floats(D)) + tid;
     const float4 ml = part[4 * DB * kPartLanes];
     float4 a[4];
 #pragma unroll
