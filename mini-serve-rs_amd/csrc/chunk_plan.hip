@@ -25,21 +25,33 @@ struct PlanParams {
   int wide_cap;
 };
 
+// Inclusive prefix of x over the wave's lanes (row: over each 16 lanes), by data
+// parallel primitives: a few cycles a step, where shuffles go through LDS.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int from_lane(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, ROWS == 0xf);
+}
+__device__ __forceinline__ int row_scan(int x) {
+  x += from_lane<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8
+  x += from_lane<0x112, 0xf>(x);
+  x += from_lane<0x114, 0xf>(x);
+  return x + from_lane<0x118, 0xf>(x);
+}
+__device__ __forceinline__ int wave_scan(int x) {
+  x = row_scan(x);
+  x += from_lane<0x142, 0xa>(x);        // row_bcast 15 to rows 1 and 3,
+  return x + from_lane<0x143, 0xc>(x);  // row_bcast 31 to rows 2 and 3
+}
+
 // Exclusive prefixes of the N values x over the workgroup, and their sums
 // (s_w: kPlanWaves * N ints). (One pass for all: the round trips count here.)
 template <int N>
 __device__ __forceinline__ void block_scan(int (&x)[N], int (*s_w)[N], int (&sum)[N]) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  static_assert(kPlanWaves == 16, "a row holds the waves' sums");
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int inc[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) inc[i] = x[i];
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1)
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int y = __shfl_up(inc[i], o, 64);
-      if (lane >= o) inc[i] += y;
-    }
+  for (int i = 0; i < N; ++i) inc[i] = wave_scan(x[i]);
   __syncthreads();
   if (lane == 63)
 #pragma unroll
@@ -47,15 +59,9 @@ __device__ __forceinline__ void block_scan(int (&x)[N], int (*s_w)[N], int (&sum
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    int before = 0, all = 0;
-#pragma unroll
-    for (int k = 0; k < kPlanWaves; ++k) {
-      const int s = s_w[k][i];
-      before += k < wave ? s : 0;
-      all += s;
-    }
-    sum[i] = all;
-    x[i] = before + inc[i] - x[i];
+    const int all = row_scan(s_w[lane & 15][i]);
+    sum[i] = __builtin_amdgcn_readlane(all, 15);
+    x[i] = inc[i] - x[i] + (wave ? __builtin_amdgcn_readlane(all, wave - 1) : 0);
   }
 }
 
@@ -75,9 +81,9 @@ __device__ __forceinline__ int tile_of(const int* held, const ChunkTile* a, int 
 // workgroups of at least min_units each, equal shares, but a boundary within
 // snap units of a tile's moves there, and with `whole` (n * Hkv <= max_groups)
 // each gets one tile. (A tile cut for the sake of a few units costs more than
-// they do.) Worked out by kDealThreads threads, t among them; starts:
-// max_groups + 1 numbers in LDS. I: an integer type that holds units * Hkv *
-// max_groups.
+// they do.) Worked out by kDealThreads threads, t among them; starts and
+// firsts: max_groups + 1 numbers in LDS, where each share starts and in which
+// tile. I: an integer type that holds units * Hkv * max_groups.
 constexpr int kMaxShares = 1024;
 constexpr int kDealThreads = kPlanThreads / 2;
 struct DealList {
@@ -97,28 +103,35 @@ __device__ int deal_groups(const DealList& d, int Hkv) {
   return (int)(want < (I)d.max_groups ? want : (I)d.max_groups);
 }
 template <typename I>
-__device__ void deal_starts(const DealList& d, int Hkv, int t, I* starts) {
+__device__ void deal_starts(const DealList& d, int Hkv, int t, I* starts, int* firsts) {
   const I total = (I)d.units * Hkv;
   if (total == 0) return;
   const int groups = deal_groups<I>(d, Hkv);
   const int snap = (int)min((I)d.snap, total / (4 * groups));
   for (int w = t; w <= groups; w += kDealThreads) {
     I x = total * w / groups;
+    int i = 0;
     if (d.whole) {
-      x = w < groups ? (I)(w / d.n) * d.units + d.unit0(w % d.n) : total;
+      i = w % d.n;
+      x = w < groups ? (I)(w / d.n) * d.units + d.unit0(i) : total;
     } else if (w > 0 && w < groups) {
       const int head = (int)(x / d.units), u = (int)(x - (I)head * d.units);
-      const int i = tile_of(d.held, d.tiles, d.n, u), lo = d.unit0(i), hi = d.unit0(i + 1);
-      if (u - lo <= snap)
+      i = tile_of(d.held, d.tiles, d.n, u);
+      const int lo = d.unit0(i), hi = d.unit0(i + 1);
+      if (u - lo <= snap) {
         x -= u - lo;
-      else if (hi - u <= snap)
+      } else if (hi - u <= snap) {
         x += hi - u;
+        if (++i == d.n) i = 0;
+      }
     }
     starts[w] = x;
+    firsts[w] = i;
   }
 }
 template <typename I>
-__device__ void deal_shares(const DealList& d, int Hkv, int t, const I* starts) {
+__device__ void deal_shares(const DealList& d, int Hkv, int t, const I* starts,
+                            const int* firsts) {
   const I total = (I)d.units * Hkv;
   const int groups = total ? deal_groups<I>(d, Hkv) : 0;
   for (int b = t; b < d.max_groups; b += kDealThreads) {
@@ -132,10 +145,12 @@ __device__ void deal_shares(const DealList& d, int Hkv, int t, const I* starts) 
     const int units = d.units;
     s.head = (int)(from / units);
     const int u = (int)(from - (I)s.head * units);
-    s.tile = tile_of(d.held, d.tiles, d.n, u);
+    s.tile = firsts[s.w];
     s.end_head = (int)((to - 1) / units);
     const I base = (I)s.end_head * units;
-    s.end_tile = tile_of(d.held, d.tiles, d.n, (int)(to - 1 - base));
+    // (The next share's tile, or the one before where that starts there.)
+    const int after = firsts[s.w + 1], end_u = (int)(to - base);
+    s.end_tile = end_u == units ? d.n - 1 : after - (d.unit0(after) == end_u);
     s.at = d.tiles[d.from_end ? s.end_tile : s.tile];
     auto holder = [&](I x) {  // the share that has unit x
       int w = d.whole ? s.w : (int)(x * groups / total);
@@ -160,6 +175,7 @@ __global__ __launch_bounds__(kPlanThreads) void chunk_plan_kernel(PlanParams p) 
   __shared__ int s_w[kPlanWaves][5], s_w1[kPlanWaves][1];
   __shared__ int s_thin[kHeld], s_unit[kHeld];  // unit0 of the thin and the wide tiles
   __shared__ unsigned long long s_starts[2][kMaxShares + 1];
+  __shared__ int s_firsts[2][kMaxShares + 1];
   __shared__ unsigned s_flags;
   __shared__ int s_longest;  // pages of the longest thin tile
   const int tid = threadIdx.x;
@@ -266,15 +282,16 @@ __global__ __launch_bounds__(kPlanThreads) void chunk_plan_kernel(PlanParams p) 
   d.out = second ? p.v.wide_share : p.v.thin_share;
   const int t = tid & (kDealThreads - 1);
   unsigned long long* starts = s_starts[second];
+  int* firsts = s_firsts[second];
   // (64-bit divisions take a few microseconds here.)
   if ((unsigned long long)max(thin_units, wide_units) * p.Hkv * p.thin_groups < (1ull << 31)) {
-    deal_starts(d, p.Hkv, t, reinterpret_cast<unsigned*>(starts));
+    deal_starts(d, p.Hkv, t, reinterpret_cast<unsigned*>(starts), firsts);
     __syncthreads();
-    deal_shares(d, p.Hkv, t, reinterpret_cast<const unsigned*>(starts));
+    deal_shares(d, p.Hkv, t, reinterpret_cast<const unsigned*>(starts), firsts);
   } else {
-    deal_starts(d, p.Hkv, t, starts);
+    deal_starts(d, p.Hkv, t, starts, firsts);
     __syncthreads();
-    deal_shares(d, p.Hkv, t, static_cast<const unsigned long long*>(starts));
+    deal_shares(d, p.Hkv, t, static_cast<const unsigned long long*>(starts), firsts);
   }
   if (tid == 0) {
     ChunkHead h;
