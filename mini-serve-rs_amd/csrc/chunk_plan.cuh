@@ -86,6 +86,9 @@ struct ChunkShare {
   int end_tile, end_head, end_u, pad[13];
 };
 static_assert(sizeof(ChunkShare) == 128, "a share is a cache line");
+static_assert(offsetof(ChunkShare, first) == 16 && offsetof(ChunkShare, at) == 32 &&
+                  offsetof(ChunkShare, end_tile) == 64,
+              "the plan stores shares as fours of words");
 
 struct ChunkHead {
   uint32_t flags;  // RLSE_WS_ERR_* of this step

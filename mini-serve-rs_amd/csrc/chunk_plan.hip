@@ -1,9 +1,10 @@
 // Builds the plan of a ragged step (chunk_plan.cuh) in one launch of one
 // workgroup: a step has one plan, read by every layer, and its work -- a few
 // scans over the sequences and the wide tiles -- is bound by the launch and
-// the round trips of its dependent loads, not by bytes or operations: 7.8 us for
-// one sequence, 10 for 32, 12 for 64, 14 with 128 wide
-// tiles.
+// the round trips of its dependent loads, not by bytes or operations: 4.1 us for
+// one sequence, 5.9 for 32, 7.7 for 64, 8.0 with 128 wide tiles. (With shuffles
+// for the prefixes, a second search for each share's end and prefixes read through
+// generic addresses: 7.8, 10, 12 and 14.)
 #include "chunk_plan.h"
 
 #include "chunk_plan.cuh"
@@ -68,11 +69,18 @@ __device__ __forceinline__ void block_scan(int (&x)[N], int (*s_w)[N], int (&sum
 // Last index i of a[0..n) with a[i] <= u (a[0] = 0). The first kHeld prefixes
 // are held in LDS: a search through memory is a round trip per step.
 constexpr int kHeld = 4096;
+__device__ __forceinline__ int unit0_of(const int* held, const ChunkTile* a, int n, int i) {
+  int u = held[min(i, kHeld - 1)];
+  // (Else the two become one load from either address, slow for both.)
+  asm volatile("" : "+v"(u));
+  if (n > kHeld && i >= kHeld) u = a[i].unit0;
+  return u;
+}
 __device__ __forceinline__ int tile_of(const int* held, const ChunkTile* a, int n, int u) {
   int lo = 0, hi = n;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if ((mid < kHeld ? held[mid] : a[mid].unit0) <= u) lo = mid; else hi = mid;
+    if (unit0_of(held, a, n, mid) <= u) lo = mid; else hi = mid;
   }
   return lo;
 }
@@ -93,7 +101,8 @@ struct DealList {
   bool whole, from_end;
   ChunkShare* out;
   __device__ int unit0(int i) const {
-    return i < n ? (i < kHeld ? held[i] : tiles[i].unit0) : units;
+    const int u = unit0_of(held, tiles, n, min(i, n - 1));
+    return i < n ? u : units;
   }
 };
 template <typename I>
@@ -139,41 +148,45 @@ __device__ void deal_shares(const DealList& d, int Hkv, int t, const I* starts,
       d.out[b].count = 0;
       continue;
     }
-    ChunkShare s;
-    s.w = share_index(b, groups);
-    const I from = starts[s.w], to = starts[s.w + 1];
+    const int w = share_index(b, groups);
+    const I from = starts[w], to = starts[w + 1];
     const int units = d.units;
-    s.head = (int)(from / units);
-    const int u = (int)(from - (I)s.head * units);
-    s.tile = firsts[s.w];
-    s.end_head = (int)((to - 1) / units);
-    const I base = (I)s.end_head * units;
+    const int tile = firsts[w], after = firsts[w + 1];
+    const int end_head = (int)((to - 1) / units);
+    const I base = (I)end_head * units;
     // (The next share's tile, or the one before where that starts there.)
-    const int after = firsts[s.w + 1], end_u = (int)(to - base);
-    s.end_tile = end_u == units ? d.n - 1 : after - (d.unit0(after) == end_u);
-    s.at = d.tiles[d.from_end ? s.end_tile : s.tile];
+    const int to_u = (int)(to - base);
+    const int end_tile = to_u == units ? d.n - 1 : after - (d.unit0(after) == to_u);
+    // The tile's copy, on its way during the rest.
+    const u32x4_t* at = reinterpret_cast<const u32x4_t*>(d.tiles + (d.from_end ? end_tile : tile));
+    const u32x4_t at0 = at[0], at1 = at[1];
     auto holder = [&](I x) {  // the share that has unit x
-      int w = d.whole ? s.w : (int)(x * groups / total);
-      while (starts[w] > x) --w;
-      while (starts[w + 1] <= x) ++w;
-      return w;
+      int i = d.whole ? w : (int)(x * groups / total);
+      while (starts[i] > x) --i;
+      while (starts[i + 1] <= x) ++i;
+      return i;
     };
-    s.u0 = u - d.unit0(s.tile);
-    s.count = (int)(to - from);
-    s.first = s.u0 ? holder(from - s.u0) : s.w;
-    const I tile_end = from - s.u0 + (d.unit0(s.tile + 1) - d.unit0(s.tile));
-    s.pieces = (tile_end > to ? holder(tile_end - 1) : s.w) - s.first + 1;
-    const I end = base + d.unit0(s.end_tile + 1);
-    s.last = end > to && base + d.unit0(s.end_tile) >= from ? holder(end - 1) : s.w;
-    s.end_u = (int)(to - base - d.unit0(s.end_tile));
-    d.out[b] = s;
+    const int head = (int)(from / units), lo = d.unit0(tile);
+    const int u0 = (int)(from - (I)head * units) - lo;
+    const int first = u0 ? holder(from - u0) : w;
+    const I tile_end = from - u0 + (d.unit0(tile + 1) - lo);
+    const int pieces = (tile_end > to ? holder(tile_end - 1) : w) - first + 1;
+    const int end_lo = d.unit0(end_tile);
+    const I end = base + d.unit0(end_tile + 1);
+    const int last = end > to && base + end_lo >= from ? holder(end - 1) : w;
+    u32x4_t* out = reinterpret_cast<u32x4_t*>(d.out + b);
+    out[0] = u32x4_t{(uint32_t)w, (uint32_t)head, (uint32_t)u0, (uint32_t)(to - from)};
+    out[1] = u32x4_t{(uint32_t)first, (uint32_t)pieces, (uint32_t)last, (uint32_t)tile};
+    out[2] = at0;
+    out[3] = at1;
+    out[4] = u32x4_t{(uint32_t)end_tile, (uint32_t)end_head, (uint32_t)(to_u - end_lo), 0u};
   }
 }
 
 __global__ __launch_bounds__(kPlanThreads) void chunk_plan_kernel(PlanParams p) {
   __shared__ int s_wide[kMaxChunkSeqs + 1];  // wide tiles before each sequence
   __shared__ int s_w[kPlanWaves][5], s_w1[kPlanWaves][1];
-  __shared__ int s_thin[kHeld], s_unit[kHeld];  // unit0 of the thin and the wide tiles
+  __shared__ int s_held[2][kHeld];  // unit0 of the thin and the wide tiles
   __shared__ unsigned long long s_starts[2][kMaxShares + 1];
   __shared__ int s_firsts[2][kMaxShares + 1];
   __shared__ unsigned s_flags;
@@ -215,7 +228,7 @@ __global__ __launch_bounds__(kPlanThreads) void chunk_plan_kernel(PlanParams p) 
       const int at = x[0] + thin_tiles;
       t.unit0 = x[1] + thin_units;
       p.v.thin[at] = t;
-      if (at < kHeld) s_thin[at] = t.unit0;
+      if (at < kHeld) s_held[0][at] = t.unit0;
       atomicMax(&s_longest, t.pages);
     }
     if (wide) {
@@ -261,7 +274,7 @@ __global__ __launch_bounds__(kPlanThreads) void chunk_plan_kernel(PlanParams p) 
     wide_units += sum[0];
     if (i < wide_tiles) {
       p.v.wide[i] = t;
-      if (i < kHeld) s_unit[i] = t.unit0;
+      if (i < kHeld) s_held[1][i] = t.unit0;
     }
   }
   __syncthreads();
@@ -270,7 +283,7 @@ __global__ __launch_bounds__(kPlanThreads) void chunk_plan_kernel(PlanParams p) 
   // by the second.
   const bool second = tid >= kDealThreads;
   DealList d;
-  d.held = second ? s_unit : s_thin;
+  d.held = s_held[second];
   d.tiles = second ? p.v.wide : p.v.thin;
   d.n = second ? wide_tiles : thin_tiles;
   d.units = second ? wide_units : thin_units;

@@ -1,6 +1,7 @@
 """Attention of ragged steps (rlse_chunk_plan, rlse_chunk_attn) against its
 definition in 64 bits: decode steps, drafts and prompt chunks, windows and
 sinks, and what masked places, pages and rows may hold."""
+import copy
 import math
 
 import pytest
@@ -417,3 +418,89 @@ def test_a_value_of_little_weight_still_reaches_its_rows(kv, new, dtype):
     out, lse = step.run(kv)
     assert_within(out, want, tol, "out")
     assert_within(lse, wlse, ltol, "lse")
+
+
+@pytest.mark.parametrize("window", [(0, 0), (300, 5)])
+def test_more_tiles_than_the_plan_holds_on_chip(kv, window):
+    """5000 tokens of 256 heads that share one KV head: a tile a token. Four of
+    the heads are compared."""
+    step = Step(30, "bf16", (256, 1, 64), [4300, 700], [0, 40], *window).upload().plan(kv)
+    out, lse = step.run(kv)
+    torch.cuda.synchronize()
+    kv.workspace_check(step.dev["plan"])
+    some = [0, 1, 100, 255]
+    part = copy.copy(step)
+    part.hq, part.q = len(some), step.q[:, some]
+    want, wlse, tol, ltol = part.attention()
+    assert_within(out[:, some], want, tol, "out")
+    assert_within(lse[:, some], wlse, ltol, "lse")
+    weights = torch.zeros(2, 1, step.mbps * 16, device=DEV)
+    d = step.dev
+    kv.kv_scores(d["q"], d["k"], d["tables"], d["plan"], lse, None, weights, *step.shape())
+    # every query gives one in all
+    for b in range(2):
+        given = float(weights[b].double().sum())
+        assert abs(given - 256 * step.new[b]) <= 1e-4 * 256 * step.new[b]
+
+
+def test_two_calls_at_once(kv):
+    """One plan, two layers' calls on two streams, each with a workspace."""
+    step = Step(31, "bf16", (28, 4, 128), [150, 1, 90, 1, 260], [100, 2500, 0, 4000, 700])
+    step.upload().plan(kv)
+    want = [t.clone() for t in step.run(kv)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    spaces = [step.workspace(kv) for _ in streams]
+    outs = [(torch.full_like(want[0], 7.0), torch.full_like(want[1], 7.0)) for _ in streams]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for st, ws, (out, lse) in zip(streams, spaces, outs):
+            with torch.cuda.stream(st):
+                step.run(kv, ws, out, lse, st)
+    torch.cuda.synchronize()
+    for out, lse in outs:
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+
+
+def test_a_captured_step_follows_its_lengths(kv):
+    """Plan, attention and key weights captured once; every replay attends what
+    the lengths say then, from no new token to all of them."""
+    step = Step(32, "f16", (16, 8, 128), [3, 1, 40], [300, 50, 200], 64, 4).upload().plan(kv)
+    d, ws = step.dev, step.workspace(kv)
+    out, lse = torch.empty_like(d["q"]), torch.empty(step.total, step.hq, device=DEV)
+    acc = torch.empty(step.n, step.hkv, step.mbps * 16, device=DEV)
+    st = torch.cuda.Stream()
+
+    def all_of_it(stream=None):
+        step.build(kv, stream)
+        step.run(kv, ws, out, lse, stream)
+        kv.kv_scores(d["q"], d["k"], d["tables"], d["plan"], lse, None, acc, *step.shape(),
+                     stream)
+
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        all_of_it(st)
+    for new, cached in [([3, 1, 40], [300, 50, 200]), ([0, 0, 40], [300, 51, 10]),
+                        ([3, 0, 0], [0, 9, 5]), ([0, 0, 0], [1, 1, 1]), ([1, 1, 1], [299, 50, 239])]:
+        cu = [0, new[0], new[0] + new[1], sum(new)]
+        d["cu"].copy_(torch.tensor(cu, dtype=torch.int32))
+        d["lens"].copy_(torch.tensor([a + b for a, b in zip(new, cached)], dtype=torch.int32))
+        results = []
+        for call in (graph.replay, all_of_it):
+            for t in (out, lse, acc):
+                t.fill_(7)
+            call()
+            torch.cuda.synchronize()
+            kv.workspace_check(d["plan"])
+            results.append([t.clone() for t in (out, lse, acc)])
+        for a, b in zip(*results):
+            assert torch.equal(a, b)
+        assert (results[0][0][sum(new):] == 7).all()
+        now = copy.copy(step)
+        now.new, now.cached, now.cu = new, cached, cu
+        now.lens = [a + b for a, b in zip(new, cached)]
+        want, wlse, tol, ltol = now.attention()
+        rows = slice(0, sum(new))
+        assert_within(results[0][0][rows], want[rows], tol[rows], f"{new} out")
+        assert_within(results[0][1][rows], wlse[rows], ltol[rows], f"{new} lse")
