@@ -234,6 +234,22 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictParams p,
     }
 }
 
+// Whether a layer of a and one of b, `bytes` each and `stride` bytes apart, share
+// a byte. (Two sets of weights may lie between each other, layer by layer.)
+bool layers_overlap(const void* a, const void* b, int layers, long long stride, long long bytes) {
+  const long long delta = (long long)(reinterpret_cast<uintptr_t>(b) -
+                                      reinterpret_cast<uintptr_t>(a));
+  if (layers == 1) return delta < bytes && delta > -bytes;
+  // The whole strides next below and above their distance.
+  long long k = delta / stride;
+  if (delta < k * stride) --k;
+  for (int i = 0; i < 2; ++i, ++k) {
+    const long long off = delta - k * stride;
+    if (k < layers && k > -layers && off < bytes && off > -bytes) return true;
+  }
+  return false;
+}
+
 template <int PPR>
 int launch_evict(const EvictParams& p, int heads, hipStream_t stream) {
   hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)heads), dim3(kSelectThreads), 0, stream,
@@ -290,9 +306,7 @@ extern "C" int rlse_kv_evict(void* k_pool, void* v_pool, long long layer_stride_
   if (!k_pool || !v_pool || !block_tables || !seq_lens || !scores || !new_tables || !new_lens ||
       !new_scores || !keep)
     return fail(RLSE_ERR_INVALID_VALUE, "kv_evict: null pointer argument");
-  const size_t sbytes =
-      (num_layers > 1 ? (size_t)(num_layers - 1) * score_layer_stride + row : (size_t)row) * 4;
-  if (overlap(scores, sbytes, new_scores, sbytes))
+  if (layers_overlap(scores, new_scores, num_layers, score_layer_stride * 4, row * 4))
     return fail(RLSE_ERR_INVALID_VALUE, "kv_evict: new_scores overlaps scores");
   if (overlap(seq_lens, (size_t)num_seqs * 4, new_lens, (size_t)num_seqs * 4))
     return fail(RLSE_ERR_INVALID_VALUE, "kv_evict: new_lens overlaps seq_lens");

@@ -109,3 +109,17 @@ def test_overlaps_name_their_reason(kv):
     for prev in (4092, 4100, 4096 + 4 * GOOD["n"] * GOOD["hkv"] * GOOD["mbps"] * 16 - 4):
         assert _scores(kv, **{**GOOD, "prev": prev}) == kv.ERR_INVALID_VALUE
         assert "prev overlaps" in kv.last_error()
+
+
+def test_layers_of_weights_that_meet(kv):
+    """Two layers of 2048 floats 5000 apart: refused where one of the new ones
+    meets one of the old ones."""
+    row, stride = 4 * 2 * 8 * 128, 4 * 5000
+    base = 1 << 20
+    for at in (0, row - 4, stride, stride - row + 4, stride + row - 4, -stride, -4, 4 - row):
+        _evict(kv, **{**EVICT, "scores": base, "sstride": 5000, "new": base + at})
+        assert "new_scores overlaps" in kv.last_error(), at
+    for at in (row, stride - row, -row, 2 * stride, -2 * stride):
+        _evict(kv, **{**EVICT, "scores": base, "sstride": 5000, "new": base + at, "lens": 16,
+                      "nlens": 16})
+        assert "new_lens overlaps" in kv.last_error(), at

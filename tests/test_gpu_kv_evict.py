@@ -189,3 +189,17 @@ def test_pool_offsets_past_32_bits(kv):
     torch.cuda.synchronize()
     c.dev["pool"] = big[:, :, first:].clone()
     c.check(kept)
+
+
+def test_weights_between_each_other(kv):
+    """Old and new weights in one buffer, layer by layer."""
+    c = Cache(48, "bf16", 3, 2, 64, [200, 90], 50, 2, 10).upload()
+    both = torch.full((3, 2) + tuple(c.scores.shape[1:]), -5.0, device=DEV)
+    both[:, 0] = c.dev["scores"]
+    d = c.dev
+    kv.kv_evict(d["pool"][0, 0], d["pool"][0, 1], d["pool"][0].numel(), 3, d["tables"], d["lens"],
+                both[0, 0], both[0].numel(), d["new_tables"], d["new_lens"], both[0, 1],
+                d["keep"], c.n, c.hkv, c.d, c.mbps, c.nbps, c.nb, c.budget, c.sinks, c.recent,
+                c.dtype)
+    d["scores"], d["new_scores"] = both[:, 0].contiguous(), both[:, 1].contiguous()
+    c.check()
